@@ -4,7 +4,8 @@ ARCH  ?= gfx950
 CSRC  := mpnn_amd/csrc
 OUT   := mpnn_amd/libmpnn_hip.so
 HIPFLAGS := -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -Iinclude -I$(CSRC) -Wno-unused-result $(EXTRA)
-OBJS  := $(CSRC)/mpnn_featurizer.o $(CSRC)/mpnn_edge.o $(CSRC)/mpnn_edge_bwd.o $(CSRC)/mpnn_node.o $(CSRC)/mpnn_node_bwd.o $(CSRC)/mpnn_data.o $(CSRC)/mpnn_loss.o $(CSRC)/mpnn_abi.o \
+NOPACK := -Xclang -target-feature -Xclang -packed-fp32-ops
+OBJS  := $(CSRC)/mpnn_featurizer.o $(CSRC)/mpnn_edge.o $(CSRC)/mpnn_edge_bwd.o $(CSRC)/mpnn_node.o $(CSRC)/mpnn_node_bwd.o $(CSRC)/mpnn_data.o $(CSRC)/mpnn_loss.o $(CSRC)/mpnn_beam.o $(CSRC)/mpnn_abi.o \
          $(CSRC)/mpnn_featurizer_f16.o $(CSRC)/mpnn_edge_f16.o $(CSRC)/mpnn_node_f16.o
 
 all: $(OUT)
@@ -29,6 +30,10 @@ $(CSRC)/mpnn_data.o: $(CSRC)/mpnn_data.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_ab
 
 $(CSRC)/mpnn_loss.o: $(CSRC)/mpnn_loss.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_ablation.h
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
+
+# -packed-fp32-ops: no v_pk_*_f32 (some of their forms gave wrong results on this hardware)
+$(CSRC)/mpnn_beam.o: $(CSRC)/mpnn_beam.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_ablation.h include/mpnn_hip.h
+	$(HIPCC) $(HIPFLAGS) $(NOPACK) -ffp-contract=off -c $< -o $@
 
 $(OUT): $(OBJS)
 	$(HIPCC) -shared -fPIC --offload-arch=$(ARCH) $(OBJS) -o $@

@@ -727,6 +727,50 @@ int mpnn_assemble_batch_ordered(const float* X_cat, const uint8_t* S_cat, const 
  * elsewhere (padding included). */
 int mpnn_mask_self(const int64_t* chain_encoding_all, int B, int L, float* mask_self, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Beam search (no counterpart in the reference, which has no decoding loop): the choice of the next hypotheses and the
+ * beams' states following it.  Used by the Python package's beam_select / beam_reorder and ProteinMPNN.beam_search.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/* One step of beam search for n_groups groups of n_beams hypotheses over n_tokens tokens:
+ *   x[b][w][v] = logits + bias (a token whose bias is -inf is out, whatever its logit holds)
+ *   c[b][w][v] = scores[b][w] + x[b][w][v] - log sum_u exp x[b][w][u]
+ * and of each group's n_beams * n_tokens candidates the n_out best, best first, ties to the lowest beam and then the lowest
+ * token: out_scores (fp32, rounded once from fp64), parent (the beam) and token, each [n_groups][n_out].
+ *   logits     dtype 0 fp32, 1 bf16, 2 fp16; element (b, w, v) at b * stride_group + w * stride_beam + v (strides in
+ *              elements, any value)
+ *   scores     [n_groups][n_beams] fp32; -inf = no hypothesis there
+ *   bias       NULL or fp32, element (b, w, v) at b * bias_group + w * bias_beam + v (0 strides broadcast)
+ *   forced     NULL or [n_groups][n_beams]: a beam with forced >= 0 offers that token alone (at most n_tokens - 1), at its
+ *              own score: finished hypotheses, positions whose token is given
+ * A slot that no candidate is left for gets the score -inf and keeps its beam: parent = slot % n_beams, token = that
+ * beam's forced token or 0.  A beam with NaN or +inf among its logits that are not out, or in its score, offers one
+ * candidate: token 0, score NaN, ranked first.  Outputs are fully determined by the inputs (no atomics decide anything).
+ * n_beams, n_out <= 256, n_tokens <= 2^22.  workspace: mpnn_beam_select_workspace bytes (0: none needed), 16-byte
+ * aligned, overwritten; calls that may overlap need one each.  The outputs may not overlap the inputs. */
+int mpnn_beam_select(const void* logits, int dtype, long long stride_group, long long stride_beam, const float* scores,
+                     const float* bias, long long bias_group, long long bias_beam, const int64_t* forced, int n_groups,
+                     int n_beams, int n_tokens, int n_out, float* out_scores, int64_t* parent, int64_t* token,
+                     void* workspace, long long workspace_bytes, void* stream);
+long long mpnn_beam_select_workspace(int dtype, int n_groups, int n_beams, int n_tokens, int n_out);
+
+/* One state tensor of mpnn_beam_reorder (HOST struct; strides and run in BYTES): element (group, beam, m, r) at
+ * data + group * stride_group + beam * stride_beam + m * stride_mid + r, m < n_mid, r < run. */
+typedef struct mpnn_beam_state {
+  void* data;
+  long long stride_group, stride_beam, stride_mid;
+  long long run;
+  int n_mid;
+} mpnn_beam_state;
+
+/* states[i][b][j] <- states[i][b][parent[b][j]] for all n states (HOST array), in place; parent [n_groups][n_beams].  A
+ * parent outside [0, n_beams) leaves its row as it is.  With a length - length [n_groups] on the device, or length_all >= 0
+ * for all groups - only the positions m with rank[b][m] < length move (rank [n_groups][n_mid]; NULL: rank = m), and n_mid
+ * is the number of positions of every state; the other positions are not touched.  No two states (and no two rows of one)
+ * may share memory.  At most 256 beams and 65535 groups. */
+int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int64_t* parent, int n_groups, int n_beams,
+                      int length_all, const int32_t* length, const int32_t* rank, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,7 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 
 _U64 = ctypes.c_uint64
+_L = ctypes.c_longlong
 
 
 class LevelLayer(ctypes.Structure):
@@ -29,6 +30,11 @@ class LevelLayer(ctypes.Structure):
                 ("W3_packed", _P), ("b3", _P), ("ln1_w", _P), ("ln1_b", _P), ("Win_packed", _P), ("b_in", _P),
                 ("Wout8_packed", _P), ("b_out", _P), ("ln2_w", _P), ("ln2_b", _P), ("scale", _F),
                 ("Wproj_packed", _P), ("bproj", _P), ("nproj", _I), ("hV_out", _P), ("PQ", _P)]
+
+
+class BeamState(ctypes.Structure):
+    """mpnn_beam_state (include/mpnn_hip.h): one state tensor of mpnn_beam_reorder."""
+    _fields_ = [("data", _P), ("stride_group", _L), ("stride_beam", _L), ("stride_mid", _L), ("run", _L), ("n_mid", _I)]
 
 
 # name -> argtypes (all return int except where noted)
@@ -101,6 +107,8 @@ SIGNATURES = {
     "mpnn_grad_sumsq": [_I, _P, _P, _P, _P, _I, _P],
     "mpnn_grad_scale": [_I, _P, _P, _P, _F, _P],
     "mpnn_adamw_step": [_I, _P, _P, _P, _P, _P, _F, _F, _F, _F, _F, _I, _P, _F, _P],
+    "mpnn_beam_select": [_P, _I, _L, _L, _P, _P, _L, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P],
+    "mpnn_beam_reorder": [_I, ctypes.POINTER(BeamState), _P, _I, _I, _I, _P, _P, _P],
     "mpnn_linear_rows": [_P, _I, _I, _P, _P, ctypes.c_longlong, _P, _P],
     "mpnn_probe_elementwise": [_P, _I, _I, _P, _P],
     "mpnn_range_flag": [_P, ctypes.c_longlong, _F, _P, _I, _P],
@@ -161,6 +169,8 @@ def load() -> ctypes.CDLL:
     lib.mpnn_version.argtypes = []
     lib.mpnn_workspace_bytes.restype = ctypes.c_longlong
     lib.mpnn_workspace_bytes.argtypes = [ctypes.c_char_p, _I, _I]
+    lib.mpnn_beam_select_workspace.restype = _L
+    lib.mpnn_beam_select_workspace.argtypes = [_I] * 5
     lib.mpnn_last_error.restype = ctypes.c_char_p
     lib.mpnn_last_error.argtypes = []
     lib.mpnn_ablation_build.restype = _I

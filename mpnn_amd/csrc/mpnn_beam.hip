@@ -1,0 +1,689 @@
+// Beam search: the choice of the next hypotheses over beams x vocabulary, and the beams' states following it.
+//
+//   mpnn_beam_select   c[w][v] = score[w] + x[w][v] - log sum_u exp x[w][u],  x = logits + bias;  the best n_out of a
+//                      group's W V candidates, ties to the lowest beam, then the lowest token
+//   mpnn_beam_reorder  x[b][j] <- x[b][parent[b][j]] for several state tensors, in place
+//
+// The choice compares candidates of different beams, whose scores lie close together: the log-sum-exp and the candidates
+// are held in fp64 (CDNA's fp64 vector rate is its fp32 rate without packed instructions), so that the order does not
+// hang on the order of a sum.  Only the scores handed back are rounded, to fp32.
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "mpnn_common.h"
+#include "mpnn_hip.h"
+
+namespace {
+
+constexpr int SEL_MAX_N = 256;       // hypotheses kept of a group
+constexpr int SEL_CAP = 1024;        // candidates a workgroup ranks in LDS
+constexpr long long KEY_NONE = (long long)0x8000000000000000ull;  // below every candidate
+constexpr long long KEY_NAN = 0x7fffffffffffffffll;               // NaN ranks first: a broken beam shows at once
+
+// ---- order of candidates: signed 64-bit keys that sort like the values (-0 as +0) ----
+__device__ __forceinline__ long long key_of(double c) {
+  if (c != c) return KEY_NAN;
+  const long long b = __double_as_longlong(c + 0.0);
+  return b ^ ((b >> 63) & 0x7fffffffffffffffll);
+}
+__device__ __forceinline__ double value_of(long long k) {
+  return k == KEY_NAN ? __longlong_as_double(0x7ff8000000000000ll) : __longlong_as_double(k ^ ((k >> 63) & 0x7fffffffffffffffll));
+}
+__device__ __forceinline__ bool better(long long ka, int ia, long long kb, int ib) { return ka > kb || (ka == kb && ia < ib); }
+
+// A NaN or +inf among a beam's logits makes its log-sum-exp NaN; so may its score be NaN or +inf.  Such a beam offers one
+// candidate, token 0 with the score NaN: the failure stands in the first slot and takes no more than one.
+__device__ __forceinline__ bool broken(double score, double lse) { return lse != lse || !(score < INFINITY); }
+
+// exp(d) for d <= 0 to 1.1e-12 relative (2^f by a degree-8 polynomial, tools/fit_exp2.py; exactly 1 at 0); NaN stays NaN
+__device__ __forceinline__ double exp_neg(double d) {
+  d = d < -800.0 ? -800.0 : d;
+  const double t = d * 1.4426950408889634, n = rint(t), f = t - n;
+  double p = 1.32552248847991267e-06;
+  p = fma(p, f, 1.53100794023831035e-05);
+  p = fma(p, f, 1.54034558524190164e-04);
+  p = fma(p, f, 1.33334505680000079e-03);
+  p = fma(p, f, 9.61812915940261914e-03);
+  p = fma(p, f, 5.55041094120593409e-02);
+  p = fma(p, f, 2.40226506958129887e-01);
+  p = fma(p, f, 6.93147180545933494e-01);
+  p = fma(p, f, 1.0);
+  return ldexp(p, (int)n);
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f(T x) { return (float)x; }
+template <>
+__device__ __forceinline__ float to_f<__hip_bfloat16>(__hip_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
+
+__device__ __forceinline__ double shfl_xor_d(double v, int o) { return __shfl_xor(v, o); }
+
+// the largest T for which at least q lanes have u >= T, or one that exactly q lanes reach (uniform result)
+__device__ __forceinline__ unsigned wave_kth(unsigned u, int q) {
+  unsigned T = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const unsigned t = T | (1u << bit);
+    const int cnt = __popcll(__ballot(u >= t));
+    if (cnt >= q) {
+      T = t;
+      if (cnt == q) break;
+    }
+  }
+  return T;
+}
+
+// a bound that the n-th best of a 256-thread workgroup's values is no worse than, from each thread's best (u, 0 = none):
+// the least of the waves' ceil(n / 4)-th best threads, or the best of the waves' n-th best ones.  ru: 8 words of LDS,
+// written here; the caller's barrier follows, then block_bound reads them.
+__device__ __forceinline__ void wave_bounds(unsigned u, int n, unsigned* ru) {
+  const unsigned q = wave_kth(u, (n + 3) / 4), all = n <= 64 ? wave_kth(u, n) : 0;
+  if ((threadIdx.x & 63) == 0) {
+    ru[threadIdx.x >> 6] = q;
+    ru[4 + (threadIdx.x >> 6)] = all;
+  }
+}
+__device__ __forceinline__ unsigned block_bound(const unsigned* ru) {
+  const unsigned lo01 = ru[0] < ru[1] ? ru[0] : ru[1], lo23 = ru[2] < ru[3] ? ru[2] : ru[3], lo = lo01 < lo23 ? lo01 : lo23;
+  unsigned hi = ru[4];
+#pragma unroll
+  for (int i = 5; i < 8; ++i) hi = ru[i] > hi ? ru[i] : hi;
+  return lo > hi ? lo : hi;
+}
+
+struct SelectArgs {
+  const void* logits;
+  long long sb, sw;          // strides of a group and of a beam, in elements
+  const float* scores;       // [B][W]
+  const float* bias;         // NULL or element (b, w, v) at bias[b * bb + w * bw + v]
+  long long bb, bw;
+  const long long* forced;   // NULL or [B][W]; negative = free
+  int B, W, V, n;
+  float* out_scores;
+  long long* parent;
+  long long* token;
+};
+
+__device__ __forceinline__ void write_slot(const SelectArgs& a, int b, int slot, long long key, int flat) {
+  const long long o = (long long)b * a.n + slot;
+  a.out_scores[o] = (float)value_of(key);
+  a.parent[o] = flat / a.V;
+  a.token[o] = flat % a.V;
+}
+// a slot that no candidate is left for keeps its beam: nothing has to move for it
+__device__ __forceinline__ void write_dead_slot(const SelectArgs& a, int b, int slot) {
+  const long long o = (long long)b * a.n + slot;
+  const int w = slot % a.W;
+  const long long f = a.forced ? a.forced[(long long)b * a.W + w] : -1;
+  a.out_scores[o] = -INFINITY;
+  a.parent[o] = w;
+  a.token[o] = f < 0 ? 0 : (f < a.V ? f : a.V - 1);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Small groups: one wave holds all W V candidates of a group in registers (M per lane).  Lanes are split into W
+// subgroups of g = 64 / (W rounded up to a power of two); lane j of a subgroup has tokens j, j + g, ...  No LDS
+// exchange before the winners are ranked, no barrier: at the model's 21 letters the call is bound by its own latency.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int M>
+__global__ void __launch_bounds__(64)
+k_select_small(SelectArgs a, int g_log2) {
+  __shared__ long long lk[SEL_MAX_N];
+  __shared__ int li[SEL_MAX_N];
+  const int b = blockIdx.x, lane = threadIdx.x, g = 1 << g_log2;
+  const int w = lane >> g_log2, j = lane & (g - 1);
+  const bool live = w < a.W;
+  const double s = live ? (double)a.scores[(long long)b * a.W + w] : 0.0;
+  const long long f = live && a.forced ? a.forced[(long long)b * a.W + w] : -1;
+  double x[M];
+  double top = -INFINITY;
+  {
+    const T* row = (const T*)a.logits + (long long)b * a.sb + (long long)w * a.sw;
+    const float* bias = a.bias ? a.bias + (long long)b * a.bb + (long long)w * a.bw : nullptr;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const int v = j + (i << g_log2);
+      x[i] = -INFINITY;
+      if (live && v < a.V) {
+        x[i] = (double)to_f(row[v]);
+        if (bias) {
+          const float add = bias[v];
+          x[i] = add == -INFINITY ? -INFINITY : x[i] + (double)add;
+        }
+      }
+      top = fmax(top, x[i]);
+    }
+  }
+  for (int o = 1; o < g; o <<= 1) top = fmax(top, shfl_xor_d(top, o));
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < M; ++i) sum += x[i] == -INFINITY ? 0.0 : exp_neg(x[i] - top);
+  for (int o = 1; o < g; o <<= 1) sum += shfl_xor_d(sum, o);
+  const double lse = top + log(sum);   // nothing left of the row: no candidate below
+  const bool bad = broken(s, lse);
+  long long k[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    const int v = j + (i << g_log2);
+    double c = x[i] == -INFINITY ? -INFINITY : s + (x[i] - lse);
+    if (bad) c = v == 0 ? (double)NAN : -INFINITY;
+    if (f >= 0) c = v == (int)(f < a.V ? f : a.V - 1) ? s : -INFINITY;
+    k[i] = live && v < a.V && !(c == -INFINITY) ? key_of(c) : KEY_NONE;
+  }
+  // the n best: bisection over the keys' high words, then, where candidates tie there, their low words and places
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < M; ++i) total += __popcll(__ballot(k[i] != KEY_NONE));
+  const int n = total < a.n ? total : a.n;
+  unsigned long long cut = 1;            // as unsigned words: KEY_NONE is 0
+  int last = 0x7fffffff;               // of the candidates that equal cut, those up to this place
+  if (total > n) {
+    cut = 0;
+    int cnt = total;
+    for (int bit = 63; bit >= 0 && cnt != n; --bit) {
+      const unsigned long long t = cut | (1ull << bit);
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < M; ++i) c += __popcll(__ballot(((unsigned long long)k[i] ^ (unsigned long long)KEY_NONE) >= t));
+      if (c >= n) {
+        cut = t;
+        cnt = c;
+      }
+    }
+    if (cnt > n) {                      // equal candidates: the lowest places of them
+      int above = 0;
+#pragma unroll
+      for (int i = 0; i < M; ++i) above += __popcll(__ballot(((unsigned long long)k[i] ^ (unsigned long long)KEY_NONE) > cut));
+      int lo = 0, hi = a.W * a.V - 1;   // the smallest place p with above + #(equal, place <= p) >= n
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        int c = above;
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+          c += __popcll(__ballot(((unsigned long long)k[i] ^ (unsigned long long)KEY_NONE) == cut &&
+                                 w * a.V + j + (i << g_log2) <= mid));
+        if (c >= n) hi = mid; else lo = mid + 1;
+      }
+      last = lo;
+    }
+  }
+  int at = 0;
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    const unsigned long long u = (unsigned long long)k[i] ^ (unsigned long long)KEY_NONE;
+    const int place = w * a.V + j + (i << g_log2);
+    const bool in = u > cut || (u == cut && place <= last);
+    const unsigned long long m = __ballot(in);
+    if (in) {
+      const int p = at + __popcll(m & ((1ull << lane) - 1));
+      lk[p] = k[i];
+      li[p] = place;
+    }
+    at += __popcll(m);
+  }
+  __syncthreads();
+  for (int e = lane; e < n; e += 64) {
+    const long long ke = lk[e];
+    const int ie = li[e];
+    int r = 0;
+    for (int q = 0; q < n; ++q) r += better(lk[q], li[q], ke, ie);
+    write_slot(a, b, r, ke, ie);
+  }
+  for (int e = n + lane; e < a.n; e += 64) write_dead_slot(a, b, e);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Large vocabularies, first pass: a workgroup reads a slice of 256 U logits of one beam once, keeps it in registers,
+// and leaves the slice's maximum, its sum of exponentials and its n best logits.
+// ---------------------------------------------------------------------------------------------------------------
+struct SlicePart {
+  double top, sum;
+};
+
+// rank the `cnt` <= SEL_CAP collected candidates and hand the n best to put(slot, key, place)
+template <typename Put>
+__device__ __forceinline__ void rank_collected(const long long* lk, const int* li, int cnt, int n, Put put) {
+  for (int e = threadIdx.x; e < cnt; e += 256) {
+    const long long ke = lk[e];
+    const int ie = li[e];
+    int r = 0;
+    for (int q = 0; q < cnt; ++q) r += better(lk[q], li[q], ke, ie);
+    if (r < n) put(r, ke, ie);
+  }
+}
+
+// best of the workgroup's (key, place) pairs; every thread gets it
+__device__ __forceinline__ void block_best(long long& k, int& p, long long* sk, int* sp) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const long long ok = __shfl_xor(k, o);
+    const int op = __shfl_xor(p, o);
+    if (better(ok, op, k, p)) { k = ok; p = op; }
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) { sk[threadIdx.x >> 6] = k; sp[threadIdx.x >> 6] = p; }
+  __syncthreads();
+  k = sk[0];
+  p = sp[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i)
+    if (better(sk[i], sp[i], k, p)) { k = sk[i]; p = sp[i]; }
+}
+
+template <typename T, int U, bool BIAS>
+__global__ void __launch_bounds__(256)
+k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long* __restrict__ pk, int* __restrict__ pi) {
+  __shared__ double rd[4];
+  __shared__ unsigned ru[8];
+  __shared__ int rc;
+  __shared__ long long lk[SEL_CAP];
+  __shared__ int li[SEL_CAP];
+  constexpr int VE = 16 / (int)sizeof(T);   // elements of a 16-byte load
+  const int row = blockIdx.x / splits, split = blockIdx.x % splits;
+  const int b = row / a.W, w = row % a.W, tid = threadIdx.x, wave = tid >> 6;
+  SlicePart* my = part + blockIdx.x;
+  pk += (long long)blockIdx.x * a.n;
+  pi += (long long)blockIdx.x * a.n;
+  if (a.forced && a.forced[row] >= 0) return;     // the second pass knows the row's one candidate
+  const T* lrow = (const T*)a.logits + (long long)b * a.sb + (long long)w * a.sw;
+  const float* brow = BIAS ? a.bias + (long long)b * a.bb + (long long)w * a.bw : nullptr;
+  // slices begin at multiples of 16 bytes of memory, not of the row: every full load is aligned
+  const int mis = (int)(((uintptr_t)lrow & 15) / sizeof(T));
+  const int base = split * (256 * U) - mis;
+  typedef typename std::conditional<BIAS, double, float>::type X;
+  X x[U];
+#pragma unroll
+  for (int it = 0; it < U / VE; ++it) {
+    const int e0 = base + (it * 256 + tid) * VE;
+    T raw[VE];
+    if (e0 >= 0 && e0 + VE <= a.V) {
+      __builtin_memcpy(raw, __builtin_assume_aligned(lrow + e0, 16), 16);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) x[it * VE + i] = (X)to_f(raw[i]);
+      if (BIAS) {
+        float add[VE];
+        __builtin_memcpy(add, brow + e0, 4 * VE);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) x[it * VE + i] = add[i] == -INFINITY ? (X)-INFINITY : x[it * VE + i] + (X)add[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const int e = e0 + i;
+        x[it * VE + i] = (X)-INFINITY;
+        if (e >= 0 && e < a.V) {
+          x[it * VE + i] = (X)to_f(lrow[e]);
+          if (BIAS) x[it * VE + i] = brow[e] == -INFINITY ? (X)-INFINITY : x[it * VE + i] + (X)brow[e];
+        }
+      }
+    }
+  }
+  // maximum, and the sum relative to it
+  X tmax = (X)-INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    tmax = x[i] > tmax ? x[i] : tmax;
+    nan |= x[i] != x[i];
+  }
+  double top = (double)tmax;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) top = fmax(top, shfl_xor_d(top, o));
+  const long long kt = nan ? KEY_NAN : key_of((double)tmax);
+  wave_bounds((unsigned)(kt >> 32) ^ 0x80000000u, a.n, ru);
+  if ((tid & 63) == 0) rd[wave] = top;
+  if (tid == 0) rc = 0;
+  __syncthreads();
+  top = fmax(fmax(rd[0], rd[1]), fmax(rd[2], rd[3]));
+  const unsigned cut = block_bound(ru);
+  double sum = nan ? (double)NAN : 0.0;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const double xi = (double)x[i];
+    sum += xi == -INFINITY ? 0.0 : exp_neg(xi - top);
+    const long long k = key_of(xi);
+    if (xi != -INFINITY && ((unsigned)(k >> 32) ^ 0x80000000u) >= cut) {
+      const int p = atomicAdd(&rc, 1);
+      if (p < SEL_CAP) {
+        lk[p] = k;
+        li[p] = base + (i / VE * 256 + tid) * VE + i % VE;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) sum += shfl_xor_d(sum, o);
+  __syncthreads();                     // rd has been read, the list is complete
+  if ((tid & 63) == 0) rd[wave] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    my->top = top;
+    my->sum = (rd[0] + rd[1]) + (rd[2] + rd[3]);
+  }
+  const int cnt = rc;
+  if (cnt <= SEL_CAP) {
+    rank_collected(lk, li, cnt, a.n, [&](int r, long long k, int p) { pk[r] = k; pi[r] = p; });
+    for (int r = cnt + tid; r < a.n; r += 256) pk[r] = KEY_NONE;
+    return;
+  }
+  // more ties than the list holds (constant logits): one after the other
+  long long prev = KEY_NAN;
+  int place = -1;
+  __shared__ long long sk[4];
+  __shared__ int sp[4];
+  for (int r = 0; r < a.n; ++r) {
+    long long k = KEY_NONE;
+    int p = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const double xi = (double)x[i];
+      const long long ki = xi == -INFINITY ? KEY_NONE : key_of(xi);
+      const int q = base + (i / VE * 256 + tid) * VE + i % VE;
+      if (ki != KEY_NONE && better(prev, place, ki, q) && better(ki, q, k, p)) { k = ki; p = q; }
+    }
+    block_best(k, p, sk, sp);
+    if (tid == 0) { pk[r] = k; pi[r] = p; }
+    prev = k;
+    place = p;
+  }
+}
+
+// Second pass, one workgroup a group: the beams' log-sum-exps from the slices', then the n best of the slices' lists.
+__global__ void __launch_bounds__(256)
+k_select_merge(SelectArgs a, int splits, const SlicePart* __restrict__ part, const long long* __restrict__ pk,
+               const int* __restrict__ pi) {
+  __shared__ double lse[SEL_MAX_N];
+  __shared__ float sc[SEL_MAX_N];
+  __shared__ int fc[SEL_MAX_N];
+  __shared__ unsigned ru[8];
+  __shared__ int rc;
+  __shared__ long long lk[SEL_CAP];
+  __shared__ int li[SEL_CAP];
+  const int b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  for (int w = wave; w < a.W; w += 4) {
+    const long long row = (long long)b * a.W + w;
+    const long long f = a.forced ? a.forced[row] : -1;
+    if (f < 0) {
+      const SlicePart* p = part + row * splits;
+      double top = -INFINITY, sum = 0.0;
+      for (int i = lane; i < splits; i += 64) top = fmax(top, p[i].top);
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) top = fmax(top, shfl_xor_d(top, o));
+      for (int i = lane; i < splits; i += 64) sum += p[i].top == -INFINITY ? p[i].sum : p[i].sum * exp(p[i].top - top);
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) sum += shfl_xor_d(sum, o);
+      if (lane == 0) lse[w] = top + log(sum);
+    }
+    if (lane == 0) {
+      sc[w] = a.scores[row];
+      fc[w] = f < 0 ? -1 : (f < a.V ? (int)f : a.V - 1);
+    }
+  }
+  if (tid == 0) rc = 0;
+  __syncthreads();
+  const int per = splits * a.n, total = a.W * per;
+  auto candidate = [&](int e, long long& k, int& p) {
+    const int w = e / per, r = e - w * per;
+    k = KEY_NONE;
+    p = 0;
+    if (fc[w] >= 0) {
+      if (r == 0 && !(sc[w] == -INFINITY)) { k = key_of((double)sc[w]); p = w * a.V + fc[w]; }
+      return;
+    }
+    if (broken((double)sc[w], lse[w])) {
+      if (r == 0) { k = KEY_NAN; p = w * a.V; }
+      return;
+    }
+    const long long at = (long long)b * total + e, kx = pk[at];
+    if (kx == KEY_NONE) return;
+    const double c = (double)sc[w] + (value_of(kx) - lse[w]);
+    if (c == -INFINITY) return;
+    k = key_of(c);
+    p = w * a.V + pi[at];
+  };
+  long long best = KEY_NONE;
+  for (int e = tid; e < total; e += 256) {
+    long long k;
+    int p;
+    candidate(e, k, p);
+    best = k > best ? k : best;
+  }
+  wave_bounds((unsigned)(best >> 32) ^ 0x80000000u, a.n, ru);
+  __syncthreads();
+  const unsigned T = block_bound(ru);
+  for (int e = tid; e < total; e += 256) {
+    long long k;
+    int p;
+    candidate(e, k, p);
+    if (k != KEY_NONE && ((unsigned)(k >> 32) ^ 0x80000000u) >= T) {
+      const int q = atomicAdd(&rc, 1);
+      if (q < SEL_CAP) { lk[q] = k; li[q] = p; }
+    }
+  }
+  __syncthreads();
+  const int cnt = rc;
+  if (cnt <= SEL_CAP) {
+    rank_collected(lk, li, cnt, a.n, [&](int r, long long k, int p) { write_slot(a, b, r, k, p); });
+    for (int r = cnt + tid; r < a.n; r += 256) write_dead_slot(a, b, r);
+    return;
+  }
+  long long prev = KEY_NAN;
+  int place = -1;
+  __shared__ long long sk[4];
+  __shared__ int sp[4];
+  for (int r = 0; r < a.n; ++r) {
+    long long k = KEY_NONE;
+    int p = 0x7fffffff;
+    for (int e = tid; e < total; e += 256) {
+      long long ke;
+      int pe;
+      candidate(e, ke, pe);
+      if (ke != KEY_NONE && better(prev, place, ke, pe) && better(ke, pe, k, p)) { k = ke; p = pe; }
+    }
+    block_best(k, p, sk, sp);
+    if (tid == 0) {
+      if (k != KEY_NONE) write_slot(a, b, r, k, p); else write_dead_slot(a, b, r);
+    }
+    prev = k;
+    place = p;
+  }
+}
+
+// how a call is split: 0 = one wave a group (registers), else values per thread of a 256-thread slice
+struct SelectPlan {
+  int g_log2, m;        // one wave a group
+  int u, splits;        // slices
+};
+inline SelectPlan select_plan(long long B, int W, int V, int item) {
+  SelectPlan p = {};
+  if (W <= 64) {
+    int gl = 6;
+    while ((64 >> gl) < W) --gl;
+    const int m = (V + (1 << gl) - 1) >> gl;
+    if (m <= 32) {
+      p.g_log2 = gl;
+      p.m = m;
+      return p;
+    }
+  }
+  // the largest slice that still gives every CU four workgroups; short rows take the smallest that holds them
+  const int ve = 16 / item;
+  p.u = 32;
+  while (p.u > 8 && B * W * ((V + ve - 1 + 256LL * p.u - 1) / (256LL * p.u)) < 1024) p.u >>= 1;
+  p.splits = (int)((V + ve - 1 + 256LL * p.u - 1) / (256LL * p.u));
+  return p;
+}
+
+template <typename T>
+int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_t st) {
+  if (p.u == 0) {
+    const dim3 grid(a.B), block(64);
+    if (p.m <= 2) hipLaunchKernelGGL((k_select_small<T, 2>), grid, block, 0, st, a, p.g_log2);
+    else if (p.m <= 4) hipLaunchKernelGGL((k_select_small<T, 4>), grid, block, 0, st, a, p.g_log2);
+    else if (p.m <= 8) hipLaunchKernelGGL((k_select_small<T, 8>), grid, block, 0, st, a, p.g_log2);
+    else if (p.m <= 16) hipLaunchKernelGGL((k_select_small<T, 16>), grid, block, 0, st, a, p.g_log2);
+    else hipLaunchKernelGGL((k_select_small<T, 32>), grid, block, 0, st, a, p.g_log2);
+    MPNN_LAUNCH_CHECK();
+  }
+  const long long parts = (long long)a.B * a.W * p.splits;
+  SlicePart* part = (SlicePart*)ws;
+  long long* pk = (long long*)(part + parts);
+  int* pi = (int*)(pk + parts * a.n);
+  const dim3 grid((unsigned)parts), block(256);
+#define MPNN_SLICE(U)                                                                                            \
+  do {                                                                                                           \
+    if (a.bias) hipLaunchKernelGGL((k_select_slice<T, U, true>), grid, block, 0, st, a, p.splits, part, pk, pi); \
+    else hipLaunchKernelGGL((k_select_slice<T, U, false>), grid, block, 0, st, a, p.splits, part, pk, pi);       \
+  } while (0)
+  if (p.u == 8) MPNN_SLICE(8);
+  else if (p.u == 16) MPNN_SLICE(16);
+  else MPNN_SLICE(32);
+#undef MPNN_SLICE
+  hipLaunchKernelGGL(k_select_merge, dim3(a.B), dim3(256), 0, st, a, p.splits, part, pk, pi);
+  MPNN_LAUNCH_CHECK();
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// States: a wave owns 64 columns of VEC bytes of one group - the same bytes of all its beams.  It reads the columns'
+// rows that move into LDS, then writes each row that changes from its parent's copy.  A column belongs to one lane from
+// first read to last write, so the update is in place without a barrier.  Bound by the bytes of the moving rows.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int RO_MAX = 16;
+struct ReorderTable {
+  mpnn_beam_state s[RO_MAX];
+};
+
+template <typename V>
+__device__ __forceinline__ void reorder_columns(char* data, long long sw, int W, const long long* __restrict__ parent, V* lds) {
+  const int lane = threadIdx.x;
+  for (int w0 = 0; w0 < W; w0 += 8) {   // eight rows in flight
+    V r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (w0 + i < W) r[i] = *(const V*)(data + (w0 + i) * sw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (w0 + i < W) lds[(w0 + i) * 64 + lane] = r[i];
+  }
+  for (int w = 0; w < W; ++w) {
+    const long long p = parent[w];
+    if (p != w && p >= 0 && p < W) *(V*)(data + w * sw) = lds[(int)p * 64 + lane];
+  }
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(64)
+k_beam_reorder(ReorderTable t, const long long* __restrict__ parent, int W, int length_all, const int* __restrict__ length,
+               const int* __restrict__ rank) {
+  extern __shared__ char lds[];
+  const mpnn_beam_state s = t.s[blockIdx.z];
+  const int b = blockIdx.y;
+  const unsigned per = (unsigned)(s.run / VEC);
+  const unsigned long long col = (unsigned long long)blockIdx.x * 64 + threadIdx.x;
+  if (col >= (unsigned long long)per * s.n_mid) return;
+  const unsigned mid = (unsigned)(col / per), off = (unsigned)(col % per);
+  if (length || length_all >= 0) {
+    const int len = length ? length[b] : length_all;
+    if ((rank ? rank[(long long)b * s.n_mid + mid] : (int)mid) >= len) return;
+  }
+  char* data = (char*)s.data + b * s.stride_group + mid * s.stride_mid + (long long)off * VEC;
+  const long long* p = parent + (long long)b * W;
+  if (VEC == 16) reorder_columns(data, s.stride_beam, W, p, (f32x4*)lds);
+  else if (VEC == 8) reorder_columns(data, s.stride_beam, W, p, (unsigned long long*)lds);
+  else if (VEC == 4) reorder_columns(data, s.stride_beam, W, p, (unsigned*)lds);
+  else if (VEC == 2) reorder_columns(data, s.stride_beam, W, p, (unsigned short*)lds);
+  else reorder_columns(data, s.stride_beam, W, p, (unsigned char*)lds);
+}
+
+// widest access every row of the state allows (its address, strides and run are multiples of it)
+inline int state_vec(const mpnn_beam_state& s, int W) {
+  unsigned long long bits = (unsigned long long)(uintptr_t)s.data | (unsigned long long)s.stride_group |
+                            (unsigned long long)s.stride_beam | (unsigned long long)s.run;
+  if (s.n_mid > 1) bits |= (unsigned long long)s.stride_mid;
+  int vec = 16;
+  while (vec > 1 && (bits & (vec - 1))) vec >>= 1;
+  while (vec > 1 && 64 * vec * W > 65536) vec >>= 1;   // the LDS a wave may hold
+  return vec;
+}
+
+}  // namespace
+
+extern "C" long long mpnn_beam_select_workspace(int dtype, int n_groups, int n_beams, int n_tokens, int n_out) {
+  if (dtype < 0 || dtype > 2 || n_groups <= 0 || n_beams <= 0 || n_tokens <= 0 || n_out <= 0 || n_out > SEL_MAX_N) return -1;
+  const SelectPlan p = select_plan(n_groups, n_beams, n_tokens, dtype == 0 ? 4 : 2);
+  if (p.u == 0) return 0;
+  return (long long)n_groups * n_beams * p.splits * ((long long)sizeof(SlicePart) + 12LL * n_out);
+}
+
+extern "C" int mpnn_beam_select(const void* logits, int dtype, long long stride_group, long long stride_beam,
+                                const float* scores, const float* bias, long long bias_group, long long bias_beam,
+                                const int64_t* forced, int n_groups, int n_beams, int n_tokens, int n_out,
+                                float* out_scores, int64_t* parent, int64_t* token, void* workspace,
+                                long long workspace_bytes, void* stream) {
+  MPNN_CHECK_ARG(logits && scores && out_scores && parent && token, "mpnn_beam_select: null pointer");
+  MPNN_CHECK_ARG(dtype >= 0 && dtype <= 2, "mpnn_beam_select: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+  MPNN_CHECK_ARG(n_groups > 0 && n_beams > 0 && n_beams <= SEL_MAX_N && n_out > 0 && n_out <= SEL_MAX_N && n_tokens > 0 &&
+                     n_tokens <= (1 << 22),
+                 "mpnn_beam_select: bad sizes (at most 256 beams and hypotheses kept, at most 2^22 tokens)");
+  const long long need = mpnn_beam_select_workspace(dtype, n_groups, n_beams, n_tokens, n_out);
+  MPNN_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+                 "mpnn_beam_select: workspace missing, too small (mpnn_beam_select_workspace) or not 16-byte aligned");
+  const SelectPlan p = select_plan(n_groups, n_beams, n_tokens, dtype == 0 ? 4 : 2);
+  MPNN_CHECK_ARG((long long)n_groups * n_beams * (p.u ? p.splits : 1) < (1LL << 31) &&
+                     (long long)n_beams * (p.u ? p.splits : 1) * n_out < (1LL << 31),
+                 "mpnn_beam_select: too many groups for one launch");
+  SelectArgs a = {logits, stride_group, stride_beam, scores, bias, bias_group, bias_beam, (const long long*)forced,
+                  n_groups, n_beams, n_tokens, n_out, out_scores, (long long*)parent, (long long*)token};
+  if (dtype == 0) return launch_select<float>(a, p, workspace, (hipStream_t)stream);
+  if (dtype == 1) return launch_select<__hip_bfloat16>(a, p, workspace, (hipStream_t)stream);
+  return launch_select<__half>(a, p, workspace, (hipStream_t)stream);
+}
+
+extern "C" int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int64_t* parent, int n_groups, int n_beams,
+                                 int length_all, const int32_t* length, const int32_t* rank, void* stream) {
+  MPNN_CHECK_ARG(n > 0 && states && parent, "mpnn_beam_reorder: null pointer");
+  MPNN_CHECK_ARG(n_groups > 0 && n_groups <= 65535 && n_beams > 0 && n_beams <= 256,
+                 "mpnn_beam_reorder: bad sizes (at most 65535 groups and 256 beams)");
+  MPNN_CHECK_ARG(!rank || length || length_all >= 0, "mpnn_beam_reorder: rank needs a length");
+  for (int i = 0; i < n; ++i) {
+    const mpnn_beam_state& s = states[i];
+    MPNN_CHECK_ARG(s.data && s.n_mid > 0 && s.run > 0 && (n_beams == 1 || s.stride_beam != 0) &&
+                       (n_groups == 1 || s.stride_group != 0) && (s.n_mid == 1 || s.stride_mid != 0),
+                   "mpnn_beam_reorder: a state is empty or its rows share memory");
+    MPNN_CHECK_ARG(s.run < (1LL << 31) && (double)s.run * s.n_mid / state_vec(s, n_beams) < 64.0 * 2147483647.0,
+                   "mpnn_beam_reorder: a state is too large for one launch");
+  }
+  // states of one access width share a launch
+  for (int vec = 16; vec >= 1; vec >>= 1) {
+    ReorderTable t;
+    int m = 0;
+    unsigned long long cols = 0;
+    for (int i = 0; i <= n; ++i) {
+      const bool mine = i < n && state_vec(states[i], n_beams) == vec;
+      if (m && (i == n || (mine && m == RO_MAX))) {
+        const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)n_groups, (unsigned)m), block(64);
+        const size_t lds = (size_t)64 * vec * n_beams;
+        hipStream_t st = (hipStream_t)stream;
+        const long long* p = (const long long*)parent;
+#define MPNN_REORDER(V) hipLaunchKernelGGL((k_beam_reorder<V>), grid, block, lds, st, t, p, n_beams, length_all, length, rank)
+        if (vec == 16) MPNN_REORDER(16);
+        else if (vec == 8) MPNN_REORDER(8);
+        else if (vec == 4) MPNN_REORDER(4);
+        else if (vec == 2) MPNN_REORDER(2);
+        else MPNN_REORDER(1);
+#undef MPNN_REORDER
+        m = 0;
+        cols = 0;
+      }
+      if (mine) {
+        t.s[m++] = states[i];
+        const unsigned long long c = (unsigned long long)(states[i].run / vec) * (unsigned long long)states[i].n_mid;
+        cols = c > cols ? c : cols;
+      }
+    }
+  }
+  MPNN_LAUNCH_CHECK();
+}
