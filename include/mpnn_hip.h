@@ -221,6 +221,25 @@ int mpnn_adamw_step(int n, float* const* params, const float* const* grads, floa
                     float* const* exp_avg_sq, const int* numel, float lr, float beta1, float beta2, float eps,
                     float weight_decay, int step, const float* grad_sumsq, float max_norm, void* stream);
 
+/* The same AdamW step with each tensor's moments in 8 bits or in 32 (no counterpart in the reference: 16.25 bytes of traffic
+ * and 2.1 bytes of state an element instead of 28 and 8).  HOST arrays of n device pointers; params / grads fp32.
+ *   exp_avg_scale[i] == NULL (then exp_avg_sq_scale[i] too): exp_avg / exp_avg_sq are fp32.
+ *   else: exp_avg / exp_avg_sq hold one e4m3 code (OCP: bias 7, no infinity) an element and the scales one fp32 power of two
+ *   for each 64 consecutive elements (ceil(numel / 64) of them); a moment is code * scale.  Zeros with scales of 1 (any
+ *   finite scale) are the initial state.  The block's largest moment lies in [128, 256) scales (scale >= 2^-126); moments
+ *   are rounded up with the probability of the part cut off, in steps of 2^-16, by bits of a hash of (seed, step, first + i,
+ *   element mod 2^32); a positive exp_avg_sq never becomes 0.  A block that holds a NaN, an infinity or more than fp32 can
+ *   gets the scale NaN: the tensor's failure shows in its next parameters.
+ * sumsq_parts != NULL and max_norm > 0: gradients are scaled by min(1, max_norm / (norm + 1e-6)), norm^2 = the sum of the
+ * 1024 doubles that mpnn_grad_sumsq_parts wrote (all of them, from any number of tensors; fp64, fixed order); grad_sumsq
+ * (may be NULL) gets norm^2.  Moments are fp64 up to their rounding, the update is fp32.  step >= 1.  No two tensors may
+ * share memory. */
+int mpnn_grad_sumsq_parts(int n, const float* const* grads, const long long* numel, double* parts, void* stream);
+int mpnn_adamw_mixed(int n, float* const* params, const float* const* grads, void* const* exp_avg, void* const* exp_avg_sq,
+                     float* const* exp_avg_scale, float* const* exp_avg_sq_scale, const long long* numel, double lr,
+                     double beta1, double beta2, double eps, double weight_decay, int step, uint32_t seed, int first,
+                     const double* sumsq_parts, double max_norm, float* grad_sumsq, void* stream);
+
 /* The gather helpers of the reference as ONE indexed row copy (gather_edges :13-18, gather_nodes :21-30,
  * gather_nodes_t :33-38, cat_neighbors_nodes :41-45):
  *   out[(g * n_idx + q) * out_ld + out_col0 + c] = src[(g * n_src + idx[g * n_idx + q]) * C + c],  c < C, g < G

@@ -21,6 +21,7 @@ _F = ctypes.c_float
 
 _U64 = ctypes.c_uint64
 _L = ctypes.c_longlong
+_D = ctypes.c_double
 
 
 class LevelLayer(ctypes.Structure):
@@ -107,6 +108,8 @@ SIGNATURES = {
     "mpnn_grad_sumsq": [_I, _P, _P, _P, _P, _I, _P],
     "mpnn_grad_scale": [_I, _P, _P, _P, _F, _P],
     "mpnn_adamw_step": [_I, _P, _P, _P, _P, _P, _F, _F, _F, _F, _F, _I, _P, _F, _P],
+    "mpnn_grad_sumsq_parts": [_I, _P, _P, _P, _P],
+    "mpnn_adamw_mixed": [_I] + [_P] * 7 + [_D] * 5 + [_I, ctypes.c_uint32, _I, _P, _D, _P, _P],
     "mpnn_beam_select": [_P, _I, _L, _L, _P, _P, _L, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P],
     "mpnn_beam_reorder": [_I, ctypes.POINTER(BeamState), _P, _I, _I, _I, _P, _P, _P],
     "mpnn_linear_rows": [_P, _I, _I, _P, _P, ctypes.c_longlong, _P, _P],

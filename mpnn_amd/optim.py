@@ -1,4 +1,4 @@
-"""AdamW and gradient-norm clipping of the reference's training loop on the HIP library (SURVEY 8f N3).
+"""AdamW and gradient-norm clipping of the reference's training loop on the HIP library.
 
 `AdamW` is `torch.optim.AdamW(lr, betas, eps, weight_decay)` as the reference constructs it (train.py:217; no amsgrad,
 not maximize): same update, same `state_dict` layout (`step`, `exp_avg`, `exp_avg_sq` per parameter), so the
@@ -6,6 +6,12 @@ not maximize): same update, same `state_dict` layout (`step`, `exp_avg`, `exp_av
 (`mpnn_adamw_step`); with `max_grad_norm` the clip of train.py:389-390 is folded into the same pass (the norm is
 reduced on the device by `mpnn_grad_sumsq`, nothing synchronises with the host).  `clip_grad_norm_` is the stand-alone
 form with torch's signature.  Parameters and gradients must be fp32 tensors on a ROCm device (no CPU fallback).
+
+`AdamW(state_bits=8)` keeps the moments of large tensors in 8 bits (no counterpart in the reference): 2.1 bytes an element
+instead of 8, and 16.25 bytes of traffic a step instead of 28.  A moment is an e4m3 code (`exp_avg`, `exp_avg_sq`:
+torch.float8_e4m3fn, the parameter's shape) times a power of two for each 64 consecutive elements (`exp_avg_scale`,
+`exp_avg_sq_scale`), rounded stochastically and reproducibly; `unpack_moment` / `pack_moment` convert, and checkpoints of
+either width load into either optimizer.  `adamw_step` is the functional form over lists of tensors.
 """
 from __future__ import annotations
 
@@ -57,14 +63,122 @@ def clip_grad_norm_(parameters, max_norm):
     return ss.sqrt().reshape(())
 
 
+BLOCK = 64      # elements of an 8-bit moment that share a scale
+_PARTS = 1024   # partial sums of mpnn_grad_sumsq_parts
+
+
+def pack_moment(x, positive=False):
+    """fp32 tensor -> (e4m3 codes of its shape, scales [ceil(numel / 64)]): the stored form of an 8-bit moment, rounded to
+    nearest (conversion of checkpoints; the step itself rounds stochastically).  positive: values above 0 do not become 0
+    (second moments)."""
+    n = x.numel()
+    y = torch.nn.functional.pad(x.detach().to(torch.float32).reshape(-1), (0, -n % BLOCK)).view(-1, BLOCK)
+    top = y.abs().amax(1) if n else y.new_zeros(0)
+    e = (torch.frexp(top)[1] - 8).clamp(min=-126)
+    scale = torch.where(top > 0, torch.exp2(e.double()).float(), torch.ones_like(top))
+    scale = torch.where(torch.isfinite(top), scale, torch.full_like(top, float("nan")))
+    q = y.double() / scale.double()[:, None]
+    if positive:
+        q = torch.where((q > 0) & (q < 2.0**-9), torch.full_like(q, 2.0**-9), q)
+    q = q.nan_to_num(0.0, 0.0, 0.0)
+    return q.float().to(torch.float8_e4m3fn).view(-1)[:n].view(x.shape), scale
+
+
+def unpack_moment(codes, scale):
+    """The fp32 values of an 8-bit moment."""
+    n = codes.numel()
+    return (codes.to(torch.float32).reshape(-1) * scale.repeat_interleave(BLOCK)[:n]).view(codes.shape)
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[None if t is None else t.data_ptr() for t in tensors])
+
+
+def _check_mixed(params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales):
+    """The lists belong together and every tensor is what mpnn_adamw_mixed takes it for."""
+    n = len(params)
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(scales) == len(sq_scales) == n):
+        raise ValueError("mpnn_amd.optim.adamw_step: lists of different lengths")
+    dev = params[0].device
+    _check(params, "parameters")
+    _check(grads, "gradients")
+    for p, g, m, v, a, b in zip(params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales):
+        k = p.numel()
+        want = torch.float32 if a is None else torch.float8_e4m3fn
+        if (a is None) != (b is None):
+            raise ValueError("mpnn_amd.optim.adamw_step: both moments of a tensor have scales, or none")
+        if g.numel() != k or m.numel() != k or v.numel() != k:
+            raise ValueError("mpnn_amd.optim.adamw_step: parameter, gradient and moments differ in size")
+        if m.dtype != want or v.dtype != want or not m.is_contiguous() or not v.is_contiguous():
+            raise ValueError("mpnn_amd.optim.adamw_step: moments must be contiguous fp32 tensors without scales, or "
+                             "float8_e4m3fn with scales")
+        if p.device != dev or g.device != dev or m.device != dev or v.device != dev:
+            raise RuntimeError("mpnn_amd.optim.adamw_step: all tensors must be on one device")
+        if a is not None:
+            blocks = -(-k // BLOCK)
+            if a.dtype != torch.float32 or b.dtype != torch.float32 or a.numel() != blocks or b.numel() != blocks or \
+                    not a.is_contiguous() or not b.is_contiguous() or a.device != dev or b.device != dev:
+                raise ValueError(f"mpnn_amd.optim.adamw_step: scales must be contiguous fp32 tensors of one element for each "
+                                 f"{BLOCK} of the parameter, on its device")
+
+
+def _mixed_call(params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales, step, lr, betas, eps, weight_decay, seed, first,
+                parts, max_norm, sumsq):
+    n = len(params)
+    numel = (ctypes.c_longlong * n)(*[p.numel() for p in params])
+    call("mpnn_adamw_mixed", n, _pointers(params), _pointers(grads), _pointers(exp_avgs), _pointers(exp_avg_sqs),
+         _pointers(scales), _pointers(sq_scales), numel, float(lr), float(betas[0]), float(betas[1]), float(eps),
+         float(weight_decay), int(step), int(seed) & 0xFFFFFFFF, first, ptr(parts), float(max_norm), ptr(sumsq), stream_ptr())
+
+
+def _sumsq_parts(grads):
+    parts = torch.empty(_PARTS, device=grads[0].device, dtype=torch.float64)
+    numel = (ctypes.c_longlong * len(grads))(*[g.numel() for g in grads])
+    call("mpnn_grad_sumsq_parts", len(grads), _pointers(grads), numel, ptr(parts), stream_ptr())
+    return parts
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, *, step, lr=1e-3,
+               betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0, max_grad_norm=0.0):
+    """One AdamW step over lists of tensors, in place.  params, grads: contiguous fp32.  Tensors whose scales are None keep
+    fp32 moments; the others hold float8_e4m3fn codes and fp32 scales (see the module's docstring; zeros and ones to begin
+    with).  step: 1 for the first.  seed, step, the place in the list and the element decide the rounding of 8-bit moments.
+    max_grad_norm > 0 clips by the norm over all gradients.  Returns the squared norm (a device scalar) then, else None.
+    No two tensors may share memory."""
+    lists = [list(x) for x in (params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales)]
+    if len(lists[0]) == 0:
+        return None
+    _check_mixed(*lists)
+    if int(step) < 1:
+        raise ValueError("mpnn_amd.optim.adamw_step: step counts from 1")
+    with torch.no_grad(), torch.cuda.device(lists[0][0].device):
+        if any(p.numel() == 0 for p in lists[0]):
+            raise ValueError("mpnn_amd.optim.adamw_step: empty tensor")
+        parts = sumsq = None
+        if max_grad_norm > 0.0:
+            parts = _sumsq_parts(lists[1])
+            sumsq = torch.empty(1, device=parts.device, dtype=torch.float32)
+        _mixed_call(*lists, step, lr, betas, eps, weight_decay, seed, 0, parts, max_grad_norm, sumsq)
+        torch.autograd.graph.increment_version([t for x in lists[:1] + lists[2:] for t in x if t is not None])
+    return sumsq
+
+
 class AdamW(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=0.0):
+    """torch.optim.AdamW on the HIP library.  state_bits=8: moments of tensors with at least `min_8bit_numel` elements are
+    held in 8 bits (the others in 32), rounded by `seed`; the step then counts from each parameter's own state, on the host,
+    so it cannot be captured into a HIP graph."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=0.0, state_bits=32,
+                 min_8bit_numel=4096, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError("mpnn_amd.optim.AdamW: state_bits is 8 or 32")
         if lr < 0 or eps < 0 or not 0 <= betas[0] < 1 or not 0 <= betas[1] < 1 or weight_decay < 0:
             raise ValueError("mpnn_amd.optim.AdamW: invalid hyper-parameter")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False,
                                       maximize=False, foreach=None, capturable=False, differentiable=False,
                                       fused=None, decoupled_weight_decay=True))
         self.max_grad_norm = float(max_grad_norm)
+        self.state_bits, self.min_8bit_numel, self.seed = state_bits, int(min_8bit_numel), int(seed)
         self.last_grad_sumsq = None  # device scalar of the last step (its square root is the unclipped gradient norm)
 
     @torch.no_grad()
@@ -79,6 +193,9 @@ class AdamW(torch.optim.Optimizer):
             return loss
         _check(every, "parameters")
         _check([p.grad for p in every], "gradients")
+        if self.state_bits == 8:
+            self._step_mixed(live, every)
+            return loss
         with torch.cuda.device(every[0].device):
             ss = None
             if self.max_grad_norm > 0.0:  # the clip norm spans every group, as clip_grad_norm_(model.parameters()) does
@@ -114,3 +231,61 @@ class AdamW(torch.optim.Optimizer):
                 for p in every:
                     torch.autograd.graph.increment_version(p) if hasattr(torch.autograd.graph, "increment_version") else None
         return loss
+
+    def _new_state(self, p):
+        st = {"step": torch.tensor(0.0)}
+        if p.numel() < self.min_8bit_numel:
+            st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            return st
+        for name in ("exp_avg", "exp_avg_sq"):
+            st[name] = torch.zeros(p.shape, device=p.device, dtype=torch.float8_e4m3fn)
+            st[name + "_scale"] = torch.ones(-(-p.numel() // BLOCK), device=p.device, dtype=torch.float32)
+        return st
+
+    def _step_mixed(self, live, every):
+        with torch.cuda.device(every[0].device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("mpnn_amd.optim.AdamW(state_bits=8): a step counts on the host and cannot be captured into a "
+                                   "HIP graph")
+            parts = None
+            self.last_grad_sumsq = None
+            if self.max_grad_norm > 0.0:
+                parts = _sumsq_parts([p.grad for p in every])
+                self.last_grad_sumsq = torch.empty(1, device=parts.device, dtype=torch.float32)
+            first, changed = 0, []
+            for group, ps in zip(self.param_groups, live):
+                by_step = {}
+                for p in ps:
+                    st = self.state[p]
+                    if not st:
+                        st.update(self._new_state(p))
+                    st["step"] += 1
+                    by_step.setdefault(int(st["step"]), []).append(p)
+                for k, sel in sorted(by_step.items()):
+                    states = [self.state[p] for p in sel]
+                    lists = [sel, [p.grad for p in sel]] + [[st.get(n) for st in states] for n in
+                                                            ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
+                    _check_mixed(*lists)
+                    _mixed_call(*lists, k, group["lr"], group["betas"], group["eps"], group["weight_decay"], self.seed, first,
+                                parts, self.max_grad_norm, self.last_grad_sumsq)
+                    first += len(sel)
+                    changed += sel
+            torch.autograd.graph.increment_version(changed)
+
+    def load_state_dict(self, state_dict):
+        """Checkpoints of 8-bit and of 32-bit moments (this optimizer's, torch's) load into an optimizer of either width."""
+        super().load_state_dict(state_dict)
+        for p, st in self.state.items():
+            if "exp_avg" not in st:
+                continue
+            wide = self.state_bits == 8 and p.numel() >= self.min_8bit_numel
+            for name in ("exp_avg", "exp_avg_sq"):
+                scale = st.pop(name + "_scale", None)
+                if scale is None:
+                    if wide:
+                        st[name], st[name + "_scale"] = pack_moment(st[name], name == "exp_avg_sq")
+                elif wide:   # torch has cast the codes to the parameter's type, without loss
+                    st[name], st[name + "_scale"] = st[name].to(torch.float8_e4m3fn), scale
+                else:
+                    st[name] = unpack_moment(st[name], scale)

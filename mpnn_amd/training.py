@@ -880,16 +880,20 @@ def loss_nll(S, log_probs, mask):
     return loss, torch.sum(loss * mask) / torch.sum(mask), true_false
 
 
-def make_optimizer(model, lr=1e-3, weight_decay=1e-2, total_steps=None, max_grad_norm=0.0):
+def make_optimizer(model, lr=1e-3, weight_decay=1e-2, total_steps=None, max_grad_norm=0.0, state_bits=32):
     """AdamW and, when `total_steps` is given, the reference's schedule (train.py:217-222): linear warm-up from 1e-8 over
     the first 1 % of the steps, then cosine annealing to 0.  On a ROCm device the optimizer is the in-tree multi-tensor
     kernel (`mpnn_amd.optim.AdamW`: all 1.66 M parameters in three launches, gradient clipping of train.py:389-390
     folded in when `max_grad_norm` > 0); a model with any parameter off the device gets torch.optim.AdamW (train_step
-    then clips with torch.nn.utils.clip_grad_norm_).  -> (optimizer, scheduler or None)."""
+    then clips with torch.nn.utils.clip_grad_norm_).  state_bits=8 holds the moments of its weight matrices in 8 bits (on a
+    ROCm device only).  -> (optimizer, scheduler or None)."""
     from torch.optim.lr_scheduler import CosineAnnealingLR, LinearLR, SequentialLR
     if all(p.is_cuda for p in model.parameters()):
         from .optim import AdamW
-        optimizer = AdamW(model.parameters(), lr=lr, weight_decay=weight_decay, max_grad_norm=max_grad_norm)
+        optimizer = AdamW(model.parameters(), lr=lr, weight_decay=weight_decay, max_grad_norm=max_grad_norm,
+                          state_bits=state_bits)
+    elif state_bits != 32:
+        raise RuntimeError("make_optimizer: state_bits=8 needs every parameter on a ROCm device")
     else:
         optimizer = torch.optim.AdamW(model.parameters(), lr=lr, weight_decay=weight_decay)
     if total_steps is None:
