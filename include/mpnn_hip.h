@@ -790,6 +790,30 @@ typedef struct mpnn_beam_state {
 int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int64_t* parent, int n_groups, int n_beams,
                       int length_all, const int32_t* length, const int32_t* rank, void* stream);
 
+/* The whole beam search of the model in one call, beside mpnn_decode_run: n_groups structures of L residues, n_beams
+ * hypotheses of each, residue id = beam * (n_groups * L) + structure * L + i; encoder-side arrays hold n_groups * L residues.
+ * A structure's hypotheses share one decoding order.  For position t of it: every decoder layer on node_list[t] (ids of the
+ * residue that comes t-th, [L][n_groups][n_beams]; mpnn_dec_layer_subset, above K = 48 mpnn_dec_message_subset +
+ * mpnn_node_update_subset with gsum [residue][4][128]), logits = W_out h + b, mpnn_beam_select with logit_bias [n_letters]
+ * (may be NULL) and forced [L][n_groups][n_beams], mpnn_beam_reorder of the layers' A rows, S and log_probs of the residues
+ * decided before, and for the residue itself A rows = the parent's + TS[token], S = token, log_probs = log_softmax(logits).
+ *   rank [n_beams][n_groups][L] (equal for all beams); layers as in mpnn_decode_run (K > 48: Wout8_packed is W_out as FOUR
+ *   128-column blocks, as mpnn_node_update_subset takes it); logits [n_groups][n_beams][n_letters], parent, token
+ *   [n_groups][n_beams]: scratch.  scores [2][n_groups][n_beams]: the first half holds the initial scores (0, then -inf);
+ *   the final ones stand in half L % 2.  A dead hypothesis (score -inf) holds a valid sequence all the same.
+ * At most 64 beams. */
+int mpnn_beam_run(const float* hE_frag, const float* PVenc, int ldenc, const int32_t* rank, const int32_t* E_idx32,
+                  const float* mask, const float* edge_mask, const int32_t* node_list, const int64_t* forced, int n_groups,
+                  int n_beams, int L, int K, const mpnn_level_layer* layers, int n_layers, const float* Wlogit_packed,
+                  const float* blogit, const float* logit_bias, int n_letters, const float* TS, int ld_ts, float* gsum,
+                  float* logits, float* scores, int64_t* parent, int64_t* token, int64_t* S, float* log_probs, void* stream);
+int mpnn_beam_run_f16(const float* hE_frag, const float* PVenc, int ldenc, const int32_t* rank, const int32_t* E_idx32,
+                      const float* mask, const float* edge_mask, const int32_t* node_list, const int64_t* forced,
+                      int n_groups, int n_beams, int L, int K, const mpnn_level_layer* layers, int n_layers,
+                      const float* Wlogit_packed, const float* blogit, const float* logit_bias, int n_letters,
+                      const float* TS, int ld_ts, float* gsum, float* logits, float* scores, int64_t* parent,
+                      int64_t* token, int64_t* S, float* log_probs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -112,6 +112,7 @@ SIGNATURES = {
     "mpnn_adamw_mixed": [_I] + [_P] * 7 + [_D] * 5 + [_I, ctypes.c_uint32, _I, _P, _D, _P, _P],
     "mpnn_beam_select": [_P, _I, _L, _L, _P, _P, _L, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P],
     "mpnn_beam_reorder": [_I, ctypes.POINTER(BeamState), _P, _I, _I, _I, _P, _P, _P],
+    "mpnn_beam_run": [_P, _P, _I] + [_P] * 6 + [_I] * 4 + [ctypes.POINTER(LevelLayer), _I, _P, _P, _P, _I, _P, _I] + [_P] * 8,
     "mpnn_linear_rows": [_P, _I, _I, _P, _P, ctypes.c_longlong, _P, _P],
     "mpnn_probe_elementwise": [_P, _I, _I, _P, _P],
     "mpnn_range_flag": [_P, ctypes.c_longlong, _F, _P, _I, _P],
@@ -122,7 +123,7 @@ SIGNATURES = {
 F16_ENTRIES = ("mpnn_edge_features", "mpnn_enc_message", "mpnn_enc_edge_update", "mpnn_dec_message", "mpnn_node_update",
                "mpnn_dec_message_subset", "mpnn_node_update_subset", "mpnn_dec_message_shared", "mpnn_dec_layer_subset", "mpnn_dec_layer_sample_subset",
                "mpnn_linear_rows", "mpnn_edge_features_biased", "mpnn_dec_message_valid",
-               "mpnn_decode_run")
+               "mpnn_decode_run", "mpnn_beam_run")
 for _n in F16_ENTRIES:
     SIGNATURES[_n + "_f16"] = SIGNATURES[_n]
 

@@ -609,6 +609,86 @@ inline int state_vec(const mpnn_beam_state& s, int W) {
   return vec;
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// The model's own search: logits of the residues of a step, and the chosen letters' way into the decoder's rows.
+// ---------------------------------------------------------------------------------------------------------------
+
+// logits[q][v] = W_out hV[list[q]] + b for the listed residues: 16 of them a wave, one column each
+__global__ void __launch_bounds__(64)
+k_beam_logits(const float* __restrict__ hV, const f32x4* __restrict__ Wp, const float* __restrict__ bias, int n_letters,
+              const int* __restrict__ list, int n_list, float* __restrict__ logits) {
+  const int lane = threadIdx.x, g = lane >> 4, q = blockIdx.x * 16 + (lane & 15);
+  const bool live = q < n_list;
+  const int nd = list[live ? q : n_list - 1];
+  f32x4 h[MPNN_NT][1], y[2][1];
+#pragma unroll
+  for (int t = 0; t < MPNN_NT; ++t) h[t][0] = *reinterpret_cast<const f32x4*>(hV + (size_t)nd * MPNN_H + 16 * t + 4 * g);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int letter = 16 * t + 4 * g + r;
+      y[t][0][r] = letter < n_letters ? bias[letter] : 0.f;
+    }
+  tile_gemm<1, MPNN_NT, 0, 2>(Wp, lane, h, y);
+  if (!live) return;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int letter = 16 * t + 4 * g + r;
+      if (letter < n_letters) logits[(size_t)q * n_letters + letter] = y[t][0][r];
+    }
+}
+
+struct PlaceArgs {
+  const int* list;             // residue id of (group, beam)
+  const long long* parent;
+  const long long* token;
+  const float* logits;         // [group][beam][n_letters]
+  int W, n_letters, n_layers;
+  float* A[4];                 // gathered rows of each decoder layer
+  int lda[4], offA[4];
+  const float* TS;             // letters' terms, 128 columns a layer
+  int ld_ts;
+  long long* S;
+  float* log_probs;
+};
+
+// The residue just decided, beam by beam: its gathered rows become the parent's plus the letter's term (block y < n_layers),
+// its letter and log-probs are written down (the last block).  A lane owns two columns of all beams, as in k_beam_reorder.
+__global__ void __launch_bounds__(64)
+k_beam_place(PlaceArgs a) {
+  extern __shared__ char lds[];
+  const int b = blockIdx.x, l = blockIdx.y, lane = threadIdx.x, W = a.W;
+  const long long* parent = a.parent + (long long)b * W;
+  const long long* token = a.token + (long long)b * W;
+  const int* list = a.list + b * W;
+  if (l < a.n_layers) {
+    float2* row = reinterpret_cast<float2*>(lds);
+    float* A = a.A[l] + a.offA[l] + 2 * lane;
+    for (int w = 0; w < W; ++w) row[w * 64 + lane] = *reinterpret_cast<const float2*>(A + (size_t)list[w] * a.lda[l]);
+    for (int w = 0; w < W; ++w) {
+      float2 v = row[(int)parent[w] * 64 + lane];
+      const float2 t = *reinterpret_cast<const float2*>(a.TS + (size_t)token[w] * a.ld_ts + l * MPNN_H + 2 * lane);
+      v.x += t.x;
+      v.y += t.y;
+      *reinterpret_cast<float2*>(A + (size_t)list[w] * a.lda[l]) = v;
+    }
+    return;
+  }
+  for (int w = lane; w < W; w += 64) {
+    const float* x = a.logits + ((long long)b * W + parent[w]) * a.n_letters;
+    float top = -INFINITY, sum = 0.f;
+    for (int v = 0; v < a.n_letters; ++v) top = fmaxf(top, x[v]);
+    for (int v = 0; v < a.n_letters; ++v) sum += expf(x[v] - top);
+    const float lse = top + logf(sum);
+    float* lp = a.log_probs + (size_t)list[w] * a.n_letters;
+    for (int v = 0; v < a.n_letters; ++v) lp[v] = x[v] - lse;
+    a.S[list[w]] = token[w];
+  }
+}
+
 }  // namespace
 
 extern "C" long long mpnn_beam_select_workspace(int dtype, int n_groups, int n_beams, int n_tokens, int n_out) {
@@ -687,3 +767,103 @@ extern "C" int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int
   }
   MPNN_LAUNCH_CHECK();
 }
+
+// The whole search in one call: per position of the decoding order the decoder layers on the groups' current residues, their
+// logits, the choice, the states of the residues decided earlier following their parents, and the chosen letters' terms.
+static int beam_run(bool f16, const float* hE_frag, const float* PVenc, int ldenc, const int32_t* rank,
+                    const int32_t* E_idx32, const float* mask, const float* edge_mask, const int32_t* node_list,
+                    const int64_t* forced, int n_groups, int n_beams, int L, int K, const mpnn_level_layer* layers,
+                    int n_layers, const float* Wlogit_packed, const float* blogit, const float* logit_bias, int n_letters,
+                    const float* TS, int ld_ts, float* gsum, float* logits, float* scores, int64_t* parent, int64_t* token,
+                    int64_t* S, float* log_probs, void* stream) {
+  MPNN_CHECK_ARG(hE_frag && PVenc && rank && E_idx32 && mask && node_list && forced && layers && Wlogit_packed && blogit && TS &&
+                     logits && scores && parent && token && S && log_probs,
+                 "mpnn_beam_run: null pointer");
+  MPNN_CHECK_ARG(n_groups > 0 && n_groups <= 65535 && n_beams > 0 && n_beams <= 64 && L > 0 && K >= 1 && K <= 64 &&
+                     n_layers >= 1 && n_layers <= 4 && n_letters >= 1 && n_letters <= 32 && (K <= 48 || gsum) &&
+                     (long long)n_groups * n_beams * L < (1LL << 31),
+                 "mpnn_beam_run: bad sizes (at most 64 beams, K <= 64, 1..4 layers, 32 letters; gsum for K > 48)");
+  const long long N = (long long)n_groups * L;
+  const int n_list = n_groups * n_beams;
+  PlaceArgs place = {};
+  mpnn_beam_state states[6];
+  for (int l = 0; l < n_layers; ++l) {
+    const mpnn_level_layer& y = layers[l];
+    MPNN_CHECK_ARG(l == 0 || (y.hV_in == layers[l - 1].hV_out && layers[l - 1].nproj >= 2),
+                   "mpnn_beam_run: layer l must read the hV rows (and Pa | A projections) layer l-1 writes");
+    MPNN_CHECK_ARG((y.lda & 3) == 0 && (y.offA & 3) == 0, "mpnn_beam_run: row strides and offsets are multiples of 4 floats");
+    place.A[l] = y.RowA;
+    place.lda[l] = y.lda;
+    place.offA[l] = y.offA;
+    // residue (w, b, i) is row w N + b L + i
+    states[l] = {y.RowA + y.offA, 4LL * y.lda * L, 4LL * y.lda * N, 4LL * y.lda, 4 * MPNN_H, L};
+  }
+  MPNN_CHECK_ARG(layers[n_layers - 1].nproj == 0, "mpnn_beam_run: the last decoder layer carries no projections");
+  states[n_layers] = {S, 8LL * L, 8LL * N, 8, 8, L};
+  states[n_layers + 1] = {log_probs, 4LL * n_letters * L, 4LL * n_letters * N, 4LL * n_letters, 4LL * n_letters, L};
+  place.parent = (const long long*)parent;
+  place.token = (const long long*)token;
+  place.logits = logits;
+  place.W = n_beams;
+  place.n_letters = n_letters;
+  place.n_layers = n_layers;
+  place.TS = TS;
+  place.ld_ts = ld_ts;
+  place.S = (long long*)S;
+  place.log_probs = log_probs;
+  float* now = scores;                      // the scores alternate between the two halves of their buffer
+  float* next = scores + n_list;
+  hipStream_t st = (hipStream_t)stream;
+  for (int t = 0; t < L; ++t) {
+    const int32_t* list = node_list + (long long)t * n_list;
+    for (int l = 0; l < n_layers; ++l) {
+      const mpnn_level_layer& y = layers[l];
+      int rc;
+      if (K <= 48) {
+        rc = (f16 ? mpnn_dec_layer_subset_f16 : mpnn_dec_layer_subset)(
+            hE_frag, y.P, y.ldp, y.offP, y.RowA, y.lda, y.offA, PVenc, ldenc, y.offEnc, rank, E_idx32, mask, edge_mask,
+            y.W1b_packed, y.W2_packed, y.b2, list, n_list, (int)N, L, K, y.hV_in, (float)K, y.W3_packed, y.b3, y.ln1_w,
+            y.ln1_b, y.Win_packed, y.b_in, y.Wout8_packed, y.b_out, y.ln2_w, y.ln2_b, y.scale, y.Wproj_packed, y.bproj,
+            y.nproj, y.hV_out, y.PQ, stream);
+      } else {
+        rc = (f16 ? mpnn_dec_message_subset_f16 : mpnn_dec_message_subset)(
+            hE_frag, y.P, y.ldp, y.offP, y.RowA, y.lda, y.offA, PVenc, ldenc, y.offEnc, rank, E_idx32, mask, edge_mask,
+            y.W1b_packed, y.W2_packed, y.b2, list, n_list, (int)N, L, K, gsum, stream);
+        if (!rc)
+          rc = (f16 ? mpnn_node_update_subset_f16 : mpnn_node_update_subset)(
+              y.hV_in, gsum, (K + 15) / 16, (float)K, mask, y.W3_packed, y.b3, y.ln1_w, y.ln1_b, y.Win_packed, y.b_in,
+              y.Wout8_packed, y.b_out, y.ln2_w, y.ln2_b, y.scale, y.Wproj_packed, y.bproj, y.nproj, list, n_list, y.hV_out,
+              y.PQ, stream);
+      }
+      if (rc) return rc;
+    }
+    hipLaunchKernelGGL(k_beam_logits, dim3((n_list + 15) / 16), dim3(64), 0, st, layers[n_layers - 1].hV_out,
+                       (const f32x4*)Wlogit_packed, blogit, n_letters, list, n_list, logits);
+    int rc = mpnn_beam_select(logits, 0, (long long)n_beams * n_letters, n_letters, now, logit_bias, 0, 0,
+                              forced + (long long)t * n_list, n_groups, n_beams, n_letters, n_beams, next, parent, token,
+                              nullptr, 0, stream);
+    if (!rc && t > 0)
+      rc = mpnn_beam_reorder(n_layers + 2, states, parent, n_groups, n_beams, t, nullptr, rank, stream);
+    if (rc) return rc;
+    place.list = list;
+    hipLaunchKernelGGL(k_beam_place, dim3(n_groups, n_layers + 1), dim3(64), (size_t)n_beams * 512, st, place);
+    float* s = now;
+    now = next;
+    next = s;
+  }
+  MPNN_LAUNCH_CHECK();
+}
+
+#define MPNN_BEAM_RUN(name, f16)                                                                                          \
+  extern "C" int name(const float* hE_frag, const float* PVenc, int ldenc, const int32_t* rank, const int32_t* E_idx32,   \
+                      const float* mask, const float* edge_mask, const int32_t* node_list, const int64_t* forced,         \
+                      int n_groups, int n_beams, int L, int K, const mpnn_level_layer* layers, int n_layers,              \
+                      const float* Wlogit_packed, const float* blogit, const float* logit_bias, int n_letters,            \
+                      const float* TS, int ld_ts, float* gsum, float* logits, float* scores, int64_t* parent,             \
+                      int64_t* token, int64_t* S, float* log_probs, void* stream) {                                       \
+    return beam_run(f16, hE_frag, PVenc, ldenc, rank, E_idx32, mask, edge_mask, node_list, forced, n_groups, n_beams, L,  \
+                    K, layers, n_layers, Wlogit_packed, blogit, logit_bias, n_letters, TS, ld_ts, gsum, logits, scores,   \
+                    parent, token, S, log_probs, stream);                                                                 \
+  }
+MPNN_BEAM_RUN(mpnn_beam_run, false)
+MPNN_BEAM_RUN(mpnn_beam_run_f16, true)

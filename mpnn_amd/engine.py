@@ -873,18 +873,7 @@ def _sample(model, X, mask, chain_M, residue_idx, chain_encoding_all, S_true, n_
             f_head = lambda *a: (call("mpnn_sample_subset", *a), 0)[1]
         layers = (_lib.LevelLayer * n_dec)()
         for l, lw in enumerate(pw.dec):
-            grp = pw.g_dec[l]
-            y = layers[l]
-            y.P, y.ldp, y.offP = ptr(PA[l]), 2 * H, 0
-            y.RowA, y.lda, y.offA = ptr(PA[l]), 2 * H, H
-            y.offEnc = base + 2 * H + H * l
-            y.W1b_packed, y.W2_packed, y.b2 = ptr(lw["W1b"]), ptr(lw["W2"]), ptr(lw["b2"])
-            y.hV_in, y.hV_out = ptr(hVs[l]), ptr(hVs[l + 1])
-            y.W3_packed, y.b3, y.ln1_w, y.ln1_b = ptr(lw["W3"]), ptr(lw["b3"]), ptr(lw["ln1w"]), ptr(lw["ln1b"])
-            y.Win_packed, y.b_in, y.Wout8_packed, y.b_out = ptr(lw["Win"]), ptr(lw["bin"]), ptr(lw["Wout8"]), ptr(lw["bout"])
-            y.ln2_w, y.ln2_b, y.scale = ptr(lw["ln2w"]), ptr(lw["ln2b"]), lw["scale"]
-            y.Wproj_packed, y.bproj, y.nproj = ptr(grp[0]), ptr(grp[1]), grp[2]
-            y.PQ = ptr(PA[l + 1]) if grp[2] else None
+            _level_layer(layers[l], lw, pw.g_dec[l], PA, hVs, l, base)
         # everything above (state tensors, argument lists) was prepared without knowing the level sizes; now the call's
         # one host read, which waits for the side stream only
         with torch.cuda.stream(side):
@@ -928,6 +917,110 @@ def _sample(model, X, mask, chain_M, residue_idx, chain_encoding_all, S_true, n_
                                f"{lib.mpnn_last_error().decode(errors='replace')}")
     return dict(S=S_out.view(n_samples, B, L), log_probs=log_probs.view(n_samples, B, L, -1),
                 order=order.view(n_samples, B, L), n_levels=len(counts))
+
+
+def _level_layer(y, lw, grp, PA, hVs, l, base):
+    """Fill mpnn_level_layer number l: Pa | A rows PA[l], hVs[l] -> hVs[l + 1], packed weights lw, next projections grp."""
+    y.P, y.ldp, y.offP = ptr(PA[l]), 2 * H, 0
+    y.RowA, y.lda, y.offA = ptr(PA[l]), 2 * H, H
+    y.offEnc = base + 2 * H + H * l
+    y.W1b_packed, y.W2_packed, y.b2 = ptr(lw["W1b"]), ptr(lw["W2"]), ptr(lw["b2"])
+    y.hV_in, y.hV_out = ptr(hVs[l]), ptr(hVs[l + 1])
+    y.W3_packed, y.b3, y.ln1_w, y.ln1_b = ptr(lw["W3"]), ptr(lw["b3"]), ptr(lw["ln1w"]), ptr(lw["ln1b"])
+    y.Win_packed, y.b_in, y.Wout8_packed, y.b_out = ptr(lw["Win"]), ptr(lw["bin"]), ptr(lw["Wout8"]), ptr(lw["bout"])
+    y.ln2_w, y.ln2_b, y.scale = ptr(lw["ln2w"]), ptr(lw["ln2b"]), lw["scale"]
+    y.Wproj_packed, y.bproj, y.nproj = ptr(grp[0]), ptr(grp[1]), grp[2]
+    y.PQ = ptr(PA[l + 1]) if grp[2] else None
+
+
+# ---------------------------------------------------------------------------
+# beam search (no reference function): the sampler's decoder, one position of the order at a time
+# ---------------------------------------------------------------------------
+def beam_search(model, X, mask, chain_M, residue_idx, chain_encoding_all, S_true=None, beam_width=8, seed=0,
+                fix_order=None, logit_bias=None, backbone_noise=None):
+    """Search for the most probable sequences of each structure in a random (or given, fix_order [B,L]) decoding order.
+
+    Returns dict(S [beam_width,B,L] int64, scores [beam_width,B], log_probs [beam_width,B,L,21], order [B,L]), best first.
+    A score is the sum of the designed residues' log-probs, of log_softmax(logits + logit_bias) where a bias is given;
+    log_probs are the model's own, as a teacher-forced forward on S with the same order returns them.  Residues with
+    chain_M * mask == 0 keep S_true.  beam_width 1 is greedy decoding; with more beams than sequences (logit_bias = -inf
+    takes letters out) the places left over have the score -inf.  The featurizer and encoder run once per structure."""
+    _require_device(X, "X")
+    W = int(beam_width)
+    if not 1 <= W <= 64:
+        raise ValueError("mpnn_amd.beam_search: beam_width must lie in 1..64")
+    guard = numerics_guard(model, X.device)
+    guard.poll()
+    _lib.set_precision(getattr(model, "precision", "fp32"))
+    try:
+        out = _beam_search(model, X, mask, chain_M, residue_idx, chain_encoding_all, S_true, W, seed, fix_order, logit_bias,
+                           backbone_noise)
+        guard.watch(out["log_probs"], "a beam search")
+        return out
+    finally:
+        _lib.set_precision("fp32")
+
+
+def _beam_search(model, X, mask, chain_M, residue_idx, chain_encoding_all, S_true, W, seed, fix_order, logit_bias,
+                 backbone_noise):
+    dev = X.device
+    mask = _f32(mask)
+    B, L = mask.shape
+    N = B * L
+    pw = packed(model)
+    n_dec = len(pw.dec)
+    if n_dec == 0 or n_dec > 4:
+        raise ValueError("mpnn_amd.beam_search needs 1..4 decoder layers")
+    with torch.no_grad():
+        cm = _f32(chain_M) * mask
+        if fix_order is not None:
+            order = _i64(fix_order)
+            if tuple(order.shape) != (B, L) or not bool((torch.sort(order, dim=-1).values == torch.arange(L, device=dev)).all()):
+                raise ValueError(f"fix_order must be [{B}, {L}] and every row a permutation of 0..{L - 1}")
+        else:  # reference :489-491
+            g_ = torch.Generator(device=dev)
+            g_.manual_seed(int(seed))
+            order = torch.argsort((cm + 0.0001) * torch.abs(torch.randn(B, L, device=dev, generator=g_)), dim=-1)
+        enc = _encode(model, X, mask, _i64(residue_idx), _i64(chain_encoding_all), backbone_noise)
+        K = enc["K"]
+        if K > 64:
+            raise NotImplementedError("mpnn_amd.beam_search covers k_neighbors <= 64")
+        st = stream_ptr()
+        rank1 = torch.zeros(N, device=dev, dtype=torch.int32)
+        call("mpnn_order_rank", ptr(order), B, L, ptr(rank1), st)
+        rank = rank1.repeat(W)
+        # ids of the residues that come t-th, and the letters of those that are not designed
+        ids = (torch.arange(W, device=dev).view(1, 1, W) * N + (torch.arange(B, device=dev).view(1, B) * L + order.t()).unsqueeze(2))
+        ids = ids.to(torch.int32).contiguous()
+        S_in = _i64(S_true).reshape(B, L).clamp(0, pw.n_letters - 1) if S_true is not None else \
+            torch.zeros(B, L, device=dev, dtype=torch.int64)
+        forced = torch.where(cm != 0, torch.full_like(S_in, -1), S_in).gather(1, order).t().unsqueeze(2).expand(L, B, W).contiguous()
+        scores = torch.full((2, B, W), float("-inf"), device=dev, dtype=torch.float32)
+        scores[0, :, 0] = 0.0
+        S = torch.zeros(W, N, device=dev, dtype=torch.int64)
+        log_probs = torch.zeros(W * N, pw.n_letters, device=dev, dtype=torch.float32)
+        base = 2 * H if len(pw.enc) else 0
+        PQenc = enc["PQ"]
+        hVs = [enc["hV"].repeat(W, 1)] + [torch.empty(W * N, H, device=dev) for _ in range(n_dec)]
+        PA = [PQenc[:, base:base + 2 * H].repeat(W, 1)] + [torch.empty(W * N, 2 * H, device=dev) for _ in range(n_dec - 1)]
+        lb = _f32(logit_bias).to(dev) if logit_bias is not None else None
+        if lb is not None and lb.numel() != pw.n_letters:
+            raise ValueError(f"logit_bias must hold one number for each of the {pw.n_letters} letters")
+        mask_s = mask.reshape(1, N).expand(W, N).contiguous()
+        gsum = torch.empty(W * N, 4, H, device=dev, dtype=torch.float32) if K > 48 else None
+        logits = torch.empty(B, W, pw.n_letters, device=dev, dtype=torch.float32)
+        parent = torch.empty(B, W, device=dev, dtype=torch.int64)
+        token = torch.empty(B, W, device=dev, dtype=torch.int64)
+        layers = (_lib.LevelLayer * n_dec)()
+        for l, lw in enumerate(pw.dec):
+            _level_layer(layers[l], lw, pw.g_dec[l], PA, hVs, l, base)
+            if K > 48:   # the separate node update takes W_out in 128-column blocks
+                layers[l].Wout8_packed = ptr(lw["Wout"])
+        call("mpnn_beam_run", ptr(enc["hE"]), ptr(PQenc), PQenc.shape[1], ptr(rank), ptr(enc["E_idx32"]), ptr(mask_s),
+             ptr(enc["edge_mask"]), ptr(ids), ptr(forced), B, W, L, K, layers, n_dec, ptr(pw.Wlogit), ptr(pw.blogit), ptr(lb),
+             pw.n_letters, ptr(pw.TS), pw.TS.shape[1], ptr(gsum), ptr(logits), ptr(scores), ptr(parent), ptr(token), ptr(S),
+             ptr(log_probs), st)
+    return dict(S=S.view(W, B, L), scores=scores[L % 2].t(), log_probs=log_probs.view(W, B, L, -1), order=order)
 
 
 def edges_to_natural(hE, n_nodes, K):

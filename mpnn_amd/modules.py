@@ -233,3 +233,11 @@ class ProteinMPNN(nn.Module):
         with _on_device_of(X), torch.autocast(device_type="cuda", enabled=False):
             return engine.sample(self, X, mask, chain_M, residue_idx, chain_encoding_all, S_true, n_samples,
                                  temperature, seed, fix_order, logit_bias)
+
+    def beam_search(self, X, mask, chain_M, residue_idx, chain_encoding_all, S_true=None, beam_width=8, seed=0,
+                    fix_order=None, logit_bias=None):
+        """The most probable sequences in one decoding order per structure (no counterpart in the reference; see
+        engine.beam_search)."""
+        with _on_device_of(X), torch.autocast(device_type="cuda", enabled=False):
+            return engine.beam_search(self, X, mask, chain_M, residue_idx, chain_encoding_all, S_true, beam_width, seed,
+                                      fix_order, logit_bias)
