@@ -3,8 +3,8 @@ HIPCC ?= /opt/rocm/bin/hipcc
 ARCH  ?= gfx950
 CSRC  := mpnn_amd/csrc
 OUT   := mpnn_amd/libmpnn_hip.so
-HIPFLAGS := -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -Iinclude -I$(CSRC) -Wno-unused-result $(EXTRA)
 NOPACK := -Xclang -target-feature -Xclang -packed-fp32-ops
+HIPFLAGS := $(NOPACK) -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -Iinclude -I$(CSRC) -Wno-unused-result $(EXTRA)
 OBJS  := $(CSRC)/mpnn_featurizer.o $(CSRC)/mpnn_edge.o $(CSRC)/mpnn_edge_bwd.o $(CSRC)/mpnn_node.o $(CSRC)/mpnn_node_bwd.o $(CSRC)/mpnn_data.o $(CSRC)/mpnn_loss.o $(CSRC)/mpnn_beam.o $(CSRC)/mpnn_optim.o $(CSRC)/mpnn_abi.o \
          $(CSRC)/mpnn_featurizer_f16.o $(CSRC)/mpnn_edge_f16.o $(CSRC)/mpnn_node_f16.o
 
@@ -33,10 +33,10 @@ $(CSRC)/mpnn_loss.o: $(CSRC)/mpnn_loss.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_ab
 
 # -packed-fp32-ops: no v_pk_*_f32 (some of their forms gave wrong results on this hardware)
 $(CSRC)/mpnn_beam.o: $(CSRC)/mpnn_beam.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_ablation.h include/mpnn_hip.h
-	$(HIPCC) $(HIPFLAGS) $(NOPACK) -ffp-contract=off -c $< -o $@
+	$(HIPCC) $(HIPFLAGS) -ffp-contract=off -c $< -o $@
 
 $(CSRC)/mpnn_optim.o: $(CSRC)/mpnn_optim.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_ablation.h include/mpnn_hip.h
-	$(HIPCC) $(HIPFLAGS) $(NOPACK) -ffp-contract=off -c $< -o $@
+	$(HIPCC) $(HIPFLAGS) -ffp-contract=off -c $< -o $@
 
 $(OUT): $(OBJS)
 	$(HIPCC) -shared -fPIC --offload-arch=$(ARCH) $(OBJS) -o $@

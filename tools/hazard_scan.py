@@ -195,7 +195,7 @@ def scan(asm_text):
 def main():
     src, extra = sys.argv[1], sys.argv[2:]
     with tempfile.NamedTemporaryFile(suffix=".s") as f:
-        subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-Iinclude", "-Impnn_amd/csrc",
+        subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-std=c++17", "--offload-arch=gfx950", "-Iinclude", "-Impnn_amd/csrc",
                         "-S", "--cuda-device-only", "-o", f.name, src] + extra, check=True, stderr=subprocess.DEVNULL)
         text = open(f.name).read()
     found = scan(text)
