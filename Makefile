@@ -8,7 +8,18 @@ HIPFLAGS := $(NOPACK) -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -Iinclude -I$(
 OBJS  := $(CSRC)/mpnn_featurizer.o $(CSRC)/mpnn_edge.o $(CSRC)/mpnn_edge_bwd.o $(CSRC)/mpnn_node.o $(CSRC)/mpnn_node_bwd.o $(CSRC)/mpnn_data.o $(CSRC)/mpnn_loss.o $(CSRC)/mpnn_beam.o $(CSRC)/mpnn_optim.o $(CSRC)/mpnn_abi.o \
          $(CSRC)/mpnn_featurizer_f16.o $(CSRC)/mpnn_edge_f16.o $(CSRC)/mpnn_node_f16.o
 
-all: $(OUT)
+# host side of the many-tensor entry points: a CPython extension on torch's C++ headers, in-tree like the library
+PYTHON ?= python3
+TORCH  := $(shell $(PYTHON) -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
+PYINC  := $(shell $(PYTHON) -c "import sysconfig; print(sysconfig.get_paths()['include'])")
+HOST   := mpnn_amd/_host.so
+
+all: $(OUT) $(HOST)
+
+$(HOST): $(CSRC)/mpnn_host.cpp include/mpnn_hip.h
+	g++ -O2 -std=c++17 -fPIC -shared -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -D_GLIBCXX_USE_CXX11_ABI=1 -Iinclude -I$(TORCH)/include \
+	  -I$(PYINC) -I/opt/rocm/include -Wno-deprecated-declarations $< -o $@ -L$(TORCH)/lib -ltorch_python -ltorch_cpu -lc10 \
+	  -lc10_hip -Wl,-rpath,$(TORCH)/lib
 
 # neighbour search must round like the reference's separate ATen ops: no FMA contraction there
 # -fno-slp-vectorize: packed fp32 VALU forms occupy the issue port ~10 cycles next to MFMAs against 4.2 for the scalar
@@ -42,7 +53,7 @@ $(OUT): $(OBJS)
 	$(HIPCC) -shared -fPIC --offload-arch=$(ARCH) $(OBJS) -o $@
 
 clean:
-	rm -f $(OBJS) $(OUT)
+	rm -f $(OBJS) $(OUT) $(HOST)
 
 # Every compile-time switch left in the sources, compiled once (front end + device code generation, nothing linked):
 # the f16-product twin is part of `all`; here the phase stamps and each timing-only ablation of mpnn_ablation.h.

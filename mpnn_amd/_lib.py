@@ -187,6 +187,40 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_host = None
+# functions of the library that csrc/mpnn_host.cpp calls, in the order its bind() takes them
+_HOST_ENTRIES = ("mpnn_beam_select", "mpnn_beam_select_workspace", "mpnn_beam_reorder", "mpnn_grad_sumsq_parts",
+                 "mpnn_adamw_mixed", "mpnn_last_error")
+
+
+def host():
+    """The CPython extension with the host side of the many-tensor entry points (csrc/mpnn_host.cpp), bound to the library."""
+    global _host
+    if _host is None:
+        lib = load()
+        try:
+            from . import _host as ext
+        except ImportError as e:
+            raise RuntimeError(f"mpnn_amd/_host.so is missing or does not load ({e}): build it first (`make` at the repo root or "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`). mpnn_amd has no CPU fallback.") from e
+        ext.bind(*[ctypes.cast(getattr(lib, n), _P).value for n in _HOST_ENTRIES])
+        _host = ext
+    return _host
+
+
+def host_call(name: str, fn: str, *args):
+    """A function of host(); `name` is the entry point its device time is booked on while a profiler is set."""
+    f = getattr(_host or host(), fn)
+    if _profile is None:
+        return f(*args)
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    out = f(*args)
+    e1.record()
+    _profile.setdefault(name, []).append((e0, e1))
+    return out
+
+
 def ptr(t):
     """Device pointer of a tensor (None -> NULL).  Tensors must be contiguous."""
     if t is None:

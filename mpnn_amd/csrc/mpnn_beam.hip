@@ -551,9 +551,10 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
 // rows that move into LDS, then writes each row that changes from its parent's copy.  A column belongs to one lane from
 // first read to last write, so the update is in place without a barrier.  Bound by the bytes of the moving rows.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int RO_MAX = 16;
+constexpr int RO_MAX = 32;
 struct ReorderTable {
   mpnn_beam_state s[RO_MAX];
+  unsigned char vec_log2[RO_MAX];   // bytes of a column
 };
 
 template <typename V>
@@ -574,14 +575,13 @@ __device__ __forceinline__ void reorder_columns(char* data, long long sw, int W,
   }
 }
 
-template <int VEC>
 __global__ void __launch_bounds__(64)
 k_beam_reorder(ReorderTable t, const long long* __restrict__ parent, int W, int length_all, const int* __restrict__ length,
                const int* __restrict__ rank) {
   extern __shared__ char lds[];
   const mpnn_beam_state s = t.s[blockIdx.z];
-  const int b = blockIdx.y;
-  const unsigned per = (unsigned)(s.run / VEC);
+  const int b = blockIdx.y, vl = t.vec_log2[blockIdx.z];
+  const unsigned per = (unsigned)(s.run >> vl);
   const unsigned long long col = (unsigned long long)blockIdx.x * 64 + threadIdx.x;
   if (col >= (unsigned long long)per * s.n_mid) return;
   const unsigned mid = (unsigned)(col / per), off = (unsigned)(col % per);
@@ -589,24 +589,24 @@ k_beam_reorder(ReorderTable t, const long long* __restrict__ parent, int W, int 
     const int len = length ? length[b] : length_all;
     if ((rank ? rank[(long long)b * s.n_mid + mid] : (int)mid) >= len) return;
   }
-  char* data = (char*)s.data + b * s.stride_group + mid * s.stride_mid + (long long)off * VEC;
+  char* data = (char*)s.data + b * s.stride_group + mid * s.stride_mid + ((long long)off << vl);
   const long long* p = parent + (long long)b * W;
-  if (VEC == 16) reorder_columns(data, s.stride_beam, W, p, (f32x4*)lds);
-  else if (VEC == 8) reorder_columns(data, s.stride_beam, W, p, (unsigned long long*)lds);
-  else if (VEC == 4) reorder_columns(data, s.stride_beam, W, p, (unsigned*)lds);
-  else if (VEC == 2) reorder_columns(data, s.stride_beam, W, p, (unsigned short*)lds);
+  if (vl == 4) reorder_columns(data, s.stride_beam, W, p, (f32x4*)lds);
+  else if (vl == 3) reorder_columns(data, s.stride_beam, W, p, (unsigned long long*)lds);
+  else if (vl == 2) reorder_columns(data, s.stride_beam, W, p, (unsigned*)lds);
+  else if (vl == 1) reorder_columns(data, s.stride_beam, W, p, (unsigned short*)lds);
   else reorder_columns(data, s.stride_beam, W, p, (unsigned char*)lds);
 }
 
-// widest access every row of the state allows (its address, strides and run are multiples of it)
-inline int state_vec(const mpnn_beam_state& s, int W) {
+// widest access every row of the state allows (its address, strides and run are multiples of it), as a power of two
+inline int state_vec_log2(const mpnn_beam_state& s, int W) {
   unsigned long long bits = (unsigned long long)(uintptr_t)s.data | (unsigned long long)s.stride_group |
                             (unsigned long long)s.stride_beam | (unsigned long long)s.run;
   if (s.n_mid > 1) bits |= (unsigned long long)s.stride_mid;
-  int vec = 16;
-  while (vec > 1 && (bits & (vec - 1))) vec >>= 1;
-  while (vec > 1 && 64 * vec * W > 65536) vec >>= 1;   // the LDS a wave may hold
-  return vec;
+  int vl = 4;
+  while (vl > 0 && (bits & ((1u << vl) - 1))) --vl;
+  while (vl > 0 && (64 << vl) * W > 65536) --vl;   // the LDS a wave may hold
+  return vl;
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -733,37 +733,26 @@ extern "C" int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int
     MPNN_CHECK_ARG(s.data && s.n_mid > 0 && s.run > 0 && (n_beams == 1 || s.stride_beam != 0) &&
                        (n_groups == 1 || s.stride_group != 0) && (s.n_mid == 1 || s.stride_mid != 0),
                    "mpnn_beam_reorder: a state is empty or its rows share memory");
-    MPNN_CHECK_ARG(s.run < (1LL << 31) && (double)s.run * s.n_mid / state_vec(s, n_beams) < 64.0 * 2147483647.0,
+    MPNN_CHECK_ARG(s.run < (1LL << 31) && ((unsigned long long)(s.run >> state_vec_log2(s, n_beams)) * s.n_mid + 63) / 64 < (1ULL << 31),
                    "mpnn_beam_reorder: a state is too large for one launch");
   }
-  // states of one access width share a launch
-  for (int vec = 16; vec >= 1; vec >>= 1) {
+  for (int i0 = 0; i0 < n; i0 += RO_MAX) {
     ReorderTable t;
-    int m = 0;
+    const int m = n - i0 < RO_MAX ? n - i0 : RO_MAX;
     unsigned long long cols = 0;
-    for (int i = 0; i <= n; ++i) {
-      const bool mine = i < n && state_vec(states[i], n_beams) == vec;
-      if (m && (i == n || (mine && m == RO_MAX))) {
-        const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)n_groups, (unsigned)m), block(64);
-        const size_t lds = (size_t)64 * vec * n_beams;
-        hipStream_t st = (hipStream_t)stream;
-        const long long* p = (const long long*)parent;
-#define MPNN_REORDER(V) hipLaunchKernelGGL((k_beam_reorder<V>), grid, block, lds, st, t, p, n_beams, length_all, length, rank)
-        if (vec == 16) MPNN_REORDER(16);
-        else if (vec == 8) MPNN_REORDER(8);
-        else if (vec == 4) MPNN_REORDER(4);
-        else if (vec == 2) MPNN_REORDER(2);
-        else MPNN_REORDER(1);
-#undef MPNN_REORDER
-        m = 0;
-        cols = 0;
-      }
-      if (mine) {
-        t.s[m++] = states[i];
-        const unsigned long long c = (unsigned long long)(states[i].run / vec) * (unsigned long long)states[i].n_mid;
-        cols = c > cols ? c : cols;
-      }
+    int widest = 0;
+    for (int i = 0; i < m; ++i) {
+      const mpnn_beam_state& s = states[i0 + i];
+      const int vl = state_vec_log2(s, n_beams);
+      t.s[i] = s;
+      t.vec_log2[i] = (unsigned char)vl;
+      widest = vl > widest ? vl : widest;
+      const unsigned long long c = (unsigned long long)(s.run >> vl) * (unsigned long long)s.n_mid;
+      cols = c > cols ? c : cols;
     }
+    hipLaunchKernelGGL(k_beam_reorder, dim3((unsigned)((cols + 63) / 64), (unsigned)n_groups, (unsigned)m), dim3(64),
+                       (size_t)(64 << widest) * n_beams, (hipStream_t)stream, t, (const long long*)parent, n_beams, length_all,
+                       length, rank);
   }
   MPNN_LAUNCH_CHECK();
 }

@@ -19,7 +19,7 @@ import ctypes
 
 import torch
 
-from ._lib import call, ptr, stream_ptr
+from ._lib import call, host_call, ptr, stream_ptr
 
 
 def _tables(tensors):
@@ -64,7 +64,6 @@ def clip_grad_norm_(parameters, max_norm):
 
 
 BLOCK = 64      # elements of an 8-bit moment that share a scale
-_PARTS = 1024   # partial sums of mpnn_grad_sumsq_parts
 
 
 def pack_moment(x, positive=False):
@@ -90,54 +89,6 @@ def unpack_moment(codes, scale):
     return (codes.to(torch.float32).reshape(-1) * scale.repeat_interleave(BLOCK)[:n]).view(codes.shape)
 
 
-def _pointers(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[None if t is None else t.data_ptr() for t in tensors])
-
-
-def _check_mixed(params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales):
-    """The lists belong together and every tensor is what mpnn_adamw_mixed takes it for."""
-    n = len(params)
-    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(scales) == len(sq_scales) == n):
-        raise ValueError("mpnn_amd.optim.adamw_step: lists of different lengths")
-    dev = params[0].device
-    _check(params, "parameters")
-    _check(grads, "gradients")
-    for p, g, m, v, a, b in zip(params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales):
-        k = p.numel()
-        want = torch.float32 if a is None else torch.float8_e4m3fn
-        if (a is None) != (b is None):
-            raise ValueError("mpnn_amd.optim.adamw_step: both moments of a tensor have scales, or none")
-        if g.numel() != k or m.numel() != k or v.numel() != k:
-            raise ValueError("mpnn_amd.optim.adamw_step: parameter, gradient and moments differ in size")
-        if m.dtype != want or v.dtype != want or not m.is_contiguous() or not v.is_contiguous():
-            raise ValueError("mpnn_amd.optim.adamw_step: moments must be contiguous fp32 tensors without scales, or "
-                             "float8_e4m3fn with scales")
-        if p.device != dev or g.device != dev or m.device != dev or v.device != dev:
-            raise RuntimeError("mpnn_amd.optim.adamw_step: all tensors must be on one device")
-        if a is not None:
-            blocks = -(-k // BLOCK)
-            if a.dtype != torch.float32 or b.dtype != torch.float32 or a.numel() != blocks or b.numel() != blocks or \
-                    not a.is_contiguous() or not b.is_contiguous() or a.device != dev or b.device != dev:
-                raise ValueError(f"mpnn_amd.optim.adamw_step: scales must be contiguous fp32 tensors of one element for each "
-                                 f"{BLOCK} of the parameter, on its device")
-
-
-def _mixed_call(params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales, step, lr, betas, eps, weight_decay, seed, first,
-                parts, max_norm, sumsq):
-    n = len(params)
-    numel = (ctypes.c_longlong * n)(*[p.numel() for p in params])
-    call("mpnn_adamw_mixed", n, _pointers(params), _pointers(grads), _pointers(exp_avgs), _pointers(exp_avg_sqs),
-         _pointers(scales), _pointers(sq_scales), numel, float(lr), float(betas[0]), float(betas[1]), float(eps),
-         float(weight_decay), int(step), int(seed) & 0xFFFFFFFF, first, ptr(parts), float(max_norm), ptr(sumsq), stream_ptr())
-
-
-def _sumsq_parts(grads):
-    parts = torch.empty(_PARTS, device=grads[0].device, dtype=torch.float64)
-    numel = (ctypes.c_longlong * len(grads))(*[g.numel() for g in grads])
-    call("mpnn_grad_sumsq_parts", len(grads), _pointers(grads), numel, ptr(parts), stream_ptr())
-    return parts
-
-
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, *, step, lr=1e-3,
                betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, seed=0, max_grad_norm=0.0):
     """One AdamW step over lists of tensors, in place.  params, grads: contiguous fp32.  Tensors whose scales are None keep
@@ -145,22 +96,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_
     with).  step: 1 for the first.  seed, step, the place in the list and the element decide the rounding of 8-bit moments.
     max_grad_norm > 0 clips by the norm over all gradients.  Returns the squared norm (a device scalar) then, else None.
     No two tensors may share memory."""
-    lists = [list(x) for x in (params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales)]
-    if len(lists[0]) == 0:
-        return None
-    _check_mixed(*lists)
-    if int(step) < 1:
-        raise ValueError("mpnn_amd.optim.adamw_step: step counts from 1")
-    with torch.no_grad(), torch.cuda.device(lists[0][0].device):
-        if any(p.numel() == 0 for p in lists[0]):
-            raise ValueError("mpnn_amd.optim.adamw_step: empty tensor")
-        parts = sumsq = None
-        if max_grad_norm > 0.0:
-            parts = _sumsq_parts(lists[1])
-            sumsq = torch.empty(1, device=parts.device, dtype=torch.float32)
-        _mixed_call(*lists, step, lr, betas, eps, weight_decay, seed, 0, parts, max_grad_norm, sumsq)
-        torch.autograd.graph.increment_version([t for x in lists[:1] + lists[2:] for t in x if t is not None])
-    return sumsq
+    return host_call("mpnn_adamw_mixed", "adamw", params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step,
+                     lr, betas[0], betas[1], eps, weight_decay, int(seed) & 0xFFFFFFFF, 0, max_grad_norm, None)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -244,34 +181,29 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     def _step_mixed(self, live, every):
-        with torch.cuda.device(every[0].device):
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("mpnn_amd.optim.AdamW(state_bits=8): a step counts on the host and cannot be captured into a "
-                                   "HIP graph")
-            parts = None
-            self.last_grad_sumsq = None
-            if self.max_grad_norm > 0.0:
-                parts = _sumsq_parts([p.grad for p in every])
-                self.last_grad_sumsq = torch.empty(1, device=parts.device, dtype=torch.float32)
-            first, changed = 0, []
-            for group, ps in zip(self.param_groups, live):
-                by_step = {}
-                for p in ps:
-                    st = self.state[p]
-                    if not st:
-                        st.update(self._new_state(p))
-                    st["step"] += 1
-                    by_step.setdefault(int(st["step"]), []).append(p)
-                for k, sel in sorted(by_step.items()):
-                    states = [self.state[p] for p in sel]
-                    lists = [sel, [p.grad for p in sel]] + [[st.get(n) for st in states] for n in
-                                                            ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
-                    _check_mixed(*lists)
-                    _mixed_call(*lists, k, group["lr"], group["betas"], group["eps"], group["weight_decay"], self.seed, first,
-                                parts, self.max_grad_norm, self.last_grad_sumsq)
-                    first += len(sel)
-                    changed += sel
-            torch.autograd.graph.increment_version(changed)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("mpnn_amd.optim.AdamW(state_bits=8): a step counts on the host and cannot be captured into a HIP "
+                               "graph")
+        parts, self.last_grad_sumsq = None, None
+        if self.max_grad_norm > 0.0:
+            parts = host_call("mpnn_grad_sumsq_parts", "grad_sumsq_parts", [p.grad for p in every])
+        first = 0
+        for group, ps in zip(self.param_groups, live):
+            by_step = {}
+            for p in ps:
+                st = self.state[p]
+                if not st:
+                    st.update(self._new_state(p))
+                st["step"] += 1
+                by_step.setdefault(int(st["step"]), []).append(p)
+            for k, sel in sorted(by_step.items()):
+                states = [self.state[p] for p in sel]
+                lists = [[st.get(n) for st in states] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
+                ss = host_call("mpnn_adamw_mixed", "adamw", sel, [p.grad for p in sel], *lists, k, group["lr"], group["betas"][0],
+                               group["betas"][1], group["eps"], group["weight_decay"], self.seed & 0xFFFFFFFF, first,
+                               self.max_grad_norm, parts)
+                self.last_grad_sumsq = ss if ss is not None else self.last_grad_sumsq
+                first += len(sel)
 
     def load_state_dict(self, state_dict):
         """Checkpoints of 8-bit and of 32-bit moments (this optimizer's, torch's) load into an optimizer of either width."""

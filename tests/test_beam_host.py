@@ -43,20 +43,19 @@ def test_bad_arguments_are_refused_by_the_library():
 
 
 def test_layouts():
-    from mpnn_amd.beam import _apart, _layout, _span
+    from mpnn_amd import _lib
 
+    layout, span = _lib.host().state_layout, _lib.host().state_span
     x = torch.zeros(2, 3, 4, 6, 8)
-    assert _layout(x, False) == (1, 0, 192) and _layout(x, True) == (4, 48, 48)
-    assert _layout(x[:, :, :, :5], False) == (4, 48, 40) and _layout(x[:, :, :, :5], True) == (4, 48, 40)
-    assert _layout(x[..., 0], False) == (24, 8, 1) and _layout(x[..., 0], True) is None
-    assert _layout(x[..., :7], False) == (24, 8, 7) and _layout(x[:, :, :3, :5, :7], False) is None
-    assert _layout(x[:, :, :1, :1, :1], False) == (1, 0, 1)
-    assert _span(x) == x.numel() and _span(x.expand(2, 3, 4, 6, 8)[:, :, :2]) == 1152 - 96
-    assert _span(torch.zeros(2, 1, 4).expand(2, 3, 4)) is None
-    assert _span(torch.zeros(30).as_strided((2, 3, 4), (12, 3, 1))) is None
-    a = (0, 100, (64, 32, 16), 8)
-    assert _apart(a, (8, 108, (64, 32, 16), 8)) and not _apart(a, (4, 104, (64, 32, 16), 8))
-    assert not _apart(a, (8, 108, (64, 32, 16), 9)) and not _apart(a, (8, 108, (64, 32, 24), 8))
+    assert layout(x, False) == (1, 0, 192) and layout(x, True) == (4, 48, 48)
+    assert layout(x[:, :, :, :5], False) == (4, 48, 40) and layout(x[:, :, :, :5], True) == (4, 48, 40)
+    assert layout(x[..., 0], False) == (24, 8, 1) and layout(x[..., 0], True) is None
+    assert layout(x[..., :7], False) == (24, 8, 7) and layout(x[:, :, :3, :5, :7], False) is None
+    assert layout(x[:, :, :1, :1, :1], False) == (1, 0, 1) and layout(x[:, :, :1, 0], True) == (1, 48, 8)
+    assert layout(torch.zeros(2, 3), False) == (1, 0, 1) and layout(torch.zeros(2, 3, 5), True) == (5, 1, 1)
+    assert span(x) == x.numel() and span(x.expand(2, 3, 4, 6, 8)[:, :, :2]) == 1152 - 96
+    assert span(torch.zeros(2, 1, 4).expand(2, 3, 4)) is None
+    assert span(torch.zeros(30).as_strided((2, 3, 4), (12, 3, 1))) is None
 
 
 def test_oracle_finds_the_best_sequences():
