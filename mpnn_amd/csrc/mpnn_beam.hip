@@ -38,10 +38,13 @@ __device__ __forceinline__ bool better(long long ka, int ia, long long kb, int i
 // candidate, token 0 with the score NaN: the failure stands in the first slot and takes no more than one.
 __device__ __forceinline__ bool broken(double score, double lse) { return lse != lse || !(score < INFINITY); }
 
-// exp(d) for d <= 0 to 1.1e-12 relative (2^f by a degree-8 polynomial, tools/fit_exp2.py; exactly 1 at 0); NaN stays NaN
+// exp(d) for d <= 0 to 1.1e-12 relative (2^f by a degree-8 polynomial, tools/fit_exp2.py; exactly 1 at 0).  d below -700 and
+// NaN count as -700: 1e-304, nothing beside a sum that holds a 1.  15 instructions: adding 1.5 * 2^52 rounds to the nearest
+// integer and leaves it in the low word, which goes straight into the exponent.
 __device__ __forceinline__ double exp_neg(double d) {
-  d = d < -800.0 ? -800.0 : d;
-  const double t = d * 1.4426950408889634, n = rint(t), f = t - n;
+  d = fmax(d, -700.0);
+  const double t = fma(d, 1.4426950408889634, 6755399441055744.0), n = t - 6755399441055744.0;
+  const double f = fma(d, 1.4426950408889634, -n);
   double p = 1.32552248847991267e-06;
   p = fma(p, f, 1.53100794023831035e-05);
   p = fma(p, f, 1.54034558524190164e-04);
@@ -51,7 +54,7 @@ __device__ __forceinline__ double exp_neg(double d) {
   p = fma(p, f, 2.40226506958129887e-01);
   p = fma(p, f, 6.93147180545933494e-01);
   p = fma(p, f, 1.0);
-  return ldexp(p, (int)n);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
 }
 
 template <typename T>
@@ -63,7 +66,33 @@ __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x)
 
 __device__ __forceinline__ double shfl_xor_d(double v, int o) { return __shfl_xor(v, o); }
 
-// the largest T for which at least q lanes have u >= T, or one that exactly q lanes reach (uniform result)
+// 32 bits that order values (NaN above all), and the least value that has at least those bits; fp64 by its high word
+template <typename X>
+struct Order;
+template <>
+struct Order<float> {
+  static __device__ __forceinline__ unsigned bits(float x, bool nan) {
+    const int b = __float_as_int(x + 0.0f);
+    return nan ? 0xffffffffu : (unsigned)(b ^ ((b >> 31) & 0x7fffffff)) ^ 0x80000000u;
+  }
+  static __device__ __forceinline__ float least(unsigned u) {
+    const int k = (int)(u ^ 0x80000000u), b = k ^ ((k >> 31) & 0x7fffffff);
+    return u <= 0x007fffffu ? -3.4028234663852886e38f : u >= 0xff800000u ? INFINITY : __int_as_float(b);
+  }
+};
+template <>
+struct Order<double> {
+  static __device__ __forceinline__ unsigned bits(double x, bool nan) {
+    return nan ? 0xffffffffu : (unsigned)(key_of(x) >> 32) ^ 0x80000000u;
+  }
+  static __device__ __forceinline__ double least(unsigned u) {   // u <= -inf's: everything but -inf
+    return u <= 0x000fffffu   ? -1.7976931348623157e308
+           : u >= 0xfff00000u ? INFINITY
+                              : value_of((long long)((unsigned long long)(u ^ 0x80000000u) << 32));
+  }
+};
+
+// some T that at least q lanes' u reach, and seldom half as many more (uniform): bisection over ballots
 __device__ __forceinline__ unsigned wave_kth(unsigned u, int q) {
   unsigned T = 0;
   for (int bit = 31; bit >= 0; --bit) {
@@ -71,7 +100,7 @@ __device__ __forceinline__ unsigned wave_kth(unsigned u, int q) {
     const int cnt = __popcll(__ballot(u >= t));
     if (cnt >= q) {
       T = t;
-      if (cnt == q) break;
+      if (cnt <= q + (q >> 1)) break;
     }
   }
   return T;
@@ -129,43 +158,51 @@ __device__ __forceinline__ void write_dead_slot(const SelectArgs& a, int b, int 
 // subgroups of g = 64 / (W rounded up to a power of two); lane j of a subgroup has tokens j, j + g, ...  No LDS
 // exchange before the winners are ranked, no barrier: at the model's 21 letters the call is bound by its own latency.
 // ---------------------------------------------------------------------------------------------------------------
+constexpr int SMALL_CAP = 512;   // candidates a wave ranks in LDS
+
 template <typename T, int M>
 __global__ void __launch_bounds__(64)
 k_select_small(SelectArgs a, int g_log2) {
-  __shared__ long long lk[SEL_MAX_N];
-  __shared__ int li[SEL_MAX_N];
+  __shared__ long long lk[SMALL_CAP];
+  __shared__ int li[SMALL_CAP];
   const int b = blockIdx.x, lane = threadIdx.x, g = 1 << g_log2;
   const int w = lane >> g_log2, j = lane & (g - 1);
   const bool live = w < a.W;
-  const double s = live ? (double)a.scores[(long long)b * a.W + w] : 0.0;
-  const long long f = live && a.forced ? a.forced[(long long)b * a.W + w] : -1;
+  const long long row = (long long)b * a.W + (live ? w : 0);
+  const double s = (double)a.scores[row];
+  const long long f = a.forced ? a.forced[row] : -1;
   double x[M];
   double top = -INFINITY;
+  bool nan = false;
   {
-    const T* row = (const T*)a.logits + (long long)b * a.sb + (long long)w * a.sw;
-    const float* bias = a.bias ? a.bias + (long long)b * a.bb + (long long)w * a.bw : nullptr;
+    const T* logits = (const T*)a.logits + (long long)b * a.sb + (live ? w : 0) * a.sw;
+    const float* bias = a.bias ? a.bias + (long long)b * a.bb + (live ? w : 0) * a.bw : nullptr;
+    T raw[M];
+    float add[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {      // every load is in flight before the first is used; places beyond V read the last one
+      const int v = j + (i << g_log2);
+      raw[i] = logits[v < a.V ? v : a.V - 1];
+      add[i] = bias ? bias[v < a.V ? v : a.V - 1] : 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < M; ++i) {
       const int v = j + (i << g_log2);
-      x[i] = -INFINITY;
-      if (live && v < a.V) {
-        x[i] = (double)to_f(row[v]);
-        if (bias) {
-          const float add = bias[v];
-          x[i] = add == -INFINITY ? -INFINITY : x[i] + (double)add;
-        }
-      }
+      x[i] = live && v < a.V && add[i] != -INFINITY ? (double)to_f(raw[i]) + (double)add[i] : -INFINITY;
       top = fmax(top, x[i]);
+      nan |= x[i] != x[i];
     }
   }
   for (int o = 1; o < g; o <<= 1) top = fmax(top, shfl_xor_d(top, o));
-  double sum = 0.0;
+  double sum = nan || top == INFINITY ? (double)NAN : 0.0;
+  const double base = top == -INFINITY ? 0.0 : top;
 #pragma unroll
-  for (int i = 0; i < M; ++i) sum += x[i] == -INFINITY ? 0.0 : exp_neg(x[i] - top);
+  for (int i = 0; i < M; ++i) sum += exp_neg(x[i] - base);
   for (int o = 1; o < g; o <<= 1) sum += shfl_xor_d(sum, o);
-  const double lse = top + log(sum);   // nothing left of the row: no candidate below
+  const double lse = base + log(sum);   // of no use where nothing is left of the row: no candidate below
   const bool bad = broken(s, lse);
   long long k[M];
+  long long best = KEY_NONE;
 #pragma unroll
   for (int i = 0; i < M; ++i) {
     const int v = j + (i << g_log2);
@@ -173,67 +210,89 @@ k_select_small(SelectArgs a, int g_log2) {
     if (bad) c = v == 0 ? (double)NAN : -INFINITY;
     if (f >= 0) c = v == (int)(f < a.V ? f : a.V - 1) ? s : -INFINITY;
     k[i] = live && v < a.V && !(c == -INFINITY) ? key_of(c) : KEY_NONE;
+    best = k[i] > best ? k[i] : best;
   }
-  // the n best: bisection over the keys' high words, then, where candidates tie there, their low words and places
-  int total = 0;
+  // at least n candidates reach the bound that n lanes' best ones do, seldom many more
+  int cnt = SMALL_CAP + 1;
+  if (a.n <= 64) {
+    const unsigned T32 = wave_kth((unsigned)(best >> 32) ^ 0x80000000u, a.n);
+    const long long bound = T32 ? (long long)((unsigned long long)(T32 ^ 0x80000000u) << 32) : KEY_NONE + 1;
+    cnt = 0;
 #pragma unroll
-  for (int i = 0; i < M; ++i) total += __popcll(__ballot(k[i] != KEY_NONE));
-  const int n = total < a.n ? total : a.n;
-  unsigned long long cut = 1;            // as unsigned words: KEY_NONE is 0
-  int last = 0x7fffffff;               // of the candidates that equal cut, those up to this place
-  if (total > n) {
-    cut = 0;
-    int cnt = total;
-    for (int bit = 63; bit >= 0 && cnt != n; --bit) {
-      const unsigned long long t = cut | (1ull << bit);
-      int c = 0;
-#pragma unroll
-      for (int i = 0; i < M; ++i) c += __popcll(__ballot(((unsigned long long)k[i] ^ (unsigned long long)KEY_NONE) >= t));
-      if (c >= n) {
-        cut = t;
-        cnt = c;
+    for (int i = 0; i < M; ++i) {
+      const bool in = k[i] >= bound && k[i] != KEY_NONE;
+      const unsigned long long m = __ballot(in);
+      const int p = cnt + __popcll(m & ((1ull << lane) - 1));
+      if (in && p < SMALL_CAP) {
+        lk[p] = k[i];
+        li[p] = w * a.V + j + (i << g_log2);
       }
+      cnt += __popcll(m);
     }
-    if (cnt > n) {                      // equal candidates: the lowest places of them
-      int above = 0;
+  }
+  if (cnt > SMALL_CAP) {
+    // many kept, or many equal ones: the n best exactly, by bisection over the keys and then over places of equal ones
+    int total = 0;
 #pragma unroll
-      for (int i = 0; i < M; ++i) above += __popcll(__ballot(((unsigned long long)k[i] ^ (unsigned long long)KEY_NONE) > cut));
-      int lo = 0, hi = a.W * a.V - 1;   // the smallest place p with above + #(equal, place <= p) >= n
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        int c = above;
+    for (int i = 0; i < M; ++i) total += __popcll(__ballot(k[i] != KEY_NONE));
+    const int n = total < a.n ? total : a.n;
+    unsigned long long cut = 1;            // as unsigned words: KEY_NONE is 0
+    int last = 0x7fffffff;                 // of the candidates that equal cut, those up to this place
+    if (total > n) {
+      cut = 0;
+      int reach = total;
+      for (int bit = 63; bit >= 0 && reach != n; --bit) {
+        const unsigned long long t = cut | (1ull << bit);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < M; ++i) c += __popcll(__ballot(((unsigned long long)k[i] ^ (unsigned long long)KEY_NONE) >= t));
+        if (c >= n) {
+          cut = t;
+          reach = c;
+        }
+      }
+      if (reach > n) {
+        int above = 0;
 #pragma unroll
         for (int i = 0; i < M; ++i)
-          c += __popcll(__ballot(((unsigned long long)k[i] ^ (unsigned long long)KEY_NONE) == cut &&
-                                 w * a.V + j + (i << g_log2) <= mid));
-        if (c >= n) hi = mid; else lo = mid + 1;
-      }
-      last = lo;
-    }
-  }
-  int at = 0;
+          above += __popcll(__ballot(((unsigned long long)k[i] ^ (unsigned long long)KEY_NONE) > cut));
+        int lo = 0, hi = a.W * a.V - 1;    // the smallest place p with above + #(equal, place <= p) >= n
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          int c = above;
 #pragma unroll
-  for (int i = 0; i < M; ++i) {
-    const unsigned long long u = (unsigned long long)k[i] ^ (unsigned long long)KEY_NONE;
-    const int place = w * a.V + j + (i << g_log2);
-    const bool in = u > cut || (u == cut && place <= last);
-    const unsigned long long m = __ballot(in);
-    if (in) {
-      const int p = at + __popcll(m & ((1ull << lane) - 1));
-      lk[p] = k[i];
-      li[p] = place;
+          for (int i = 0; i < M; ++i)
+            c += __popcll(__ballot(((unsigned long long)k[i] ^ (unsigned long long)KEY_NONE) == cut &&
+                                   w * a.V + j + (i << g_log2) <= mid));
+          if (c >= n) hi = mid; else lo = mid + 1;
+        }
+        last = lo;
+      }
     }
-    at += __popcll(m);
+    cnt = 0;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const unsigned long long u = (unsigned long long)k[i] ^ (unsigned long long)KEY_NONE;
+      const int place = w * a.V + j + (i << g_log2);
+      const bool in = u > cut || (u == cut && place <= last);
+      const unsigned long long m = __ballot(in);
+      if (in) {
+        const int p = cnt + __popcll(m & ((1ull << lane) - 1));
+        lk[p] = k[i];
+        li[p] = place;
+      }
+      cnt += __popcll(m);
+    }
   }
   __syncthreads();
-  for (int e = lane; e < n; e += 64) {
+  for (int e = lane; e < cnt; e += 64) {
     const long long ke = lk[e];
     const int ie = li[e];
     int r = 0;
-    for (int q = 0; q < n; ++q) r += better(lk[q], li[q], ke, ie);
-    write_slot(a, b, r, ke, ie);
+    for (int q = 0; q < cnt; ++q) r += better(lk[q], li[q], ke, ie);
+    if (r < a.n) write_slot(a, b, r, ke, ie);
   }
-  for (int e = n + lane; e < a.n; e += 64) write_dead_slot(a, b, e);
+  for (int e = cnt + lane; e < a.n; e += 64) write_dead_slot(a, b, e);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -273,6 +332,9 @@ __device__ __forceinline__ void block_best(long long& k, int& p, long long* sk, 
   for (int i = 1; i < 4; ++i)
     if (better(sk[i], sp[i], k, p)) { k = sk[i]; p = sp[i]; }
 }
+
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
 
 template <typename T, int U, bool BIAS>
 __global__ void __launch_bounds__(256)
@@ -327,29 +389,28 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
   bool nan = false;
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    tmax = x[i] > tmax ? x[i] : tmax;
+    tmax = max_of(tmax, x[i]);
     nan |= x[i] != x[i];
   }
   double top = (double)tmax;
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) top = fmax(top, shfl_xor_d(top, o));
-  const long long kt = nan ? KEY_NAN : key_of((double)tmax);
-  wave_bounds((unsigned)(kt >> 32) ^ 0x80000000u, a.n, ru);
+  wave_bounds(Order<X>::bits(tmax, nan), a.n, ru);
   if ((tid & 63) == 0) rd[wave] = top;
   if (tid == 0) rc = 0;
   __syncthreads();
   top = fmax(fmax(rd[0], rd[1]), fmax(rd[2], rd[3]));
-  const unsigned cut = block_bound(ru);
-  double sum = nan ? (double)NAN : 0.0;
+  const X least = Order<X>::least(block_bound(ru));
+  double sum = nan || top == INFINITY ? (double)NAN : 0.0;
+  const double from = top == -INFINITY ? 0.0 : top;
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const double xi = (double)x[i];
-    sum += xi == -INFINITY ? 0.0 : exp_neg(xi - top);
-    const long long k = key_of(xi);
-    if (xi != -INFINITY && ((unsigned)(k >> 32) ^ 0x80000000u) >= cut) {
+    sum += exp_neg(xi - from);
+    if (!(x[i] < least)) {
       const int p = atomicAdd(&rc, 1);
       if (p < SEL_CAP) {
-        lk[p] = k;
+        lk[p] = key_of(xi);
         li[p] = base + (i / VE * 256 + tid) * VE + i % VE;
       }
     }
@@ -361,7 +422,7 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
   __syncthreads();
   if (tid == 0) {
     my->top = top;
-    my->sum = (rd[0] + rd[1]) + (rd[2] + rd[3]);
+    my->sum = top == -INFINITY ? 0.0 : (rd[0] + rd[1]) + (rd[2] + rd[3]);
   }
   const int cnt = rc;
   if (cnt <= SEL_CAP) {
@@ -391,9 +452,12 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
   }
 }
 
-// Second pass, one workgroup a group: the beams' log-sum-exps from the slices', then the n best of the slices' lists.
+// Second pass, one workgroup a group: the beams' log-sum-exps from the slices', then the n best of the slices' lists.  E: list
+// entries a thread holds in registers, read before anything else (the pass is a chain of latencies); 0: any number, read
+// where they are needed.
+template <int E>
 __global__ void __launch_bounds__(256)
-k_select_merge(SelectArgs a, int splits, const SlicePart* __restrict__ part, const long long* __restrict__ pk,
+k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict__ part, const long long* __restrict__ pk,
                const int* __restrict__ pi) {
   __shared__ double lse[SEL_MAX_N];
   __shared__ float sc[SEL_MAX_N];
@@ -402,71 +466,98 @@ k_select_merge(SelectArgs a, int splits, const SlicePart* __restrict__ part, con
   __shared__ int rc;
   __shared__ long long lk[SEL_CAP];
   __shared__ int li[SEL_CAP];
-  const int b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  for (int w = wave; w < a.W; w += 4) {
-    const long long row = (long long)b * a.W + w;
-    const long long f = a.forced ? a.forced[row] : -1;
-    if (f < 0) {
-      const SlicePart* p = part + row * splits;
-      double top = -INFINITY, sum = 0.0;
-      for (int i = lane; i < splits; i += 64) top = fmax(top, p[i].top);
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int per = splits * a.n, total = a.W * per;
+  constexpr int R = E ? E : 1;
+  long long k[R];
+  int p[R];
+  if (E) {
 #pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) top = fmax(top, shfl_xor_d(top, o));
-      for (int i = lane; i < splits; i += 64) sum += p[i].top == -INFINITY ? p[i].sum : p[i].sum * exp(p[i].top - top);
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) sum += shfl_xor_d(sum, o);
-      if (lane == 0) lse[w] = top + log(sum);
+    for (int i = 0; i < R; ++i) {
+      const int e = tid + 256 * i;
+      const long long at = (long long)b * total + (e < total ? e : 0);
+      k[i] = pk[at];
+      p[i] = pi[at];
     }
-    if (lane == 0) {
-      sc[w] = a.scores[row];
+  }
+  // 2^g_log2 lanes a beam
+  const int g = 1 << g_log2, j = tid & (g - 1);
+  for (int w0 = 0; w0 < a.W; w0 += 256 >> g_log2) {
+    const int w = w0 + (tid >> g_log2);
+    const bool live = w < a.W;
+    const long long row = (long long)b * a.W + (live ? w : 0);
+    const long long f = a.forced ? a.forced[row] : -1;
+    const float score = a.scores[row];
+    double top = -INFINITY, sum = 0.0;
+    if (f < 0) {
+      const SlicePart* q = part + row * splits;
+      for (int i = j; i < splits; i += g) top = fmax(top, q[i].top);
+      for (int o = 1; o < g; o <<= 1) top = fmax(top, shfl_xor_d(top, o));
+      for (int i = j; i < splits; i += g) sum += q[i].top == -INFINITY ? q[i].sum : q[i].sum * exp_neg(q[i].top - top);
+      for (int o = 1; o < g; o <<= 1) sum += shfl_xor_d(sum, o);
+    }
+    if (live && j == 0) {
+      lse[w] = top + log(sum);
+      sc[w] = score;
       fc[w] = f < 0 ? -1 : (f < a.V ? (int)f : a.V - 1);
     }
   }
   if (tid == 0) rc = 0;
   __syncthreads();
-  const int per = splits * a.n, total = a.W * per;
-  auto candidate = [&](int e, long long& k, int& p) {
+  // entry e of the lists as a candidate
+  auto candidate = [&](int e, long long kx, int px, long long& ke, int& pe) {
+    ke = KEY_NONE;
+    pe = 0;
+    if (e >= total) return;
     const int w = e / per, r = e - w * per;
-    k = KEY_NONE;
-    p = 0;
     if (fc[w] >= 0) {
-      if (r == 0 && !(sc[w] == -INFINITY)) { k = key_of((double)sc[w]); p = w * a.V + fc[w]; }
-      return;
+      if (r == 0 && !(sc[w] == -INFINITY)) { ke = key_of((double)sc[w]); pe = w * a.V + fc[w]; }
+    } else if (broken((double)sc[w], lse[w])) {
+      if (r == 0) { ke = KEY_NAN; pe = w * a.V; }
+    } else if (kx != KEY_NONE) {
+      const double c = (double)sc[w] + (value_of(kx) - lse[w]);
+      if (c != -INFINITY) { ke = key_of(c); pe = w * a.V + px; }
     }
-    if (broken((double)sc[w], lse[w])) {
-      if (r == 0) { k = KEY_NAN; p = w * a.V; }
-      return;
-    }
-    const long long at = (long long)b * total + e, kx = pk[at];
-    if (kx == KEY_NONE) return;
-    const double c = (double)sc[w] + (value_of(kx) - lse[w]);
-    if (c == -INFINITY) return;
-    k = key_of(c);
-    p = w * a.V + pi[at];
+  };
+  auto entry = [&](int e, long long& ke, int& pe) {
+    const long long at = (long long)b * total + e;
+    candidate(e, pk[at], pi[at], ke, pe);
   };
   long long best = KEY_NONE;
-  for (int e = tid; e < total; e += 256) {
-    long long k;
-    int p;
-    candidate(e, k, p);
-    best = k > best ? k : best;
+  if (E) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      candidate(tid + 256 * i, k[i], p[i], k[i], p[i]);
+      best = k[i] > best ? k[i] : best;
+    }
+  } else {
+    for (int e = tid; e < total; e += 256) {
+      entry(e, k[0], p[0]);
+      best = k[0] > best ? k[0] : best;
+    }
   }
   wave_bounds((unsigned)(best >> 32) ^ 0x80000000u, a.n, ru);
   __syncthreads();
   const unsigned T = block_bound(ru);
-  for (int e = tid; e < total; e += 256) {
-    long long k;
-    int p;
-    candidate(e, k, p);
-    if (k != KEY_NONE && ((unsigned)(k >> 32) ^ 0x80000000u) >= T) {
+  auto collect = [&](long long ke, int pe) {
+    if (ke != KEY_NONE && ((unsigned)(ke >> 32) ^ 0x80000000u) >= T) {
       const int q = atomicAdd(&rc, 1);
-      if (q < SEL_CAP) { lk[q] = k; li[q] = p; }
+      if (q < SEL_CAP) { lk[q] = ke; li[q] = pe; }
+    }
+  };
+  if (E) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) collect(k[i], p[i]);
+  } else {
+    for (int e = tid; e < total; e += 256) {
+      entry(e, k[0], p[0]);
+      collect(k[0], p[0]);
     }
   }
   __syncthreads();
   const int cnt = rc;
   if (cnt <= SEL_CAP) {
-    rank_collected(lk, li, cnt, a.n, [&](int r, long long k, int p) { write_slot(a, b, r, k, p); });
+    rank_collected(lk, li, cnt, a.n, [&](int r, long long ke, int pe) { write_slot(a, b, r, ke, pe); });
     for (int r = cnt + tid; r < a.n; r += 256) write_dead_slot(a, b, r);
     return;
   }
@@ -475,20 +566,26 @@ k_select_merge(SelectArgs a, int splits, const SlicePart* __restrict__ part, con
   __shared__ long long sk[4];
   __shared__ int sp[4];
   for (int r = 0; r < a.n; ++r) {
-    long long k = KEY_NONE;
-    int p = 0x7fffffff;
-    for (int e = tid; e < total; e += 256) {
-      long long ke;
-      int pe;
-      candidate(e, ke, pe);
-      if (ke != KEY_NONE && better(prev, place, ke, pe) && better(ke, pe, k, p)) { k = ke; p = pe; }
+    long long kb = KEY_NONE;
+    int pb = 0x7fffffff;
+    auto improve = [&](long long ke, int pe) {
+      if (ke != KEY_NONE && better(prev, place, ke, pe) && better(ke, pe, kb, pb)) { kb = ke; pb = pe; }
+    };
+    if (E) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) improve(k[i], p[i]);
+    } else {
+      for (int e = tid; e < total; e += 256) {
+        entry(e, k[0], p[0]);
+        improve(k[0], p[0]);
+      }
     }
-    block_best(k, p, sk, sp);
+    block_best(kb, pb, sk, sp);
     if (tid == 0) {
-      if (k != KEY_NONE) write_slot(a, b, r, k, p); else write_dead_slot(a, b, r);
+      if (kb != KEY_NONE) write_slot(a, b, r, kb, pb); else write_dead_slot(a, b, r);
     }
-    prev = k;
-    place = p;
+    prev = kb;
+    place = pb;
   }
 }
 
@@ -542,7 +639,12 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
   else if (p.u == 16) MPNN_SLICE(16);
   else MPNN_SLICE(32);
 #undef MPNN_SLICE
-  hipLaunchKernelGGL(k_select_merge, dim3(a.B), dim3(256), 0, st, a, p.splits, part, pk, pi);
+  const long long total = (long long)a.W * p.splits * a.n;
+  int gl = 0;                               // lanes that share a beam's slices
+  while (gl < 6 && (1 << gl) < p.splits && (long long)a.W << (gl + 1) <= 256) ++gl;
+  if (total <= 1024) hipLaunchKernelGGL((k_select_merge<4>), dim3(a.B), block, 0, st, a, p.splits, gl, part, pk, pi);
+  else if (total <= 2048) hipLaunchKernelGGL((k_select_merge<8>), dim3(a.B), block, 0, st, a, p.splits, gl, part, pk, pi);
+  else hipLaunchKernelGGL((k_select_merge<0>), dim3(a.B), block, 0, st, a, p.splits, gl, part, pk, pi);
   MPNN_LAUNCH_CHECK();
 }
 
@@ -826,7 +928,6 @@ extern "C" int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int
   hipLaunchKernelGGL((k_beam_reorder<R>), grid, block, R ? 0 : (size_t)(64 << widest) * n_beams, (hipStream_t)stream, t, \
                      (const long long*)parent, n_beams, length_all, length, rank)
     if (n_beams <= 4) MPNN_REORDER(4);
-    else if (n_beams <= 8) MPNN_REORDER(8);
     else if (n_beams <= 16) MPNN_REORDER(16);
     else if (n_beams <= 32) MPNN_REORDER(32);
     else MPNN_REORDER(0);
