@@ -64,7 +64,30 @@ __device__ __forceinline__ float to_f<__hip_bfloat16>(__hip_bfloat16 x) { return
 template <>
 __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
 
-__device__ __forceinline__ double shfl_xor_d(double v, int o) { return __shfl_xor(v, o); }
+// Reductions over groups of g = 1, 2, 4 .. 64 neighbouring lanes, the result in every lane.  DPP moves (quad permutations,
+// mirrors of 8 and 16 lanes: the lanes they pair hold different parts of the sum) take a few cycles each, a shuffle through
+// the LDS crossbar a hundred, and every step of a reduction waits for the one before.
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, false),
+                          __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, false));
+}
+template <typename Op>
+__device__ __forceinline__ double group_reduce(double v, int g, Op op) {
+  if (g > 1) v = op(v, dpp_d<0xB1>(v));      // lane ^ 1
+  if (g > 2) v = op(v, dpp_d<0x4E>(v));      // lane ^ 2
+  if (g > 4) v = op(v, dpp_d<0x141>(v));     // mirrored in 8 lanes
+  if (g > 8) v = op(v, dpp_d<0x140>(v));     // mirrored in 16 lanes
+  if (g > 16) v = op(v, __shfl_xor(v, 16));
+  if (g > 32) v = op(v, __shfl_xor(v, 32));
+  return v;
+}
+__device__ __forceinline__ double group_max(double v, int g) {
+  return group_reduce(v, g, [](double a, double b) { return fmax(a, b); });
+}
+__device__ __forceinline__ double group_sum(double v, int g) {
+  return group_reduce(v, g, [](double a, double b) { return a + b; });
+}
 
 // 32 bits that order values (NaN above all), and the least value that has at least those bits; fp64 by its high word
 template <typename X>
@@ -95,6 +118,7 @@ struct Order<double> {
 // some T that at least q lanes' u reach, and seldom half as many more (uniform): bisection over ballots
 __device__ __forceinline__ unsigned wave_kth(unsigned u, int q) {
   unsigned T = 0;
+#pragma unroll 1
   for (int bit = 31; bit >= 0; --bit) {
     const unsigned t = T | (1u << bit);
     const int cnt = __popcll(__ballot(u >= t));
@@ -106,22 +130,22 @@ __device__ __forceinline__ unsigned wave_kth(unsigned u, int q) {
   return T;
 }
 
-// a bound that the n-th best of a 256-thread workgroup's values is no worse than, from each thread's best (u, 0 = none):
-// the least of the waves' ceil(n / 4)-th best threads, or the best of the waves' n-th best ones.  ru: 8 words of LDS,
-// written here; the caller's barrier follows, then block_bound reads them.
-__device__ __forceinline__ void wave_bounds(unsigned u, int n, unsigned* ru) {
-  const unsigned q = wave_kth(u, (n + 3) / 4), all = n <= 64 ? wave_kth(u, n) : 0;
-  if ((threadIdx.x & 63) == 0) {
-    ru[threadIdx.x >> 6] = q;
-    ru[4 + (threadIdx.x >> 6)] = all;
-  }
+// a bound that the n-th best of a 256-thread workgroup's values is no worse than, from each thread's best (u, 0 = none): the
+// least of the waves' ceil(n / 4)-th best threads where every thread has values (close to the n-th best), else the best of
+// the waves' n-th best threads, which threads without values do not spoil.  ru: 4 words of LDS, written here; the caller's
+// barrier follows, then block_bound reads them.
+__device__ __forceinline__ void wave_bounds(unsigned u, int n, bool full, unsigned* ru) {
+  const unsigned q = wave_kth(u, full || n > 64 ? (n + 3) / 4 : n);
+  if ((threadIdx.x & 63) == 0) ru[threadIdx.x >> 6] = q;
 }
-__device__ __forceinline__ unsigned block_bound(const unsigned* ru) {
-  const unsigned lo01 = ru[0] < ru[1] ? ru[0] : ru[1], lo23 = ru[2] < ru[3] ? ru[2] : ru[3], lo = lo01 < lo23 ? lo01 : lo23;
-  unsigned hi = ru[4];
+__device__ __forceinline__ unsigned block_bound(int n, bool full, const unsigned* ru) {
+  unsigned lo = ru[0], hi = ru[0];
 #pragma unroll
-  for (int i = 5; i < 8; ++i) hi = ru[i] > hi ? ru[i] : hi;
-  return lo > hi ? lo : hi;
+  for (int i = 1; i < 4; ++i) {
+    lo = ru[i] < lo ? ru[i] : lo;
+    hi = ru[i] > hi ? ru[i] : hi;
+  }
+  return full || n > 64 ? lo : hi;
 }
 
 struct SelectArgs {
@@ -193,12 +217,12 @@ k_select_small(SelectArgs a, int g_log2) {
       nan |= x[i] != x[i];
     }
   }
-  for (int o = 1; o < g; o <<= 1) top = fmax(top, shfl_xor_d(top, o));
+  top = group_max(top, g);
   double sum = nan || top == INFINITY ? (double)NAN : 0.0;
   const double base = top == -INFINITY ? 0.0 : top;
 #pragma unroll
   for (int i = 0; i < M; ++i) sum += exp_neg(x[i] - base);
-  for (int o = 1; o < g; o <<= 1) sum += shfl_xor_d(sum, o);
+  sum = group_sum(sum, g);
   const double lse = base + log(sum);   // of no use where nothing is left of the row: no candidate below
   const bool bad = broken(s, lse);
   long long k[M];
@@ -289,6 +313,7 @@ k_select_small(SelectArgs a, int g_log2) {
     const long long ke = lk[e];
     const int ie = li[e];
     int r = 0;
+#pragma unroll 8
     for (int q = 0; q < cnt; ++q) r += better(lk[q], li[q], ke, ie);
     if (r < a.n) write_slot(a, b, r, ke, ie);
   }
@@ -310,6 +335,7 @@ __device__ __forceinline__ void rank_collected(const long long* lk, const int* l
     const long long ke = lk[e];
     const int ie = li[e];
     int r = 0;
+#pragma unroll 8
     for (int q = 0; q < cnt; ++q) r += better(lk[q], li[q], ke, ie);
     if (r < n) put(r, ke, ie);
   }
@@ -340,7 +366,7 @@ template <typename T, int U, bool BIAS>
 __global__ void __launch_bounds__(256)
 k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long* __restrict__ pk, int* __restrict__ pi) {
   __shared__ double rd[4];
-  __shared__ unsigned ru[8];
+  __shared__ unsigned ru[4];
   __shared__ int rc;
   __shared__ long long lk[SEL_CAP];
   __shared__ int li[SEL_CAP];
@@ -393,14 +419,14 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
     nan |= x[i] != x[i];
   }
   double top = (double)tmax;
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) top = fmax(top, shfl_xor_d(top, o));
-  wave_bounds(Order<X>::bits(tmax, nan), a.n, ru);
+  top = group_max(top, 64);
+  const bool full = base >= 0 && base + 256 * U <= a.V;
+  wave_bounds(Order<X>::bits(tmax, nan), a.n, full, ru);
   if ((tid & 63) == 0) rd[wave] = top;
   if (tid == 0) rc = 0;
   __syncthreads();
   top = fmax(fmax(rd[0], rd[1]), fmax(rd[2], rd[3]));
-  const X least = Order<X>::least(block_bound(ru));
+  const X least = Order<X>::least(block_bound(a.n, full, ru));
   double sum = nan || top == INFINITY ? (double)NAN : 0.0;
   const double from = top == -INFINITY ? 0.0 : top;
 #pragma unroll
@@ -415,8 +441,7 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
       }
     }
   }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) sum += shfl_xor_d(sum, o);
+  sum = group_sum(sum, 64);
   __syncthreads();                     // rd has been read, the list is complete
   if ((tid & 63) == 0) rd[wave] = sum;
   __syncthreads();
@@ -452,34 +477,25 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
   }
 }
 
-// Second pass, one workgroup a group: the beams' log-sum-exps from the slices', then the n best of the slices' lists.  E: list
-// entries a thread holds in registers, read before anything else (the pass is a chain of latencies); 0: any number, read
-// where they are needed.
-template <int E>
+// Second pass, one workgroup a group: the beams' log-sum-exps from the slices', then the n best of the slices' lists.  The
+// lists are sorted, so their heads (one a thread) bound the n-th best from below and each list is followed down to that
+// bound only: an entry or two of it as a rule.  A chain of latencies, 7-9 us (17 us at 8 x 33 slices when every thread read
+// its share of all the lists).
 __global__ void __launch_bounds__(256)
 k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict__ part, const long long* __restrict__ pk,
                const int* __restrict__ pi) {
   __shared__ double lse[SEL_MAX_N];
   __shared__ float sc[SEL_MAX_N];
   __shared__ int fc[SEL_MAX_N];
-  __shared__ unsigned ru[8];
+  __shared__ unsigned ru[4];
   __shared__ int rc;
   __shared__ long long lk[SEL_CAP];
   __shared__ int li[SEL_CAP];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const int per = splits * a.n, total = a.W * per;
-  constexpr int R = E ? E : 1;
-  long long k[R];
-  int p[R];
-  if (E) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int e = tid + 256 * i;
-      const long long at = (long long)b * total + (e < total ? e : 0);
-      k[i] = pk[at];
-      p[i] = pi[at];
-    }
-  }
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const int lists = a.W * splits;
+  const long long* keys = pk + (long long)b * lists * a.n;
+  const int* places = pi + (long long)b * lists * a.n;
+  const long long head = keys[(long long)(tid < lists ? tid : 0) * a.n];   // under way while the sums are made
   // 2^g_log2 lanes a beam
   const int g = 1 << g_log2, j = tid & (g - 1);
   for (int w0 = 0; w0 < a.W; w0 += 256 >> g_log2) {
@@ -492,10 +508,13 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
     if (f < 0) {
       const SlicePart* q = part + row * splits;
       for (int i = j; i < splits; i += g) top = fmax(top, q[i].top);
-      for (int o = 1; o < g; o <<= 1) top = fmax(top, shfl_xor_d(top, o));
-      for (int i = j; i < splits; i += g) sum += q[i].top == -INFINITY ? q[i].sum : q[i].sum * exp_neg(q[i].top - top);
-      for (int o = 1; o < g; o <<= 1) sum += shfl_xor_d(sum, o);
     }
+    top = group_max(top, g);
+    if (f < 0) {
+      const SlicePart* q = part + row * splits;
+      for (int i = j; i < splits; i += g) sum += q[i].top == -INFINITY ? q[i].sum : q[i].sum * exp_neg(q[i].top - top);
+    }
+    sum = group_sum(sum, g);
     if (live && j == 0) {
       lse[w] = top + log(sum);
       sc[w] = score;
@@ -504,54 +523,44 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
   }
   if (tid == 0) rc = 0;
   __syncthreads();
-  // entry e of the lists as a candidate
-  auto candidate = [&](int e, long long kx, int px, long long& ke, int& pe) {
-    ke = KEY_NONE;
-    pe = 0;
-    if (e >= total) return;
-    const int w = e / per, r = e - w * per;
-    if (fc[w] >= 0) {
-      if (r == 0 && !(sc[w] == -INFINITY)) { ke = key_of((double)sc[w]); pe = w * a.V + fc[w]; }
-    } else if (broken((double)sc[w], lse[w])) {
-      if (r == 0) { ke = KEY_NAN; pe = w * a.V; }
-    } else if (kx != KEY_NONE) {
-      const double c = (double)sc[w] + (value_of(kx) - lse[w]);
-      if (c != -INFINITY) { ke = key_of(c); pe = w * a.V + px; }
-    }
+  // entry r of list l, whose key is kx, as a candidate's key
+  auto candidate = [&](int l, int r, long long kx) -> long long {
+    const int w = l / splits;
+    const bool first = r == 0 && l == w * splits;
+    if (fc[w] >= 0) return first && !(sc[w] == -INFINITY) ? key_of((double)sc[w]) : KEY_NONE;
+    if (broken((double)sc[w], lse[w])) return first ? KEY_NAN : KEY_NONE;
+    if (kx == KEY_NONE) return KEY_NONE;
+    const double c = (double)sc[w] + (value_of(kx) - lse[w]);
+    return c == -INFINITY ? KEY_NONE : key_of(c);
   };
-  auto entry = [&](int e, long long& ke, int& pe) {
-    const long long at = (long long)b * total + e;
-    candidate(e, pk[at], pi[at], ke, pe);
+  auto place_of = [&](int l, int px) -> int {
+    const int w = l / splits;
+    if (fc[w] >= 0) return w * a.V + fc[w];
+    return w * a.V + (broken((double)sc[w], lse[w]) ? 0 : px);
   };
-  long long best = KEY_NONE;
-  if (E) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      candidate(tid + 256 * i, k[i], p[i], k[i], p[i]);
-      best = k[i] > best ? k[i] : best;
-    }
-  } else {
-    for (int e = tid; e < total; e += 256) {
-      entry(e, k[0], p[0]);
-      best = k[0] > best ? k[0] : best;
-    }
+  long long best = tid < lists ? candidate(tid, 0, head) : KEY_NONE;
+  for (int l = tid + 256; l < lists; l += 256) {
+    const long long k = candidate(l, 0, keys[(long long)l * a.n]);
+    best = k > best ? k : best;
   }
-  wave_bounds((unsigned)(best >> 32) ^ 0x80000000u, a.n, ru);
+  wave_bounds((unsigned)(best >> 32) ^ 0x80000000u, a.n, false, ru);
   __syncthreads();
-  const unsigned T = block_bound(ru);
-  auto collect = [&](long long ke, int pe) {
-    if (ke != KEY_NONE && ((unsigned)(ke >> 32) ^ 0x80000000u) >= T) {
-      const int q = atomicAdd(&rc, 1);
-      if (q < SEL_CAP) { lk[q] = ke; li[q] = pe; }
-    }
-  };
-  if (E) {
+  const unsigned T = block_bound(a.n, false, ru);
+  for (int l = tid; l < lists; l += 256) {
+    bool more = true;
+    for (int r0 = 0; r0 < a.n && more; r0 += 4) {
+      long long k[4];
 #pragma unroll
-    for (int i = 0; i < R; ++i) collect(k[i], p[i]);
-  } else {
-    for (int e = tid; e < total; e += 256) {
-      entry(e, k[0], p[0]);
-      collect(k[0], p[0]);
+      for (int i = 0; i < 4; ++i) k[i] = keys[(long long)l * a.n + (r0 + i < a.n ? r0 + i : 0)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long ke = r0 + i < a.n ? candidate(l, r0 + i, k[i]) : KEY_NONE;
+        more = more && ke != KEY_NONE && ((unsigned)(ke >> 32) ^ 0x80000000u) >= T;
+        if (more) {
+          const int q = atomicAdd(&rc, 1);
+          if (q < SEL_CAP) { lk[q] = ke; li[q] = place_of(l, places[(long long)l * a.n + r0 + i]); }
+        }
+      }
     }
   }
   __syncthreads();
@@ -561,6 +570,7 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
     for (int r = cnt + tid; r < a.n; r += 256) write_dead_slot(a, b, r);
     return;
   }
+  // more ties than the list holds: one after the other
   long long prev = KEY_NAN;
   int place = -1;
   __shared__ long long sk[4];
@@ -568,17 +578,12 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
   for (int r = 0; r < a.n; ++r) {
     long long kb = KEY_NONE;
     int pb = 0x7fffffff;
-    auto improve = [&](long long ke, int pe) {
-      if (ke != KEY_NONE && better(prev, place, ke, pe) && better(ke, pe, kb, pb)) { kb = ke; pb = pe; }
-    };
-    if (E) {
-#pragma unroll
-      for (int i = 0; i < R; ++i) improve(k[i], p[i]);
-    } else {
-      for (int e = tid; e < total; e += 256) {
-        entry(e, k[0], p[0]);
-        improve(k[0], p[0]);
-      }
+    for (int e = tid; e < lists * a.n; e += 256) {
+      const int l = e / a.n;
+      const long long ke = candidate(l, e - l * a.n, keys[e]);
+      if (ke == KEY_NONE) continue;
+      const int pe = place_of(l, places[e]);
+      if (better(prev, place, ke, pe) && better(ke, pe, kb, pb)) { kb = ke; pb = pe; }
     }
     block_best(kb, pb, sk, sp);
     if (tid == 0) {
@@ -606,10 +611,10 @@ inline SelectPlan select_plan(long long B, int W, int V, int item) {
       return p;
     }
   }
-  // the largest slice that still gives every CU four workgroups; short rows take the smallest that holds them
+  // 16 values a thread once that gives every CU four workgroups, 8 below (32 x 8 x 131072: 78 us with 16, 86 with 32 - the
+  // registers let four waves a SIMD run instead of six - and 102 with 8, twice the per-slice work)
   const int ve = 16 / item;
-  p.u = 32;
-  while (p.u > 8 && B * W * ((V + ve - 1 + 256LL * p.u - 1) / (256LL * p.u)) < 1024) p.u >>= 1;
+  p.u = B * W * ((V + ve - 1 + 4095LL) / 4096) < 1024 ? 8 : 16;
   p.splits = (int)((V + ve - 1 + 256LL * p.u - 1) / (256LL * p.u));
   return p;
 }
@@ -636,15 +641,11 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
     else hipLaunchKernelGGL((k_select_slice<T, U, false>), grid, block, 0, st, a, p.splits, part, pk, pi);       \
   } while (0)
   if (p.u == 8) MPNN_SLICE(8);
-  else if (p.u == 16) MPNN_SLICE(16);
-  else MPNN_SLICE(32);
+  else MPNN_SLICE(16);
 #undef MPNN_SLICE
-  const long long total = (long long)a.W * p.splits * a.n;
   int gl = 0;                               // lanes that share a beam's slices
   while (gl < 6 && (1 << gl) < p.splits && (long long)a.W << (gl + 1) <= 256) ++gl;
-  if (total <= 1024) hipLaunchKernelGGL((k_select_merge<4>), dim3(a.B), block, 0, st, a, p.splits, gl, part, pk, pi);
-  else if (total <= 2048) hipLaunchKernelGGL((k_select_merge<8>), dim3(a.B), block, 0, st, a, p.splits, gl, part, pk, pi);
-  else hipLaunchKernelGGL((k_select_merge<0>), dim3(a.B), block, 0, st, a, p.splits, gl, part, pk, pi);
+  hipLaunchKernelGGL(k_select_merge, dim3(a.B), block, 0, st, a, p.splits, gl, part, pk, pi);
   MPNN_LAUNCH_CHECK();
 }
 
