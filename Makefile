@@ -43,10 +43,10 @@ $(CSRC)/mpnn_loss.o: $(CSRC)/mpnn_loss.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_ab
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
 # -packed-fp32-ops: no v_pk_*_f32 (some of their forms gave wrong results on this hardware)
-$(CSRC)/mpnn_beam.o: $(CSRC)/mpnn_beam.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_ablation.h include/mpnn_hip.h
+$(CSRC)/mpnn_beam.o: $(CSRC)/mpnn_beam.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_reduce.h $(CSRC)/mpnn_ablation.h include/mpnn_hip.h
 	$(HIPCC) $(HIPFLAGS) -ffp-contract=off -c $< -o $@
 
-$(CSRC)/mpnn_optim.o: $(CSRC)/mpnn_optim.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_ablation.h include/mpnn_hip.h
+$(CSRC)/mpnn_optim.o: $(CSRC)/mpnn_optim.hip $(CSRC)/mpnn_common.h $(CSRC)/mpnn_reduce.h $(CSRC)/mpnn_ablation.h include/mpnn_hip.h
 	$(HIPCC) $(HIPFLAGS) -ffp-contract=off -c $< -o $@
 
 $(OUT): $(OBJS)

@@ -319,15 +319,16 @@ PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 // ---- optimizer ----
-constexpr int kBlock = 64, kParts = 1024;
+constexpr int kBlock = 64, kParts = 256;
 
 void check_dense(const at::Tensor& t, const char* what) {
-  if (!t.is_cuda() || t.scalar_type() != at::kFloat || !t.is_contiguous())
+  const c10::TensorImpl* x = t.unsafeGetTensorImpl();
+  if (!x->is_cuda() || x->dtype() != caffe2::TypeMeta::fromScalarType(at::kFloat) || !x->is_contiguous())
     runtime_error(std::string("mpnn_amd.optim: ") + what +
                   " must be contiguous fp32 tensors on a ROCm device (the HIP path has no CPU fallback)");
 }
 
-// grad_sumsq_parts(grads) -> float64 [1024]
+// grad_sumsq_parts(grads) -> float64 [256]
 at::Tensor sumsq_parts(const Items& grads) {
   std::vector<const float*> p(grads.n);
   std::vector<long long> numel(grads.n);
@@ -373,23 +374,26 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     std::vector<long long> numel(n);
     const c10::Device dev = tensor(P.at[0], "optim", "parameters").device();
     const char* name = "optim.adamw_step";
+    const auto fp32 = caffe2::TypeMeta::fromScalarType(at::kFloat), fp8 = caffe2::TypeMeta::fromScalarType(at::kFloat8_e4m3fn);
     for (Py_ssize_t i = 0; i < n; ++i) {
       const at::Tensor &tp = tensor(P.at[i], name, "params"), &tg = tensor(G.at[i], name, "grads"),
                        &tm = tensor(M.at[i], name, "exp_avgs"), &tv = tensor(V.at[i], name, "exp_avg_sqs");
       check_dense(tp, "parameters");
       check_dense(tg, "gradients");
-      const long long k = tp.numel();
+      const c10::TensorImpl *xp = tp.unsafeGetTensorImpl(), *xg = tg.unsafeGetTensorImpl(), *xm = tm.unsafeGetTensorImpl(),
+                            *xv = tv.unsafeGetTensorImpl();
+      const long long k = xp->numel();
       const bool wide = A.at[i] != Py_None;
       if (wide != (S.at[i] != Py_None))
         value_error("mpnn_amd.optim.adamw_step: both moments of a tensor have scales, or none");
       if (!k) value_error("mpnn_amd.optim.adamw_step: empty tensor");
-      if (tg.numel() != k || tm.numel() != k || tv.numel() != k)
+      if (xg->numel() != k || xm->numel() != k || xv->numel() != k)
         value_error("mpnn_amd.optim.adamw_step: parameter, gradient and moments differ in size");
-      const auto want = wide ? at::kFloat8_e4m3fn : at::kFloat;
-      if (tm.scalar_type() != want || tv.scalar_type() != want || !tm.is_contiguous() || !tv.is_contiguous())
+      const auto want = wide ? fp8 : fp32;
+      if (xm->dtype() != want || xv->dtype() != want || !xm->is_contiguous() || !xv->is_contiguous())
         value_error("mpnn_amd.optim.adamw_step: moments must be contiguous fp32 tensors without scales, or float8_e4m3fn with "
                     "scales");
-      if (tp.device() != dev || tg.device() != dev || tm.device() != dev || tv.device() != dev)
+      if (xp->device() != dev || xg->device() != dev || xm->device() != dev || xv->device() != dev)
         runtime_error("mpnn_amd.optim.adamw_step: all tensors must be on one device");
       p[i] = (float*)tp.data_ptr();
       g[i] = (const float*)tg.const_data_ptr();
@@ -400,10 +404,12 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       if (wide) {
         const at::Tensor &ta = tensor(A.at[i], name, "exp_avg_scales"), &ts = tensor(S.at[i], name, "exp_avg_sq_scales");
         const long long blocks = (k + kBlock - 1) / kBlock;
-        for (const at::Tensor* t : {&ta, &ts})
-          if (t->scalar_type() != at::kFloat || t->numel() != blocks || !t->is_contiguous() || t->device() != dev)
+        for (const at::Tensor* t : {&ta, &ts}) {
+          const c10::TensorImpl* x = t->unsafeGetTensorImpl();
+          if (x->dtype() != fp32 || x->numel() != blocks || !x->is_contiguous() || x->device() != dev)
             value_error("mpnn_amd.optim.adamw_step: scales must be contiguous fp32 tensors of one element for each 64 of the "
                         "parameter, on its device");
+        }
         ms[i] = (float*)ta.data_ptr();
         vs[i] = (float*)ts.data_ptr();
       }

@@ -18,26 +18,33 @@
 
 #include "mpnn_common.h"
 #include "mpnn_hip.h"
+#include "mpnn_reduce.h"
 
 namespace {
 
-constexpr int AW_MAX = 60;       // tensors of a launch: the table travels as a kernel argument of less than 4 KB
-constexpr int AW_CHUNK = 2048;   // elements of a workgroup's turn
+constexpr int AW_MAX = 120;      // tensors of a launch: the table travels as a kernel argument of less than 4 KB
+constexpr int AW_CHUNK = 1024;   // elements of a workgroup's turn: four a thread
+constexpr int AW_WGS = 16384;    // workgroups of a launch at most (100 M parameters: 429 us with 8192 or 16384, 457 with 2048)
 constexpr int AW_BLOCK = 64;     // elements that share a scale: 16 lanes of four elements
-constexpr int AW_PARTS = 1024;   // workgroups (and partial sums) of the norm, over all launches of a call
+constexpr int AW_PARTS = 256;    // workgroups (and partial sums) of the norm, over all launches of a call
+constexpr int NT_THREADS = 1024;
+constexpr int NT_CHUNK = 4 * NT_THREADS * 4;   // elements of a workgroup's turn in the norm
 constexpr int NT_MAX = 128;      // tensors of a launch of the norm
 
+// A tensor's six addresses as distances from those of the first tensor of its kind, in units of four bytes: 32 bytes a
+// tensor, where pointers take 56 and two launches for the model's 118 tensors.  A tensor that lies 8 GB away from the first
+// (or whose codes have another residue modulo four) opens the next table.
+struct Origin {
+  char *p, *g, *m, *v, *ms, *vs;
+};
 struct AdamTable {
-  float* p[AW_MAX];
-  const float* g[AW_MAX];
-  void* m[AW_MAX];
-  void* v[AW_MAX];
-  float* ms[AW_MAX];             // scales; NULL = 32-bit moments
-  float* vs[AW_MAX];
-  long long numel[AW_MAX];
+  Origin origin[2];              // of 32-bit moments, of 8-bit ones
+  int p[AW_MAX], g[AW_MAX], m[AW_MAX], v[AW_MAX], ms[AW_MAX], vs[AW_MAX];   // ms: NO_SCALE for 32-bit moments
+  unsigned numel[AW_MAX];
   int chunk0[AW_MAX + 1];        // first chunk of each tensor
   int n;
 };
+constexpr int NO_SCALE = (int)0x80000000;
 
 struct NormTable {
   const float* g[NT_MAX];
@@ -55,8 +62,8 @@ struct AdamHyper {
   unsigned key, tensor0;
 };
 
-__host__ __device__ __forceinline__ unsigned hash_bits(unsigned id, unsigned seed) {  // as dropout_keep's (mpnn_edge_common.h)
-  unsigned h = (id * 0x9E3779B1u) ^ seed;
+// 32 bits of a counter and a seed, as dropout_keep's (mpnn_edge_common.h)
+__host__ __device__ __forceinline__ unsigned mix_bits(unsigned h) {
   h ^= h >> 16;
   h *= 0x85EBCA6Bu;
   h ^= h >> 13;
@@ -64,6 +71,7 @@ __host__ __device__ __forceinline__ unsigned hash_bits(unsigned id, unsigned see
   h ^= h >> 16;
   return h;
 }
+__host__ __device__ __forceinline__ unsigned hash_bits(unsigned id, unsigned seed) { return mix_bits((id * 0x9E3779B1u) ^ seed); }
 
 // tensor of a chunk: each lane compares an entry of the table (or two)
 template <typename Table>
@@ -77,40 +85,47 @@ __device__ __forceinline__ int tensor_of(const Table& t, int chunk) {
   return __builtin_amdgcn_readfirstlane(at);
 }
 
+// sum over the workgroup, in every thread
+template <int WAVES>
 __device__ __forceinline__ double block_sum(double s, double* sh) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+  s = group_sum(s, 64);
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
   __syncthreads();
-  return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) s += sh[i];
+  return s;
 }
 
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(NT_THREADS)
 k_grad_sumsq_parts(NormTable t, double* __restrict__ parts) {
-  __shared__ double sh[4];
+  __shared__ double sh[NT_THREADS / 64];
   double s = 0.0;
   for (int chunk = blockIdx.x; chunk < t.chunk0[t.n]; chunk += gridDim.x) {
     const int ti = tensor_of(t, chunk);
     const float* __restrict__ g = t.g[ti];
-    const long long n = t.numel[ti], i0 = (long long)(chunk - t.chunk0[ti]) * AW_CHUNK;
-    const bool wide = ((uintptr_t)g & 15) == 0 && i0 + AW_CHUNK <= n;
-    if (wide) {
+    const long long n = t.numel[ti], i = (long long)(chunk - t.chunk0[ti]) * NT_CHUNK + threadIdx.x * 4;
+    constexpr int ROW = 4 * NT_THREADS;
+    if (((uintptr_t)g & 15) == 0 && i + NT_CHUNK - ROW + 4 <= n) {   // this thread's last four included
+      f32x4 x[NT_CHUNK / ROW];
 #pragma unroll
-      for (int it = 0; it < AW_CHUNK / 1024; ++it) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(g + i0 + it * 1024 + threadIdx.x * 4);
+      for (int k = 0; k < NT_CHUNK / ROW; ++k) x[k] = *reinterpret_cast<const f32x4*>(g + i + ROW * k);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s += (double)x[i] * (double)x[i];
-      }
+      for (int k = 0; k < NT_CHUNK / ROW; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += (double)x[k][j] * (double)x[k][j];
     } else {
-      for (long long i = i0 + threadIdx.x; i < n && i < i0 + AW_CHUNK; i += 256) s += (double)g[i] * (double)g[i];
+      for (int k = 0; k < NT_CHUNK; k += ROW)
+        for (int j = 0; j < 4; ++j)
+          if (i + k + j < n) s += (double)g[i + k + j] * (double)g[i + k + j];
     }
   }
-  s = block_sum(s, sh);
+  s = block_sum<NT_THREADS / 64>(s, sh);
   if (threadIdx.x == 0) parts[blockIdx.x] = s;
 }
 
-__device__ __forceinline__ unsigned hi_word(double x) { return (unsigned)(__double_as_longlong(x) >> 32); }
-__device__ __forceinline__ double pow2(int e) { return __longlong_as_double((long long)(1023 + e) << 52); }
+__device__ __forceinline__ unsigned hi_word(double x) { return (unsigned)__double2hiint(x); }
+__device__ __forceinline__ double pow2(int e) { return __hiloint2double((1023 + e) << 20, 0); }
 
 // largest of 16 lanes (a DPP row): the 64 elements that share a scale
 __device__ __forceinline__ unsigned row_max(unsigned x) {
@@ -124,157 +139,226 @@ __device__ __forceinline__ unsigned row_max(unsigned x) {
   return x;
 }
 
-// exponent of a block's scale from the high word of its largest magnitude: the largest lands in [128, 256)
-__device__ __forceinline__ bool scale_exponent(unsigned top, int& e) {
-  e = (int)(top >> 20) - 1023 - 7;
-  e = e < -126 ? -126 : e;
-  if (top == 0) e = 0;
-  return (top >> 20) < 1023 + 128;    // else infinite, NaN or beyond fp32: the block's scale becomes NaN
-}
-
-// |x| / scale as an e4m3 code, rounded up with probability r / 65536 of the part cut off.  floor(y / step + u) with u a
-// multiple of 2^-16 needs the 19 leading mantissa bits of y only: the high word has 20.
-__device__ __forceinline__ unsigned to_code(double x, double inv, unsigned r) {
-  const double y = fabs(x) * inv;
-  const unsigned normal = ((hi_word(y) + (r << 1)) >> 17) - (1016u << 3);
-  const unsigned small = (unsigned)(int)floor(fma(y, 512.0, (double)r * 0x1p-16));   // below 2^-6 the step is 2^-9
-  return y >= 0x1p-6 ? normal : small;
-}
+// What turns a block's moments into codes, from the high word of the largest: the scale's exponent e puts that one into
+// [128, 256) scales.  A moment's code is floor(y / step + r / 65536), y = |x| / scale, r 16 random bits.  Above 2^-6 the
+// step is an eighth of y's power of two: r added to the mantissa's high word 17 bits down, what is left above them is the
+// code (the floor depends on the 19 leading mantissa bits only, the high word has 20).  Below, the step is 2^-9 and y a
+// fixed-point number.
+struct Encoder {
+  bool finite;
+  unsigned rebias, normal;    // from the high word to e4m3's exponent; the least high word of a code above 2^-6
+  double fixed;               // 2^25 / scale
+  float scale;
+  __device__ __forceinline__ explicit Encoder(unsigned top) {
+    int e = (int)(top >> 20) - 1023 - 7;
+    e = e < -126 ? -126 : e;
+    if (top == 0) e = 0;
+    finite = (top >> 20) < 1023 + 128;    // else infinite, NaN or beyond fp32
+    rebias = (unsigned)(-e - 1016) << 20;
+    normal = (unsigned)(1023 - 6 + e) << 20;
+    fixed = pow2(25 - e);
+    scale = finite ? __int_as_float((127 + e) << 23) : NAN;
+  }
+  __device__ __forceinline__ unsigned code(double x, unsigned r) const {
+    const unsigned hi = hi_word(x) & 0x7fffffffu;
+    const unsigned above = (hi + rebias + (r << 1)) >> 17;
+    const unsigned below = ((unsigned)__double2uint_rz(fabs(x) * fixed) + r) >> 16;
+    const unsigned c = hi >= normal ? above : below;
+    return finite ? c : 0u;
+  }
+};
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ void decode4(unsigned codes, float scale, double (&x)[4]) {
+__device__ __forceinline__ void decode4(unsigned codes, double (&x)[4]) {
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
-  const double s = (double)scale;
-  x[0] = (double)a.x * s;
-  x[1] = (double)a.y * s;
-  x[2] = (double)b.x * s;
-  x[3] = (double)b.y * s;
+  x[0] = (double)a.x;
+  x[1] = (double)a.y;
+  x[2] = (double)b.x;
+  x[3] = (double)b.y;
 }
 
+// The update in fp32.  The square root and the reciprocal are the hardware's (within one step of the last place; the move
+// they scale is a small part of p): correctly rounded ones are a third of the kernel's instructions.  They count fp32
+// denormals as zero, which shows where eps does not cover sqrt(2^-126) only: then the exact ones run.
 __device__ __forceinline__ float adam_update(float p, double m, double v, const AdamHyper& h) {
+  if (h.eps >= 1e-12f) {
+    const float d = fmaf(__builtin_amdgcn_sqrtf((float)v), h.root, h.eps);
+    return fmaf(p, h.decay, -h.rate * ((float)m * __builtin_amdgcn_rcpf(d)));
+  }
   return p * h.decay - h.rate * ((float)m / (sqrtf((float)v) * h.root + h.eps));
+}
+
+// four elements of a thread on their way through the step
+struct Four {
+  float* p;
+  void *m, *v;
+  float *ms, *vs;                // of the block; NULL: 32-bit moments
+  unsigned key, id;
+  int left;                      // of the four that exist
+  bool wide;                     // moved as vectors
+  f32x4 pv, gv, mv, vv;          // 8-bit moments: four codes in mv[0], vv[0], the scale in mv[1], vv[1]
+};
+
+__device__ __forceinline__ void load_four(const AdamTable& t, const AdamHyper& h, int chunk, Four& c) {
+  const int ti = tensor_of(t, chunk);
+  const long long n = t.numel[ti], i = (long long)(chunk - t.chunk0[ti]) * AW_CHUNK + threadIdx.x * 4;
+  const bool eight = t.ms[ti] != NO_SCALE;
+  const Origin& o = t.origin[eight];
+  const float* g = (const float*)(o.g + 4LL * t.g[ti]);
+  char *m = o.m + 4LL * t.m[ti], *v = o.v + 4LL * t.v[ti];
+  c.left = i >= n ? 0 : n - i < 4 ? (int)(n - i) : 4;
+  c.p = (float*)(o.p + 4LL * t.p[ti]) + i;
+  c.pv = c.gv = c.mv = c.vv = f32x4{0.f, 0.f, 0.f, 0.f};
+  c.id = (unsigned)i * 0x9E3779B1u;
+  c.key = h.tensor0 + ti;
+  if (eight) {
+    c.m = m + i;
+    c.v = v + i;
+    c.ms = (float*)(o.ms + 4LL * t.ms[ti]) + i / AW_BLOCK;
+    c.vs = (float*)(o.vs + 4LL * t.vs[ti]) + i / AW_BLOCK;
+    c.wide = c.left == 4 && (((uintptr_t)c.p | (uintptr_t)(g + i)) & 15) == 0 && (((uintptr_t)c.m | (uintptr_t)c.v) & 3) == 0;
+    unsigned mc = 0, vc = 0;
+    if (c.wide) {
+      mc = *(const unsigned*)c.m;
+      vc = *(const unsigned*)c.v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < c.left) {
+          mc |= (unsigned)((const unsigned char*)c.m)[j] << (8 * j);
+          vc |= (unsigned)((const unsigned char*)c.v)[j] << (8 * j);
+        }
+    }
+    c.mv[0] = __uint_as_float(mc);
+    c.vv[0] = __uint_as_float(vc);
+    c.mv[1] = c.left ? *c.ms : 1.f;
+    c.vv[1] = c.left ? *c.vs : 1.f;
+  } else {
+    c.m = (float*)m + i;
+    c.v = (float*)v + i;
+    c.ms = c.vs = nullptr;
+    c.wide = c.left == 4 && (((uintptr_t)c.p | (uintptr_t)(g + i) | (uintptr_t)c.m | (uintptr_t)c.v) & 15) == 0;
+    if (c.wide) {
+      c.mv = *(const f32x4*)c.m;
+      c.vv = *(const f32x4*)c.v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < c.left) {
+          c.mv[j] = ((const float*)c.m)[j];
+          c.vv[j] = ((const float*)c.v)[j];
+        }
+    }
+  }
+  if (c.wide) {
+    c.pv = *(const f32x4*)c.p;
+    c.gv = *(const f32x4*)(g + i);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < c.left) {
+        c.pv[j] = c.p[j];
+        c.gv[j] = g[i + j];
+      }
+  }
+}
+
+__device__ __forceinline__ void finish_four(const AdamHyper& h, double coef, Four& c) {
+  if (c.ms) {
+    // a power of two multiplies exactly: b * (code * scale) = (b * scale) * code
+    const double b1 = h.b1 * (double)c.mv[1], b2 = h.b2 * (double)c.vv[1];
+    const unsigned key = hash_bits(c.key, h.key);
+    double md[4], vd[4];
+    decode4(__float_as_uint(c.mv[0]), md);
+    decode4(__float_as_uint(c.vv[0]), vd);
+    unsigned mtop = 0, vtop = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {                // elements past the end are zeros and stay so
+      const double gi = (double)c.gv[j] * coef;
+      md[j] = b1 * md[j] + h.c1 * gi;
+      vd[j] = b2 * vd[j] + h.c2 * (gi * gi);
+      const unsigned a = hi_word(md[j]) & 0x7fffffffu, b = hi_word(vd[j]) & 0x7fffffffu;
+      mtop = a > mtop ? a : mtop;
+      vtop = b > vtop ? b : vtop;
+      c.pv[j] = adam_update(c.pv[j], md[j], vd[j], h);
+    }
+    const Encoder me(row_max(mtop)), ve(row_max(vtop));
+    unsigned mc = 0, vc = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned r = mix_bits((c.id + j * 0x9E3779B1u) ^ key);
+      const unsigned a = me.code(md[j], r & 0xffffu), b = ve.code(vd[j], r >> 16);
+      const unsigned least = vd[j] > 0.0 ? 1u : 0u;
+      mc |= (a | (a ? (hi_word(md[j]) >> 24) & 0x80u : 0u)) << (8 * j);
+      vc |= (b > least ? b : least) << (8 * j);
+    }
+    if (c.wide) {
+      *(unsigned*)c.m = mc;
+      *(unsigned*)c.v = vc;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < c.left) {
+          ((unsigned char*)c.m)[j] = (unsigned char)(mc >> (8 * j));
+          ((unsigned char*)c.v)[j] = (unsigned char)(vc >> (8 * j));
+        }
+    }
+    if (c.left && (threadIdx.x & 15) == 0) {
+      *c.ms = me.scale;
+      *c.vs = ve.scale;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double gi = (double)c.gv[j] * coef;
+      const double mi = h.b1 * (double)c.mv[j] + h.c1 * gi, vi = h.b2 * (double)c.vv[j] + h.c2 * (gi * gi);
+      c.mv[j] = (float)mi;
+      c.vv[j] = (float)vi;
+      c.pv[j] = adam_update(c.pv[j], mi, vi, h);
+    }
+    if (c.wide) {
+      *(f32x4*)c.m = c.mv;
+      *(f32x4*)c.v = c.vv;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < c.left) {
+          ((float*)c.m)[j] = c.mv[j];
+          ((float*)c.v)[j] = c.vv[j];
+        }
+    }
+  }
+  if (c.wide) {
+    *(f32x4*)c.p = c.pv;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < c.left) c.p[j] = c.pv[j];
+  }
 }
 
 __global__ void __launch_bounds__(256)
 k_adamw_mixed(AdamTable t, AdamHyper h) {
   __shared__ double sh[4];
+  const int total = t.chunk0[t.n];
+  int chunk = blockIdx.x;
+  const double part = h.parts ? h.parts[threadIdx.x] : 0.0;   // requested first: loads return in order
+  Four c;
+  load_four(t, h, chunk, c);                     // under way while the norm is added up
   double coef = 1.0;
   if (h.parts) {
-    double s = 0.0;
-    for (int i = threadIdx.x; i < AW_PARTS; i += 256) s += h.parts[i];
-    s = block_sum(s, sh);
+    static_assert(AW_PARTS == 256, "one partial sum a thread");
+    const double s = block_sum<4>(part, sh);
     if (blockIdx.x == 0 && threadIdx.x == 0 && h.sumsq) *h.sumsq = (float)s;
-    const double c = h.max_norm / (sqrt(s) + 1e-6);
-    coef = c < 1.0 || c != c ? c : 1.0;          // a NaN norm reaches every parameter, as in clip_coef (mpnn_loss.hip)
+    const double f = h.max_norm / (sqrt(s) + 1e-6);
+    coef = f < 1.0 || f != f ? f : 1.0;          // a NaN norm reaches every parameter, as in clip_coef (mpnn_loss.hip)
   }
-  for (int chunk = blockIdx.x; chunk < t.chunk0[t.n]; chunk += gridDim.x) {
-    const int ti = tensor_of(t, chunk);
-    float* __restrict__ p = t.p[ti];
-    const float* __restrict__ g = t.g[ti];
-    const long long n = t.numel[ti], i0 = (long long)(chunk - t.chunk0[ti]) * AW_CHUNK;
-    if (!t.ms[ti]) {
-      float* __restrict__ m = (float*)t.m[ti];
-      float* __restrict__ v = (float*)t.v[ti];
-      for (long long i = i0 + threadIdx.x; i < n && i < i0 + AW_CHUNK; i += 256) {
-        const double gi = (double)g[i] * coef;
-        const double mi = h.b1 * (double)m[i] + h.c1 * gi, vi = h.b2 * (double)v[i] + h.c2 * (gi * gi);
-        m[i] = (float)mi;
-        v[i] = (float)vi;
-        p[i] = adam_update(p[i], mi, vi, h);
-      }
-      continue;
-    }
-    unsigned char* __restrict__ m = (unsigned char*)t.m[ti];
-    unsigned char* __restrict__ v = (unsigned char*)t.v[ti];
-    const unsigned key = hash_bits(h.tensor0 + ti, h.key);
-    const bool wide = (((uintptr_t)p | (uintptr_t)g) & 15) == 0 && (((uintptr_t)m | (uintptr_t)v) & 3) == 0;
-    for (int it = 0; it < AW_CHUNK / 1024; ++it) {
-      const long long i = i0 + it * 1024 + threadIdx.x * 4;
-      if (i0 + it * 1024 >= n) break;
-      const long long blk = i / AW_BLOCK;
-      const int left = i >= n ? 0 : n - i < 4 ? (int)(n - i) : 4;
-      f32x4 pv = {0.f, 0.f, 0.f, 0.f}, gv = pv;
-      unsigned mc = 0, vc = 0;
-      float ms = 1.f, vs = 1.f;
-      if (left) {
-        ms = t.ms[ti][blk];
-        vs = t.vs[ti][blk];
-      }
-      if (wide && left == 4) {
-        pv = *reinterpret_cast<const f32x4*>(p + i);
-        gv = *reinterpret_cast<const f32x4*>(g + i);
-        mc = *reinterpret_cast<const unsigned*>(m + i);
-        vc = *reinterpret_cast<const unsigned*>(v + i);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < left) {
-            pv[j] = p[i + j];
-            gv[j] = g[i + j];
-            mc |= (unsigned)m[i + j] << (8 * j);
-            vc |= (unsigned)v[i + j] << (8 * j);
-          }
-      }
-      double md[4], vd[4];
-      decode4(mc, ms, md);
-      decode4(vc, vs, vd);
-      unsigned mtop = 0, vtop = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const double gi = (double)gv[j] * coef;
-        md[j] = h.b1 * md[j] + h.c1 * gi;
-        vd[j] = h.b2 * vd[j] + h.c2 * (gi * gi);
-        if (j >= left) md[j] = vd[j] = 0.0;
-        const unsigned a = hi_word(md[j]) & 0x7fffffffu, b = hi_word(vd[j]) & 0x7fffffffu;
-        mtop = a > mtop ? a : mtop;
-        vtop = b > vtop ? b : vtop;
-        pv[j] = adam_update(pv[j], md[j], vd[j], h);
-      }
-      int me, ve;
-      const bool mfin = scale_exponent(row_max(mtop), me), vfin = scale_exponent(row_max(vtop), ve);
-      const double minv = pow2(-me), vinv = pow2(-ve);
-      mc = vc = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned r = hash_bits((unsigned)(i + j), key);
-        const unsigned a = mfin ? to_code(md[j], minv, r & 0xffffu) : 0u;
-        unsigned b = vfin ? to_code(vd[j], vinv, r >> 16) : 0u;
-        if (b == 0 && vd[j] > 0.0) b = 1;
-        mc |= (a | (a && md[j] < 0.0 ? 0x80u : 0u)) << (8 * j);
-        vc |= b << (8 * j);
-      }
-      if (wide && left == 4) {
-        *reinterpret_cast<f32x4*>(p + i) = pv;
-        *reinterpret_cast<unsigned*>(m + i) = mc;
-        *reinterpret_cast<unsigned*>(v + i) = vc;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < left) {
-            p[i + j] = pv[j];
-            m[i + j] = (unsigned char)(mc >> (8 * j));
-            v[i + j] = (unsigned char)(vc >> (8 * j));
-          }
-      }
-      if (left && (threadIdx.x & 15) == 0) {
-        t.ms[ti][blk] = mfin ? (float)pow2(me) : NAN;
-        t.vs[ti][blk] = vfin ? (float)pow2(ve) : NAN;
-      }
-    }
+  for (;;) {   // (the next elements requested before these are finished: 472 us instead of 429, too many registers)
+    finish_four(h, coef, c);
+    chunk += gridDim.x;
+    if (chunk >= total) return;
+    load_four(t, h, chunk, c);
   }
-}
-
-template <typename Table>
-bool place_chunks(Table& t, const long long* numel) {
-  long long chunks = 0;
-  for (int j = 0; j < t.n; ++j) {
-    t.numel[j] = numel[j];
-    t.chunk0[j] = (int)chunks;
-    chunks += (numel[j] + AW_CHUNK - 1) / AW_CHUNK;
-    if (chunks >= (1LL << 31) - 65536) return false;
-  }
-  t.chunk0[t.n] = (int)chunks;
-  return true;
 }
 
 }  // namespace
@@ -282,18 +366,31 @@ bool place_chunks(Table& t, const long long* numel) {
 extern "C" int mpnn_grad_sumsq_parts(int n, const float* const* grads, const long long* numel, double* parts, void* stream) {
   MPNN_CHECK_ARG(n > 0 && n <= AW_PARTS * NT_MAX && grads && numel && parts, "mpnn_grad_sumsq_parts: bad arguments");
   for (int j = 0; j < n; ++j)
-    MPNN_CHECK_ARG(grads[j] && numel[j] > 0 && numel[j] < (1LL << 40), "mpnn_grad_sumsq_parts: null, empty or oversized tensor");
+    MPNN_CHECK_ARG(grads[j] && numel[j] > 0 && numel[j] < (1LL << 32), "mpnn_grad_sumsq_parts: null, empty or oversized tensor");
   const int launches = (n + NT_MAX - 1) / NT_MAX, share = AW_PARTS / launches;
   for (int l = 0; l < launches; ++l) {
     NormTable t;
     const int k0 = l * NT_MAX;
     t.n = n - k0 < NT_MAX ? n - k0 : NT_MAX;
-    for (int j = 0; j < t.n; ++j) t.g[j] = grads[k0 + j];
-    MPNN_CHECK_ARG(place_chunks(t, numel + k0), "mpnn_grad_sumsq_parts: too many elements for one launch");
+    long long chunks = 0;                            // at most 128 * 2^18
+    for (int j = 0; j < t.n; ++j) {
+      t.g[j] = grads[k0 + j];
+      t.numel[j] = numel[k0 + j];
+      t.chunk0[j] = (int)chunks;
+      chunks += (numel[k0 + j] + NT_CHUNK - 1) / NT_CHUNK;
+    }
+    t.chunk0[t.n] = (int)chunks;
     const int wgs = l + 1 < launches ? share : AW_PARTS - share * (launches - 1);   // every part is written
-    hipLaunchKernelGGL(k_grad_sumsq_parts, dim3(wgs), dim3(256), 0, (hipStream_t)stream, t, parts + (long long)share * l);
+    hipLaunchKernelGGL(k_grad_sumsq_parts, dim3(wgs), dim3(NT_THREADS), 0, (hipStream_t)stream, t, parts + (long long)share * l);
   }
   MPNN_LAUNCH_CHECK();
+}
+
+// distance of x from the table's origin in units of four bytes, if it has one (NO_SCALE is none)
+static bool offset(const void* x, const char* origin, int& out) {
+  const long long d = (const char*)x - origin;
+  out = (int)(d / 4);
+  return d % 4 == 0 && d / 4 > -(1LL << 31) && d / 4 < (1LL << 31);
 }
 
 extern "C" int mpnn_adamw_mixed(int n, float* const* params, const float* const* grads, void* const* exp_avg,
@@ -306,7 +403,7 @@ extern "C" int mpnn_adamw_mixed(int n, float* const* params, const float* const*
   MPNN_CHECK_ARG(step >= 1 && lr >= 0 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && weight_decay >= 0,
                  "mpnn_adamw_mixed: bad hyper-parameters");
   for (int j = 0; j < n; ++j) {
-    MPNN_CHECK_ARG(params[j] && grads[j] && exp_avg[j] && exp_avg_sq[j] && numel[j] > 0 && numel[j] < (1LL << 40),
+    MPNN_CHECK_ARG(params[j] && grads[j] && exp_avg[j] && exp_avg_sq[j] && numel[j] > 0 && numel[j] < (1LL << 32),
                    "mpnn_adamw_mixed: null, empty or oversized tensor");
     MPNN_CHECK_ARG(!exp_avg_scale[j] == !exp_avg_sq_scale[j], "mpnn_adamw_mixed: both moments of a tensor have scales, or none");
   }
@@ -323,22 +420,35 @@ extern "C" int mpnn_adamw_mixed(int n, float* const* params, const float* const*
   h.parts = max_norm > 0 ? sumsq_parts : nullptr;
   h.key = hash_bits((unsigned)step, seed);
   h.sumsq = grad_sumsq;
-  for (int k0 = 0; k0 < n; k0 += AW_MAX) {
+  for (int k0 = 0; k0 < n;) {
     AdamTable t;
-    t.n = n - k0 < AW_MAX ? n - k0 : AW_MAX;
-    for (int j = 0; j < t.n; ++j) {
-      t.p[j] = params[k0 + j];
-      t.g[j] = grads[k0 + j];
-      t.m[j] = exp_avg[k0 + j];
-      t.v[j] = exp_avg_sq[k0 + j];
-      t.ms[j] = exp_avg_scale[k0 + j];
-      t.vs[j] = exp_avg_sq_scale[k0 + j];
+    t.origin[0] = t.origin[1] = Origin{};
+    long long chunks = 0;
+    int j = 0;
+    for (; j < AW_MAX && k0 + j < n; ++j) {
+      const int k = k0 + j;
+      const bool eight = exp_avg_scale[k] != nullptr;
+      Origin& o = t.origin[eight];
+      if (!o.p)
+        o = Origin{(char*)params[k], (char*)grads[k], (char*)exp_avg[k], (char*)exp_avg_sq[k], (char*)exp_avg_scale[k],
+                   (char*)exp_avg_sq_scale[k]};
+      const long long more = (numel[k] + AW_CHUNK - 1) / AW_CHUNK;
+      t.ms[j] = t.vs[j] = NO_SCALE;
+      if (!offset(params[k], o.p, t.p[j]) || !offset(grads[k], o.g, t.g[j]) || !offset(exp_avg[k], o.m, t.m[j]) ||
+          !offset(exp_avg_sq[k], o.v, t.v[j]) ||
+          (eight && (!offset(exp_avg_scale[k], o.ms, t.ms[j]) || !offset(exp_avg_sq_scale[k], o.vs, t.vs[j]))) ||
+          chunks + more >= (1LL << 31) - 65536)
+        break;                                       // never the first: it is an origin
+      t.numel[j] = (unsigned)numel[k];
+      t.chunk0[j] = (int)chunks;
+      chunks += more;
     }
-    MPNN_CHECK_ARG(place_chunks(t, numel + k0), "mpnn_adamw_mixed: too many elements for one launch");
+    t.n = j;
+    t.chunk0[j] = (int)chunks;
     h.tensor0 = (unsigned)(first + k0);
-    const int wgs = t.chunk0[t.n] < 2048 ? t.chunk0[t.n] : 2048;
-    hipLaunchKernelGGL(k_adamw_mixed, dim3(wgs), dim3(256), 0, (hipStream_t)stream, t, h);
+    hipLaunchKernelGGL(k_adamw_mixed, dim3((unsigned)(chunks < AW_WGS ? chunks : AW_WGS)), dim3(256), 0, (hipStream_t)stream, t, h);
     h.sumsq = nullptr;
+    k0 += j;
   }
   MPNN_LAUNCH_CHECK();
 }
