@@ -160,38 +160,33 @@ __device__ __forceinline__ void write_dead_slot(const SelectArgs& a, int b, int 
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int SMALL_CAP = 512;   // candidates a wave ranks in LDS
 
+// The candidates of lane j of the g = 2^g_log2 lanes that share beam w: keys of tokens j, j + g, ...; the best of them
 template <typename T, int M>
-__global__ void __launch_bounds__(64)
-k_select_small(SelectArgs a, int g_log2) {
-  __shared__ long long lk[SMALL_CAP];
-  __shared__ int li[SMALL_CAP];
-  const int b = blockIdx.x, lane = threadIdx.x, g = 1 << g_log2;
-  const int w = lane >> g_log2, j = lane & (g - 1);
+__device__ __forceinline__ long long lane_candidates(const SelectArgs& a, int b, int w, int j, int g_log2, long long (&k)[M]) {
+  const int g = 1 << g_log2;
   const bool live = w < a.W;
   const long long row = (long long)b * a.W + (live ? w : 0);
   const double s = (double)a.scores[row];
   const long long f = a.forced ? a.forced[row] : -1;
+  const T* logits = (const T*)a.logits + (long long)b * a.sb + (live ? w : 0) * a.sw;
+  const float* bias = a.bias ? a.bias + (long long)b * a.bb + (live ? w : 0) * a.bw : nullptr;
+  T raw[M];
+  float add[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) {      // every load is in flight before the first is used; places beyond V read the last one
+    const int v = j + (i << g_log2);
+    raw[i] = logits[v < a.V ? v : a.V - 1];
+    add[i] = bias ? bias[v < a.V ? v : a.V - 1] : 0.f;
+  }
   double x[M];
   double top = -INFINITY;
   bool nan = false;
-  {
-    const T* logits = (const T*)a.logits + (long long)b * a.sb + (live ? w : 0) * a.sw;
-    const float* bias = a.bias ? a.bias + (long long)b * a.bb + (live ? w : 0) * a.bw : nullptr;
-    T raw[M];
-    float add[M];
 #pragma unroll
-    for (int i = 0; i < M; ++i) {      // every load is in flight before the first is used; places beyond V read the last one
-      const int v = j + (i << g_log2);
-      raw[i] = logits[v < a.V ? v : a.V - 1];
-      add[i] = bias ? bias[v < a.V ? v : a.V - 1] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < M; ++i) {
-      const int v = j + (i << g_log2);
-      x[i] = live && v < a.V && add[i] != -INFINITY ? (double)to_f(raw[i]) + (double)add[i] : -INFINITY;
-      top = fmax(top, x[i]);
-      nan |= x[i] != x[i];
-    }
+  for (int i = 0; i < M; ++i) {
+    const int v = j + (i << g_log2);
+    x[i] = live && v < a.V && add[i] != -INFINITY ? (double)to_f(raw[i]) + (double)add[i] : -INFINITY;
+    top = fmax(top, x[i]);
+    nan |= x[i] != x[i];
   }
   top = group_max(top, g);
   double sum = nan || top == INFINITY ? (double)NAN : 0.0;
@@ -201,7 +196,6 @@ k_select_small(SelectArgs a, int g_log2) {
   sum = group_sum(sum, g);
   const double lse = base + log(sum);   // of no use where nothing is left of the row: no candidate below
   const bool bad = broken(s, lse);
-  long long k[M];
   long long best = KEY_NONE;
 #pragma unroll
   for (int i = 0; i < M; ++i) {
@@ -212,6 +206,17 @@ k_select_small(SelectArgs a, int g_log2) {
     k[i] = live && v < a.V && !(c == -INFINITY) ? key_of(c) : KEY_NONE;
     best = k[i] > best ? k[i] : best;
   }
+  return best;
+}
+
+template <typename T, int M>
+__global__ void __launch_bounds__(64)
+k_select_small(SelectArgs a, int g_log2) {
+  __shared__ long long lk[SMALL_CAP];
+  __shared__ int li[SMALL_CAP];
+  const int b = blockIdx.x, lane = threadIdx.x, w = lane >> g_log2, j = lane & ((1 << g_log2) - 1);
+  long long k[M];
+  const long long best = lane_candidates<T, M>(a, b, w, j, g_log2, k);
   // at least n candidates reach the bound that n lanes' best ones do, seldom many more
   int cnt = SMALL_CAP + 1;
   if (a.n <= 64) {
@@ -333,6 +338,62 @@ __device__ __forceinline__ void block_best(long long& k, int& p, long long* sk, 
 #pragma unroll
   for (int i = 1; i < 4; ++i)
     if (better(sk[i], sp[i], k, p)) { k = sk[i]; p = sp[i]; }
+}
+
+// Middling groups: four waves hold a group's candidates in registers, as one wave does for small ones, and rank those that
+// reach the bound in LDS.  64 beams x 21 letters, 64 kept: 6.2 us, where one wave took 16-21.
+template <typename T, int M>
+__global__ void __launch_bounds__(256)
+k_select_group(SelectArgs a, int g_log2) {
+  __shared__ unsigned ru[4];
+  __shared__ int rc;
+  __shared__ long long lk[SEL_CAP];
+  __shared__ int li[SEL_CAP];
+  const int b = blockIdx.x, tid = threadIdx.x, w = tid >> g_log2, j = tid & ((1 << g_log2) - 1);
+  long long k[M];
+  const long long best = lane_candidates<T, M>(a, b, w, j, g_log2, k);
+  const bool full = a.W << g_log2 >= 256;
+  wave_bounds((unsigned)(best >> 32) ^ 0x80000000u, a.n, full, ru);
+  if (tid == 0) rc = 0;
+  __syncthreads();
+  const unsigned T32 = block_bound(a.n, full, ru);
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    if (k[i] != KEY_NONE && ((unsigned)(k[i] >> 32) ^ 0x80000000u) >= T32) {
+      const int q = atomicAdd(&rc, 1);
+      if (q < SEL_CAP) {
+        lk[q] = k[i];
+        li[q] = w * a.V + j + (i << g_log2);
+      }
+    }
+  }
+  __syncthreads();
+  const int cnt = rc;
+  if (cnt <= SEL_CAP) {
+    rank_collected(lk, li, cnt, a.n, [&](int r, long long ke, int pe) { write_slot(a, b, r, ke, pe); });
+    for (int r = cnt + tid; r < a.n; r += 256) write_dead_slot(a, b, r);
+    return;
+  }
+  // more ties than the list holds: one after the other
+  long long prev = KEY_NAN;
+  int place = -1;
+  __shared__ long long sk[4];
+  __shared__ int sp[4];
+  for (int r = 0; r < a.n; ++r) {
+    long long kb = KEY_NONE;
+    int pb = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const int pe = w * a.V + j + (i << g_log2);
+      if (k[i] != KEY_NONE && better(prev, place, k[i], pe) && better(k[i], pe, kb, pb)) { kb = k[i]; pb = pe; }
+    }
+    block_best(kb, pb, sk, sp);
+    if (tid == 0) {
+      if (kb != KEY_NONE) write_slot(a, b, r, kb, pb); else write_dead_slot(a, b, r);
+    }
+    prev = kb;
+    place = pb;
+  }
 }
 
 __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
@@ -570,18 +631,20 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
   }
 }
 
-// how a call is split: 0 = one wave a group (registers), else values per thread of a 256-thread slice
+// How a call is split: one wave a group up to 8 candidates a lane (64 x 16 x 21), one workgroup of four waves up to 32 (three
+// beams or more, so that the waves have work), else slices of 256 u logits and a second pass.
 struct SelectPlan {
-  int g_log2, m;        // one wave a group
-  int u, splits;        // slices
+  int waves, g_log2, m;  // waves a group, 0 = slices; 2^g_log2 lanes a beam; candidates a lane
+  int u, splits;         // slices
 };
 inline SelectPlan select_plan(long long B, int W, int V, int item) {
   SelectPlan p = {};
-  if (W <= 64) {
+  for (int waves = 1; waves <= 4; waves += 3) {
     int gl = 6;
-    while ((64 >> gl) < W) --gl;
+    while (gl > 0 && ((64 * waves) >> gl) < W) --gl;
     const int m = (V + (1 << gl) - 1) >> gl;
-    if (m <= 32) {
+    if (((64 * waves) >> gl) >= W && m <= (waves == 1 ? 8 : W > 2 ? 32 : 0)) {
+      p.waves = waves;
       p.g_log2 = gl;
       p.m = m;
       return p;
@@ -597,13 +660,18 @@ inline SelectPlan select_plan(long long B, int W, int V, int item) {
 
 template <typename T>
 int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_t st) {
-  if (p.u == 0) {
+  if (p.waves == 1) {
     const dim3 grid(a.B), block(64);
     if (p.m <= 2) hipLaunchKernelGGL((k_select_small<T, 2>), grid, block, 0, st, a, p.g_log2);
     else if (p.m <= 4) hipLaunchKernelGGL((k_select_small<T, 4>), grid, block, 0, st, a, p.g_log2);
-    else if (p.m <= 8) hipLaunchKernelGGL((k_select_small<T, 8>), grid, block, 0, st, a, p.g_log2);
-    else if (p.m <= 16) hipLaunchKernelGGL((k_select_small<T, 16>), grid, block, 0, st, a, p.g_log2);
-    else hipLaunchKernelGGL((k_select_small<T, 32>), grid, block, 0, st, a, p.g_log2);
+    else hipLaunchKernelGGL((k_select_small<T, 8>), grid, block, 0, st, a, p.g_log2);
+    MPNN_LAUNCH_CHECK();
+  }
+  if (p.waves == 4) {
+    const dim3 grid(a.B), block(256);
+    if (p.m <= 8) hipLaunchKernelGGL((k_select_group<T, 8>), grid, block, 0, st, a, p.g_log2);
+    else if (p.m <= 16) hipLaunchKernelGGL((k_select_group<T, 16>), grid, block, 0, st, a, p.g_log2);
+    else hipLaunchKernelGGL((k_select_group<T, 32>), grid, block, 0, st, a, p.g_log2);
     MPNN_LAUNCH_CHECK();
   }
   const long long parts = (long long)a.B * a.W * p.splits;
@@ -629,7 +697,7 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
 // States: a wave owns 64 columns of up to 16 bytes of one group - the same bytes of all its beams.  It reads the columns of
 // the rows that another row becomes, all of them before the first write, then writes each row that changes.  A column belongs
 // to one lane from first read to last write, so the update is in place without a barrier.  Bound by the bytes of the rows
-// that move: a row that stays is not written, one that nobody else becomes is not read.  Up to 32 beams the rows wait in
+// that move: a row that stays is not written, one that nobody else becomes is not read.  Up to 64 beams the rows wait in
 // registers (all reads in flight at once, and more waves a CU than when they wait in LDS: 36 us against 56 for 16 structures
 // x 16 beams x 512 residues, half of them decided), beyond that in LDS.  234 us for 1.05 GB of caches of four beams.
 // ---------------------------------------------------------------------------------------------------------------
@@ -740,7 +808,7 @@ k_beam_reorder(ReorderTable t, const long long* __restrict__ parent, int W, int 
     if (R) reorder_in_registers<V, R ? R : 1>(data, s.stride_beam, live, from[0]); \
     else reorder_through_lds(data, s.stride_beam, W, live, from, (V*)lds);         \
   } while (0)
-  if (vl == 4) MPNN_COLUMNS(f32x4);
+  if (vl == 4 && R <= 32) MPNN_COLUMNS(f32x4);
   else if (vl == 3) MPNN_COLUMNS(unsigned long long);
   else if (vl == 2) MPNN_COLUMNS(unsigned);
   else if (vl == 1) MPNN_COLUMNS(unsigned short);
@@ -755,7 +823,8 @@ inline int state_vec_log2(const mpnn_beam_state& s, int W) {
   if (s.n_mid > 1) bits |= (unsigned long long)s.stride_mid;
   int vl = 4;
   while (vl > 0 && (bits & ((1u << vl) - 1))) --vl;
-  while (vl > 0 && W > 32 && (64 << vl) * W > 65536) --vl;   // the LDS a wave may hold
+  if (W > 32 && W <= 64 && vl > 3) vl = 3;                   // 64 rows of 16 bytes are all the registers a lane has
+  while (vl > 0 && W > 64 && (64 << vl) * W > 65536) --vl;   // the LDS a wave may hold
   return vl;
 }
 
@@ -806,37 +875,70 @@ struct PlaceArgs {
 };
 
 // The residue just decided, beam by beam: its gathered rows become the parent's plus the letter's term (block y < n_layers),
-// its letter and log-probs are written down (the last block).  A lane owns two columns of all beams, as in k_beam_reorder.
-__global__ void __launch_bounds__(64)
+// its letter and log-probs are written down (the last block).  Four waves share a layer's rows, sixteen at a time each, so
+// that up to 64 beams cost two round trips to memory; every row is in LDS before the first is written.
+__global__ void __launch_bounds__(256)
 k_beam_place(PlaceArgs a) {
   extern __shared__ char lds[];
-  const int b = blockIdx.x, l = blockIdx.y, lane = threadIdx.x, W = a.W;
+  const int b = blockIdx.x, l = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = a.W;
   const long long* parent = a.parent + (long long)b * W;
   const long long* token = a.token + (long long)b * W;
   const int* list = a.list + b * W;
+  const int mine = lane < W ? lane : 0;          // W <= 64: a lane's beam
+  const int at = list[mine], from = (int)parent[mine], letter = (int)token[mine];
   if (l < a.n_layers) {
     float2* row = reinterpret_cast<float2*>(lds);
     float* A = a.A[l] + a.offA[l] + 2 * lane;
-    for (int w = 0; w < W; ++w) row[w * 64 + lane] = *reinterpret_cast<const float2*>(A + (size_t)list[w] * a.lda[l]);
-    for (int w = 0; w < W; ++w) {
-      float2 v = row[(int)parent[w] * 64 + lane];
-      const float2 t = *reinterpret_cast<const float2*>(a.TS + (size_t)token[w] * a.ld_ts + l * MPNN_H + 2 * lane);
-      v.x += t.x;
-      v.y += t.y;
-      *reinterpret_cast<float2*>(A + (size_t)list[w] * a.lda[l]) = v;
+    const float* T = a.TS + l * MPNN_H + 2 * lane;
+    float2 v[16], t[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int w = wave + 4 * i;
+      if (w < W) {
+        v[i] = *reinterpret_cast<const float2*>(A + (size_t)__builtin_amdgcn_readlane(at, w) * a.lda[l]);
+        t[i] = *reinterpret_cast<const float2*>(T + (size_t)__builtin_amdgcn_readlane(letter, w) * a.ld_ts);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (wave + 4 * i < W) row[(wave + 4 * i) * 64 + lane] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int w = wave + 4 * i;
+      if (w < W) {
+        float2 x = row[__builtin_amdgcn_readlane(from, w) * 64 + lane];
+        x.x += t[i].x;
+        x.y += t[i].y;
+        *reinterpret_cast<float2*>(A + (size_t)__builtin_amdgcn_readlane(at, w) * a.lda[l]) = x;
+      }
     }
     return;
   }
-  for (int w = lane; w < W; w += 64) {
-    const float* x = a.logits + ((long long)b * W + parent[w]) * a.n_letters;
-    float top = -INFINITY, sum = 0.f;
-    for (int v = 0; v < a.n_letters; ++v) top = fmaxf(top, x[v]);
-    for (int v = 0; v < a.n_letters; ++v) sum += expf(x[v] - top);
-    const float lse = top + logf(sum);
-    float* lp = a.log_probs + (size_t)list[w] * a.n_letters;
-    for (int v = 0; v < a.n_letters; ++v) lp[v] = x[v] - lse;
-    a.S[list[w]] = token[w];
+  // four lanes a beam: 64 beams at once
+  const int w = threadIdx.x >> 2, q = threadIdx.x & 3;
+  const bool live = w < W;
+  const int p = live ? (int)parent[w] : 0;
+  const float* x = a.logits + ((long long)b * W + p) * a.n_letters;
+  float y[8], top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    y[i] = q + 4 * i < a.n_letters ? x[q + 4 * i] : -INFINITY;
+    top = fmaxf(top, y[i]);
   }
+  top = fmaxf(top, __shfl_xor(top, 1));
+  top = fmaxf(top, __shfl_xor(top, 2));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += expf(y[i] - top);
+  sum += __shfl_xor(sum, 1);
+  sum += __shfl_xor(sum, 2);
+  if (!live) return;
+  const float lse = top + logf(sum);
+  float* lp = a.log_probs + (size_t)list[w] * a.n_letters;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (q + 4 * i < a.n_letters) lp[q + 4 * i] = y[i] - lse;
+  if (q == 0) a.S[list[w]] = token[w];
 }
 
 }  // namespace
@@ -844,7 +946,7 @@ k_beam_place(PlaceArgs a) {
 extern "C" long long mpnn_beam_select_workspace(int dtype, int n_groups, int n_beams, int n_tokens, int n_out) {
   if (dtype < 0 || dtype > 2 || n_groups <= 0 || n_beams <= 0 || n_tokens <= 0 || n_out <= 0 || n_out > SEL_MAX_N) return -1;
   const SelectPlan p = select_plan(n_groups, n_beams, n_tokens, dtype == 0 ? 4 : 2);
-  if (p.u == 0) return 0;
+  if (p.waves) return 0;
   return (long long)n_groups * n_beams * p.splits * ((long long)sizeof(SlicePart) + 12LL * n_out);
 }
 
@@ -858,12 +960,13 @@ extern "C" int mpnn_beam_select(const void* logits, int dtype, long long stride_
   MPNN_CHECK_ARG(n_groups > 0 && n_beams > 0 && n_beams <= SEL_MAX_N && n_out > 0 && n_out <= SEL_MAX_N && n_tokens > 0 &&
                      n_tokens <= (1 << 22),
                  "mpnn_beam_select: bad sizes (at most 256 beams and hypotheses kept, at most 2^22 tokens)");
+  MPNN_CHECK_ARG(((uintptr_t)logits & (dtype == 0 ? 3 : 1)) == 0, "mpnn_beam_select: logits are not aligned to their type");
   const long long need = mpnn_beam_select_workspace(dtype, n_groups, n_beams, n_tokens, n_out);
   MPNN_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                  "mpnn_beam_select: workspace missing, too small (mpnn_beam_select_workspace) or not 16-byte aligned");
   const SelectPlan p = select_plan(n_groups, n_beams, n_tokens, dtype == 0 ? 4 : 2);
-  MPNN_CHECK_ARG((long long)n_groups * n_beams * (p.u ? p.splits : 1) < (1LL << 31) &&
-                     (long long)n_beams * (p.u ? p.splits : 1) * n_out < (1LL << 31),
+  MPNN_CHECK_ARG((long long)n_groups * n_beams * (p.waves ? 1 : p.splits) < (1LL << 31) &&
+                     (long long)n_beams * (p.waves ? 1 : p.splits) * n_out < (1LL << 31),
                  "mpnn_beam_select: too many groups for one launch");
   SelectArgs a = {logits, stride_group, stride_beam, scores, bias, bias_group, bias_beam, (const long long*)forced,
                   n_groups, n_beams, n_tokens, n_out, out_scores, (long long*)parent, (long long*)token};
@@ -907,6 +1010,7 @@ extern "C" int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int
     if (n_beams <= 4) MPNN_REORDER(4);
     else if (n_beams <= 16) MPNN_REORDER(16);
     else if (n_beams <= 32) MPNN_REORDER(32);
+    else if (n_beams <= 64) MPNN_REORDER(64);
     else MPNN_REORDER(0);
 #undef MPNN_REORDER
   }
@@ -991,7 +1095,7 @@ static int beam_run(bool f16, const float* hE_frag, const float* PVenc, int lden
       rc = mpnn_beam_reorder(n_layers + 2, states, parent, n_groups, n_beams, t, nullptr, rank, stream);
     if (rc) return rc;
     place.list = list;
-    hipLaunchKernelGGL(k_beam_place, dim3(n_groups, n_layers + 1), dim3(64), (size_t)n_beams * 512, st, place);
+    hipLaunchKernelGGL(k_beam_place, dim3(n_groups, n_layers + 1), dim3(256), (size_t)n_beams * 512, st, place);
     float* s = now;
     now = next;
     next = s;

@@ -287,6 +287,13 @@ PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       for (size_t j = i + 1; j < spans.size() && spans[j].begin < spans[i].end; ++j)
         if (!apart(spans[i], spans[j])) value_error("mpnn_amd.beam_reorder: two states share memory");
     const c10::OptionalDeviceGuard guard(dev);
+    // an index that lies in a state would change while it is read
+    auto beside_states = [&](at::Tensor t) {
+      const long long begin = (long long)t.const_data_ptr(), end = begin + t.numel() * t.element_size();
+      for (const Span& s : spans)
+        if (begin < s.end && s.begin < end) return t.clone();
+      return t;
+    };
     int length_all = -1;
     at::Tensor lengths, rank;
     if (positions) {
@@ -294,7 +301,7 @@ PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const at::Tensor& t = on_gpu(a[2], what, "length", &dev);
         if (t.dim() != 1 || t.size(0) != B || !whole(t))
           value_error("mpnn_amd.beam_reorder: length must be an int or integers [" + std::to_string(B) + "]");
-        lengths = t.to(at::kInt).contiguous();
+        lengths = beside_states(t.to(at::kInt).contiguous());
       } else {
         length_all = (int)std::max(0LL, std::min(integer(a[2]), 0x7fffffffLL));
       }
@@ -303,10 +310,10 @@ PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       const at::Tensor& t = on_gpu(a[3], what, "rank", &dev);
       if (!whole(t) || (L >= 0 && (t.dim() != 2 || t.size(0) != B || t.size(1) != L)))
         value_error("mpnn_amd.beam_reorder: rank must be integers [" + std::to_string(B) + ", " + std::to_string(L) + "]");
-      rank = t.to(at::kInt).contiguous();
+      rank = beside_states(t.to(at::kInt).contiguous());
     }
     if (!table.empty()) {
-      const at::Tensor parent = given.to(at::kLong).contiguous();
+      const at::Tensor parent = beside_states(given.to(at::kLong).contiguous());
       check_rc(f_reorder((int)table.size(), table.data(), parent.const_data_ptr<int64_t>(), (int)B, (int)W, length_all,
                          lengths.defined() ? lengths.const_data_ptr<int>() : nullptr,
                          rank.defined() ? rank.const_data_ptr<int>() : nullptr, stream_of(dev)),
@@ -372,6 +379,7 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     std::vector<const float*> g(n);
     std::vector<void*> m(n), v(n);
     std::vector<long long> numel(n);
+    std::vector<std::pair<const float*, const float*>> order;
     const c10::Device dev = tensor(P.at[0], "optim", "parameters").device();
     const char* name = "optim.adamw_step";
     const auto fp32 = caffe2::TypeMeta::fromScalarType(at::kFloat), fp8 = caffe2::TypeMeta::fromScalarType(at::kFloat8_e4m3fn);
@@ -414,6 +422,12 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         vs[i] = (float*)ts.data_ptr();
       }
     }
+    // a parameter listed twice would be stepped by two workgroups at once
+    order.resize(n);
+    for (Py_ssize_t i = 0; i < n; ++i) order[i] = {p[i], p[i] + numel[i]};
+    std::sort(order.begin(), order.end());
+    for (Py_ssize_t i = 1; i < n; ++i)
+      if (order[i].first < order[i - 1].second) value_error("mpnn_amd.optim.adamw_step: two parameters share memory");
     const double max_norm = number(a[14]);
     const c10::OptionalDeviceGuard guard(dev);
     at::Tensor parts, sumsq;

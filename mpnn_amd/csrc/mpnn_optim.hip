@@ -405,6 +405,10 @@ extern "C" int mpnn_adamw_mixed(int n, float* const* params, const float* const*
   for (int j = 0; j < n; ++j) {
     MPNN_CHECK_ARG(params[j] && grads[j] && exp_avg[j] && exp_avg_sq[j] && numel[j] > 0 && numel[j] < (1LL << 32),
                    "mpnn_adamw_mixed: null, empty or oversized tensor");
+    const uintptr_t moments = exp_avg_scale[j] ? 0 : (uintptr_t)exp_avg[j] | (uintptr_t)exp_avg_sq[j];
+    MPNN_CHECK_ARG((((uintptr_t)params[j] | (uintptr_t)grads[j] | (uintptr_t)exp_avg_scale[j] | (uintptr_t)exp_avg_sq_scale[j] |
+                     moments) & 3) == 0,
+                   "mpnn_adamw_mixed: fp32 tensors are aligned to four bytes");
     MPNN_CHECK_ARG(!exp_avg_scale[j] == !exp_avg_sq_scale[j], "mpnn_adamw_mixed: both moments of a tensor have scales, or none");
   }
   AdamHyper h = {};

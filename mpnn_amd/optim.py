@@ -116,6 +116,7 @@ class AdamW(torch.optim.Optimizer):
                                       fused=None, decoupled_weight_decay=True))
         self.max_grad_norm = float(max_grad_norm)
         self.state_bits, self.min_8bit_numel, self.seed = state_bits, int(min_8bit_numel), int(seed)
+        self._zero = torch.tensor(0.0)  # the step count of parameters without a step (8-bit moments)
         self.last_grad_sumsq = None  # device scalar of the last step (its square root is the unclipped gradient norm)
 
     @torch.no_grad()
@@ -128,11 +129,11 @@ class AdamW(torch.optim.Optimizer):
         every = [p for ps in live for p in ps]
         if not every:
             return loss
-        _check(every, "parameters")
-        _check([p.grad for p in every], "gradients")
         if self.state_bits == 8:
             self._step_mixed(live, every)
             return loss
+        _check(every, "parameters")
+        _check([p.grad for p in every], "gradients")
         with torch.cuda.device(every[0].device):
             ss = None
             if self.max_grad_norm > 0.0:  # the clip norm spans every group, as clip_grad_norm_(model.parameters()) does
@@ -170,7 +171,7 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _new_state(self, p):
-        st = {"step": torch.tensor(0.0)}
+        st = {"step": self._zero}
         if p.numel() < self.min_8bit_numel:
             st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
             st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
@@ -181,32 +182,48 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     def _step_mixed(self, live, every):
-        if torch.cuda.is_current_stream_capturing():
+        if every[0].is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("mpnn_amd.optim.AdamW(state_bits=8): a step counts on the host and cannot be captured into a HIP "
                                "graph")
         parts, self.last_grad_sumsq = None, None
         if self.max_grad_norm > 0.0:
             parts = host_call("mpnn_grad_sumsq_parts", "grad_sumsq_parts", [p.grad for p in every])
         first = 0
+        # parameters that took the same steps share one `step` tensor (adding to each of 118 cost more than the kernels): the
+        # next count is a new tensor, parameters without a gradient keep the old one
+        counted, shared = {}, {}
         for group, ps in zip(self.param_groups, live):
             by_step = {}
             for p in ps:
                 st = self.state[p]
                 if not st:
                     st.update(self._new_state(p))
-                st["step"] += 1
-                by_step.setdefault(int(st["step"]), []).append(p)
-            for k, sel in sorted(by_step.items()):
-                states = [self.state[p] for p in sel]
-                lists = [[st.get(n) for st in states] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
-                ss = host_call("mpnn_adamw_mixed", "adamw", sel, [p.grad for p in sel], *lists, k, group["lr"], group["betas"][0],
-                               group["betas"][1], group["eps"], group["weight_decay"], self.seed & 0xFFFFFFFF, first,
-                               self.max_grad_norm, parts)
+                old = st["step"]
+                if id(old) not in counted:
+                    counted[id(old)] = int(old) + 1
+                by_step.setdefault(counted[id(old)], []).append((p, st))
+            for k, sel in sorted(by_step.items(), key=lambda x: x[0]):
+                lists = [[st.get(n) for _, st in sel] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
+                ss = host_call("mpnn_adamw_mixed", "adamw", [p for p, _ in sel], [p.grad for p, _ in sel], *lists, k, group["lr"],
+                               group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"],
+                               self.seed & 0xFFFFFFFF, first, self.max_grad_norm, parts)
                 self.last_grad_sumsq = ss if ss is not None else self.last_grad_sumsq
                 first += len(sel)
+                now = shared.setdefault(k, torch.tensor(float(k)))
+                for _, st in sel:
+                    st["step"] = now
+
+    def state_dict(self):
+        """As torch's; with 8-bit moments every parameter gets a `step` tensor of its own (an optimizer that adds to them in
+        place may load it)."""
+        sd = super().state_dict()
+        if self.state_bits == 8:
+            sd["state"] = {k: {**st, "step": st["step"].clone()} for k, st in sd["state"].items()}
+        return sd
 
     def load_state_dict(self, state_dict):
-        """Checkpoints of 8-bit and of 32-bit moments (this optimizer's, torch's) load into an optimizer of either width."""
+        """Checkpoints of 8-bit and of 32-bit moments (this optimizer's, torch's) load into an optimizer of either width.  With
+        8-bit moments the state is copied: codes and scales of two optimizers may not get out of step."""
         super().load_state_dict(state_dict)
         for p, st in self.state.items():
             if "exp_avg" not in st:
@@ -217,7 +234,9 @@ class AdamW(torch.optim.Optimizer):
                 if scale is None:
                     if wide:
                         st[name], st[name + "_scale"] = pack_moment(st[name], name == "exp_avg_sq")
+                    elif self.state_bits == 8:
+                        st[name] = st[name].clone()
                 elif wide:   # torch has cast the codes to the parameter's type, without loss
-                    st[name], st[name + "_scale"] = st[name].to(torch.float8_e4m3fn), scale
+                    st[name], st[name + "_scale"] = st[name].to(torch.float8_e4m3fn), scale.clone()
                 else:
                     st[name] = unpack_moment(st[name], scale)

@@ -50,7 +50,7 @@ def _run(logits, scores, bias=None, forced=None, n_out=None):
     return got
 
 
-SIZES = [(1, 1, 1), (1, 4, 21), (3, 1, 21), (64, 16, 21), (2, 64, 21), (2, 64, 32), (2, 33, 21), (5, 3, 64), (2, 7, 300),
+SIZES = [(1, 1, 1), (1, 4, 21), (300, 2, 5), (2, 200, 21), (2, 128, 32), (1, 17, 480), (2, 4, 2040), (1, 3, 2700), (3, 1, 21), (64, 16, 21), (2, 64, 21), (2, 64, 32), (2, 33, 21), (5, 3, 64), (2, 7, 300),
          (4, 2, 1000), (2, 5, 1200), (3, 4, 2047), (1, 8, 2048), (2, 3, 5003), (1, 2, 40001), (1, 65, 21), (1, 256, 5)]
 
 
@@ -257,6 +257,26 @@ def test_reorder_interleaved_states_and_overlaps():
     p = torch.nn.Parameter(torch.zeros(2, 3, 4, device="cuda"))
     with pytest.raises(RuntimeError, match="gradients"):
         mpnn_amd.beam_reorder(p, parent.cuda())
+
+
+def test_reorder_of_the_parents_themselves():
+    """A history of parents is a state like any other, also the one that says who moves where, or when."""
+    import mpnn_amd
+    from oracle import beam_oracle as orc
+
+    g = torch.Generator().manual_seed(8)
+    history = torch.randint(0, 5, (3, 5, 7), generator=g)
+    dev = history.cuda()
+    mpnn_amd.beam_reorder(dev, dev[:, :, 2])
+    assert torch.equal(dev.cpu(), orc.reorder(history, history[:, :, 2]))
+    parent = torch.randint(0, 40, (2, 40), generator=g)
+    dev = parent.cuda()
+    mpnn_amd.beam_reorder([dev, dev.clone()], dev)
+    assert torch.equal(dev.cpu(), orc.reorder(parent, parent))
+    table = torch.randint(0, 9, (2, 2, 9), generator=g, dtype=torch.int32)
+    dev = table.cuda()
+    mpnn_amd.beam_reorder(dev, torch.tensor([[1, 0], [1, 1]]).cuda(), length=4, rank=dev[:, 0])
+    assert torch.equal(dev.cpu(), orc.reorder(table, torch.tensor([[1, 0], [1, 1]]), 4, table[:, 0]))
 
 
 def test_reorder_many_states():

@@ -246,6 +246,40 @@ def test_checkpoints_of_either_width(tmp_path):
     run(back, back.param_groups[0]["params"], (3,))
 
 
+def test_step_counts_of_parameters_that_join_later():
+    """Each parameter has its own bias correction; one without a gradient keeps its count; counts survive a checkpoint."""
+    from mpnn_amd.optim import AdamW
+
+    def run(opt, ps, skip):
+        for i, p in enumerate(ps):
+            p.grad = None if i in skip else torch.full_like(p, 0.1 * (i + 1))
+        opt.step()
+
+    new = lambda: [torch.nn.Parameter(torch.ones(n).cuda()) for n in (5000, 100, 70000)]   # noqa: E731
+    ps = new()
+    opt = AdamW(ps, state_bits=8)
+    for skip in ((), (1,), (0, 1), ()):
+        run(opt, ps, skip)
+    assert [float(opt.state[p]["step"]) for p in ps] == [3.0, 2.0, 4.0]
+    ref = [torch.nn.Parameter(torch.ones_like(p)) for p in ps]
+    opt_ref = torch.optim.AdamW(ref)
+    for skip in ((), (1,), (0, 1), ()):
+        run(opt_ref, ref, skip)
+    # constant gradients: every moment of a tensor is the same number, a code times a power of two is 2^-4 off at most, v's
+    # root 2^-5; four steps of 1e-3 each move p by that much of 4e-3
+    for p, q in zip(ps, ref):
+        assert float((p - q).detach().abs().max()) <= 4e-3 * 2 * (2.0**-3 + 2.0**-4)
+    other = new()
+    again = AdamW(other, state_bits=8)
+    again.load_state_dict(opt.state_dict())
+    for p, q in zip(other, ps):
+        p.data.copy_(q)
+    for o, xs in ((opt, ps), (again, other)):
+        run(o, xs, (2,))
+    assert [float(again.state[p]["step"]) for p in other] == [4.0, 3.0, 4.0]
+    assert all(torch.equal(p, q) for p, q in zip(ps, other))
+
+
 def test_refusals():
     from mpnn_amd.optim import AdamW, adamw_step
 
@@ -264,6 +298,13 @@ def test_refusals():
             adamw_step(step=1, **{**good, **change})
     with pytest.raises(ValueError):
         adamw_step(step=0, **good)
+    twice = {n: x * 2 for n, x in good.items()}
+    with pytest.raises(ValueError, match="share memory"):
+        adamw_step(step=1, **twice)
+    long = z(150)
+    lapping = {**{n: x + [y.clone() for y in x] for n, x in good.items()}, "params": [long[:100], long[50:]]}
+    with pytest.raises(ValueError, match="share memory"):
+        adamw_step(step=1, **lapping)
     assert adamw_step([], [], [], [], [], [], step=1) is None
     p = torch.nn.Parameter(z(5000))
     p.grad = torch.ones_like(p)
@@ -274,6 +315,11 @@ def test_refusals():
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             opt.step()
     assert float(opt.state[p]["step"]) == 1.0
+    p.grad = torch.ones(5000, device="cuda")[None][:, ::1].expand(2, 5000)[0].clone()
+    opt.state[p]["exp_avg_scale"] = z(3)
+    with pytest.raises(ValueError):
+        opt.step()
+    assert float(opt.state[p]["step"]) == 1.0, "a refused step does not count"
 
 
 def test_training_step_with_8_bit_moments():
