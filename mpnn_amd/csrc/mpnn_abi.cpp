@@ -40,6 +40,7 @@ extern "C" long long mpnn_workspace_bytes(const char* entry, int n_rows, int n_b
   if (!strcmp(entry, "mpnn_gather_rows")) return (n_blocks > 0 ? n_blocks : 1) * 256LL * f;  // n_blocks = max_chunks
   if (!strcmp(entry, "mpnn_grad_sumsq"))  // n_rows = the largest tensor's elements, n_blocks = tensors
     return ((n_rows + 2047) / 2048) * (long long)(n_blocks > 0 ? n_blocks : 1) * f;
+  if (!strcmp(entry, "mpnn_beam_select")) return -1;  // depends on more than two numbers: mpnn_beam_select_workspace
   if (!strncmp(entry, "mpnn_", 5)) return 0;  // every other entry point works in the caller's inputs and outputs only
   return -1;
 }

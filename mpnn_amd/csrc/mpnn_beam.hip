@@ -20,6 +20,7 @@
 namespace {
 
 constexpr int SEL_MAX_N = 256;       // hypotheses kept of a group
+constexpr int SEL_U = 32;            // logits a thread of a long slice holds
 constexpr int SEL_CAP = 1024;        // candidates a workgroup ranks in LDS
 constexpr long long KEY_NONE = (long long)0x8000000000000000ull;  // below every candidate
 constexpr long long KEY_NAN = 0x7fffffffffffffffll;               // NaN ranks first: a broken beam shows at once
@@ -91,11 +92,43 @@ struct Order<double> {
   }
 };
 
-// some T that at least q lanes' u reach, and seldom half as many more (uniform): bisection over ballots
+// largest and least value of the wave, uniform: rotations within rows of 16 lanes, then one lane of each row
+__device__ __forceinline__ unsigned wave_max_u(unsigned x) {
+#define MPNN_ROR(n)                                                                               \
+  {                                                                                               \
+    const unsigned y = (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + n, 0xf, 0xf, false); \
+    x = y > x ? y : x;                                                                            \
+  }
+  MPNN_ROR(8) MPNN_ROR(4) MPNN_ROR(2) MPNN_ROR(1)
+#undef MPNN_ROR
+  unsigned m = (unsigned)__builtin_amdgcn_readlane((int)x, 0);
+#pragma unroll
+  for (int l = 16; l < 64; l += 16) {
+    const unsigned y = (unsigned)__builtin_amdgcn_readlane((int)x, l);
+    m = y > m ? y : m;
+  }
+  return m;
+}
+__device__ __forceinline__ unsigned wave_min_u(unsigned x) { return ~wave_max_u(~x); }
+
+// Bisection starts at the first bit in which values between least and largest differ: T with the bits they share, and that
+// bit's place (-1: they are equal).  Scores share a sign and most of an exponent.
+__device__ __forceinline__ int common_prefix(unsigned least, unsigned largest, unsigned& T) {
+  const unsigned differ = least ^ largest;
+  const int bit = 31 - __clz((int)differ);     // -1 for 0
+  // (as `bit < 0 ? largest : largest & mask` hipcc 7.2 selects by an SCC that the mask's shift has overwritten)
+  T = largest & (unsigned)(~0ull << (bit + 1));
+  return bit;
+}
+
+// some T that at least q lanes' u reach, and seldom half as many more, 0 if fewer than q are above 0 (uniform): bisection
+// over ballots
 __device__ __forceinline__ unsigned wave_kth(unsigned u, int q) {
-  unsigned T = 0;
+  if (__popcll(__ballot(u != 0)) < q) return 0;
+  unsigned T;
+  int bit = common_prefix(wave_min_u(u ? u : 0xffffffffu), wave_max_u(u), T);
 #pragma unroll 1
-  for (int bit = 31; bit >= 0; --bit) {
+  for (; bit >= 0; --bit) {
     const unsigned t = T | (1u << bit);
     const int cnt = __popcll(__ballot(u >= t));
     if (cnt >= q) {
@@ -399,100 +432,126 @@ k_select_group(SelectArgs a, int g_log2) {
 __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
 
+// U logits of a thread on their way: 16-byte loads, VE = 16 / sizeof(T) neighbours each, 256 VE apart.  They stay packed as
+// they come until they are used: unpacking at the load would wait for each before the next is requested.
+template <typename T, int U, bool BIAS>
+struct Logits {
+  static constexpr int VE = 16 / (int)sizeof(T), WORDS = U * (int)sizeof(T) / 4, PER = 4 / (int)sizeof(T);
+  typedef typename std::conditional<BIAS, double, float>::type X;
+  unsigned q[WORDS];
+  float add[BIAS ? U : 1];
+  // elements base .. base + 256 U of a row (base may lie below 0); what is outside counts as -inf
+  __device__ __forceinline__ void load(const T* row, const float* bias, int base, int V) {
+    if (base >= 0 && base + 256 * U <= V) {
+#pragma unroll
+      for (int it = 0; it < U / VE; ++it) {
+        const int e0 = base + (it * 256 + (int)threadIdx.x) * VE;
+        __builtin_memcpy(q + 4 * it, __builtin_assume_aligned(row + e0, 16), 16);
+        if (BIAS) __builtin_memcpy(add + it * VE, bias + e0, 4 * VE);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      q[i] = 0;
+#pragma unroll
+      for (int h = 0; h < PER; ++h) {
+        const int e = place(base, PER * i + h);
+        const bool in = e >= 0 && e < V;
+        q[i] |= (in ? bits_of(row[e]) : minus_inf()) << (16 * h);
+        if (BIAS) add[BIAS ? PER * i + h : 0] = in ? bias[e] : 0.f;
+      }
+    }
+  }
+  static __device__ __forceinline__ unsigned bits_of(float x) { return __float_as_uint(x); }
+  static __device__ __forceinline__ unsigned bits_of(__hip_bfloat16 x) { return __bfloat16_as_ushort(x); }
+  static __device__ __forceinline__ unsigned bits_of(__half x) { return __half_as_ushort(x); }
+  static __device__ __forceinline__ unsigned minus_inf() {
+    return std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+  }
+  __device__ __forceinline__ X value(int i) const {
+    float x;
+    if (std::is_same<T, float>::value) x = __uint_as_float(q[i / PER]);
+    else if (std::is_same<T, __hip_bfloat16>::value) x = __uint_as_float(i % PER ? q[i / PER] & 0xffff0000u : q[i / PER] << 16);
+    else x = __half2float(__ushort_as_half((unsigned short)(q[i / PER] >> (i % PER * 16))));
+    if (!BIAS) return (X)x;
+    return add[BIAS ? i : 0] == -INFINITY ? (X)-INFINITY : (X)x + (X)add[BIAS ? i : 0];
+  }
+  static __device__ __forceinline__ int place(int base, int i) { return base + (i / VE * 256 + (int)threadIdx.x) * VE + i % VE; }
+};
+
 template <typename T, int U, bool BIAS>
 __global__ void __launch_bounds__(256)
 k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long* __restrict__ pk, int* __restrict__ pi) {
-  __shared__ double rd[4];
+  __shared__ double rd[8];
   __shared__ unsigned ru[4];
   __shared__ int rc;
   __shared__ long long lk[SEL_CAP];
   __shared__ int li[SEL_CAP];
-  constexpr int VE = 16 / (int)sizeof(T);   // elements of a 16-byte load
+  typedef Logits<T, U, BIAS> In;
+  typedef typename In::X X;
   const int row = blockIdx.x / splits, split = blockIdx.x % splits;
   const int b = row / a.W, w = row % a.W, tid = threadIdx.x, wave = tid >> 6;
-  SlicePart* my = part + blockIdx.x;
-  pk += (long long)blockIdx.x * a.n;
-  pi += (long long)blockIdx.x * a.n;
+  // a group's lists lie side by side: entry r of its list l at r * lists + l
+  const int lists = a.W * splits;
+  const long long mine = (long long)b * lists * a.n + w * splits + split;
   if (a.forced && a.forced[row] >= 0) return;     // the second pass knows the row's one candidate
   const T* lrow = (const T*)a.logits + (long long)b * a.sb + (long long)w * a.sw;
   const float* brow = BIAS ? a.bias + (long long)b * a.bb + (long long)w * a.bw : nullptr;
   // slices begin at multiples of 16 bytes of memory, not of the row: every full load is aligned
-  const int mis = (int)(((uintptr_t)lrow & 15) / sizeof(T));
-  const int base = split * (256 * U) - mis;
-  typedef typename std::conditional<BIAS, double, float>::type X;
-  X x[U];
-#pragma unroll
-  for (int it = 0; it < U / VE; ++it) {
-    const int e0 = base + (it * 256 + tid) * VE;
-    T raw[VE];
-    if (e0 >= 0 && e0 + VE <= a.V) {
-      __builtin_memcpy(raw, __builtin_assume_aligned(lrow + e0, 16), 16);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) x[it * VE + i] = (X)to_f(raw[i]);
-      if (BIAS) {
-        float add[VE];
-        __builtin_memcpy(add, brow + e0, 4 * VE);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) x[it * VE + i] = add[i] == -INFINITY ? (X)-INFINITY : x[it * VE + i] + (X)add[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const int e = e0 + i;
-        x[it * VE + i] = (X)-INFINITY;
-        if (e >= 0 && e < a.V) {
-          x[it * VE + i] = (X)to_f(lrow[e]);
-          if (BIAS) x[it * VE + i] = brow[e] == -INFINITY ? (X)-INFINITY : x[it * VE + i] + (X)brow[e];
-        }
-      }
-    }
-  }
-  // maximum, and the sum relative to it
-  X tmax = (X)-INFINITY;
+  const int base = split * (256 * U) - (int)(((uintptr_t)lrow & 15) / sizeof(T));
+  In in;
+  in.load(lrow, brow, base, a.V);
+  X x[U], tmax = (X)-INFINITY;
   bool nan = false;
 #pragma unroll
   for (int i = 0; i < U; ++i) {
+    x[i] = in.value(i);
     tmax = max_of(tmax, x[i]);
     nan |= x[i] != x[i];
   }
-  double top = (double)tmax;
-  top = group_max(top, 64);
   const bool full = base >= 0 && base + 256 * U <= a.V;
   wave_bounds(Order<X>::bits(tmax, nan), a.n, full, ru);
+  double top = group_max((double)tmax, 64);
   if ((tid & 63) == 0) rd[wave] = top;
   if (tid == 0) rc = 0;
   __syncthreads();
   top = fmax(fmax(rd[0], rd[1]), fmax(rd[2], rd[3]));
   const X least = Order<X>::least(block_bound(a.n, full, ru));
-  double sum = nan || top == INFINITY ? (double)NAN : 0.0;
   const double from = top == -INFINITY ? 0.0 : top;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const double xi = (double)x[i];
-    sum += exp_neg(xi - from);
-    if (!(x[i] < least)) {
-      const int p = atomicAdd(&rc, 1);
-      if (p < SEL_CAP) {
-        lk[p] = key_of(xi);
-        li[p] = base + (i / VE * 256 + tid) * VE + i % VE;
+  for (int i = 0; i < U; ++i) s[i & 3] += exp_neg((double)x[i] - from);
+  double sum = nan || top == INFINITY ? (double)NAN : (s[0] + s[1]) + (s[2] + s[3]);
+  if (!(tmax < least) || nan) {            // few threads: one look at the largest instead of one at each
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (!(x[i] < least)) {
+        const int p = atomicAdd(&rc, 1);
+        if (p < SEL_CAP) {
+          lk[p] = key_of((double)x[i]);
+          li[p] = In::place(base, i);
+        }
       }
     }
   }
   sum = group_sum(sum, 64);
-  __syncthreads();                     // rd has been read, the list is complete
-  if ((tid & 63) == 0) rd[wave] = sum;
-  __syncthreads();
+  if ((tid & 63) == 0) rd[4 + wave] = sum;
+  __syncthreads();                         // the list is complete too
   if (tid == 0) {
-    my->top = top;
-    my->sum = top == -INFINITY ? 0.0 : (rd[0] + rd[1]) + (rd[2] + rd[3]);
+    part[blockIdx.x].top = top;
+    part[blockIdx.x].sum = top == -INFINITY ? 0.0 : (rd[4] + rd[5]) + (rd[6] + rd[7]);
   }
   const int cnt = rc;
   if (cnt <= SEL_CAP) {
-    rank_collected(lk, li, cnt, a.n, [&](int r, long long k, int p) { pk[r] = k; pi[r] = p; });
-    for (int r = cnt + tid; r < a.n; r += 256) pk[r] = KEY_NONE;
+    rank_collected(lk, li, cnt, a.n, [&](int r, long long k, int p) {
+      pk[mine + (long long)r * lists] = k;
+      pi[mine + (long long)r * lists] = p;
+    });
+    for (int r = cnt + tid; r < a.n; r += 256) pk[mine + (long long)r * lists] = KEY_NONE;
     return;
   }
-  // more ties than the list holds (constant logits): one after the other
+  // more equal logits than the list holds: one after the other
   long long prev = KEY_NAN;
   int place = -1;
   __shared__ long long sk[4];
@@ -504,35 +563,94 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
     for (int i = 0; i < U; ++i) {
       const double xi = (double)x[i];
       const long long ki = xi == -INFINITY ? KEY_NONE : key_of(xi);
-      const int q = base + (i / VE * 256 + tid) * VE + i % VE;
+      const int q = In::place(base, i);
       if (ki != KEY_NONE && better(prev, place, ki, q) && better(ki, q, k, p)) { k = ki; p = q; }
     }
     block_best(k, p, sk, sp);
-    if (tid == 0) { pk[r] = k; pi[r] = p; }
+    if (tid == 0) {
+      pk[mine + (long long)r * lists] = k;
+      pi[mine + (long long)r * lists] = p;
+    }
     prev = k;
     place = p;
   }
 }
 
+// some T that at least q of the workgroup's values u reach, and seldom a quarter more; 0 if fewer than q are above 0
+template <int E>
+__device__ __forceinline__ unsigned block_kth(const unsigned (&u)[E], int q, unsigned (*cnt)[4]) {
+  unsigned largest = 0, least = 0xffffffffu;
+  int some = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    largest = u[i] > largest ? u[i] : largest;
+    least = u[i] && u[i] < least ? u[i] : least;
+    some += __popcll(__ballot(u[i] != 0));
+  }
+  largest = wave_max_u(largest);
+  least = wave_min_u(least);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    cnt[0][wave] = largest;
+    cnt[1][wave] = least;
+    cnt[2][wave] = some;
+  }
+  __syncthreads();
+  some = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    largest = cnt[0][i] > largest ? cnt[0][i] : largest;
+    least = cnt[1][i] < least ? cnt[1][i] : least;
+    some += cnt[2][i];
+  }
+  if (some < q) return 0;
+  unsigned T;
+  int bit = common_prefix(least, largest, T), turn = 3;
+#pragma unroll 1
+  for (; bit >= 0; --bit) {
+    const unsigned t = T | (1u << bit);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) c += __popcll(__ballot(u[i] >= t));
+    if ((threadIdx.x & 63) == 0) cnt[turn][wave] = c;
+    __syncthreads();
+    c = (int)(cnt[turn][0] + cnt[turn][1] + cnt[turn][2] + cnt[turn][3]);
+    turn ^= 7;             // 3, 4, 3 ...: written again two barriers from here
+    if (c >= q) {
+      T = t;
+      if (c <= q + (q >> 2)) break;
+    }
+  }
+  return T;
+}
+
 // Second pass, one workgroup a group: the beams' log-sum-exps from the slices', then the n best of the slices' lists.  The
-// lists are sorted, so their heads (one a thread) bound the n-th best from below and each list is followed down to that
-// bound only: an entry or two of it as a rule.  A chain of latencies, 7-9 us (17 us at 8 x 33 slices when every thread read
-// its share of all the lists).
+// lists are sorted; the first 256 E entries by depth (all lists' best, all lists' second ...) are in registers before
+// anything else is done and give the bound, and a list goes on beyond them only where its entries still reach it.  A chain
+// of latencies, 7-8 us (with the lists' heads alone as the bound 120 us at 32 beams x 2 slices, 32 kept).
 __global__ void __launch_bounds__(256)
 k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict__ part, const long long* __restrict__ pk,
                const int* __restrict__ pi) {
+  constexpr int E = 4;
   __shared__ double lse[SEL_MAX_N];
   __shared__ float sc[SEL_MAX_N];
   __shared__ int fc[SEL_MAX_N];
-  __shared__ unsigned ru[4];
+  __shared__ unsigned ct[5][4];
   __shared__ int rc;
   __shared__ long long lk[SEL_CAP];
   __shared__ int li[SEL_CAP];
   const int b = blockIdx.x, tid = threadIdx.x;
-  const int lists = a.W * splits;
-  const long long* keys = pk + (long long)b * lists * a.n;
-  const int* places = pi + (long long)b * lists * a.n;
-  const long long head = keys[(long long)(tid < lists ? tid : 0) * a.n];   // under way while the sums are made
+  const int lists = a.W * splits, total = lists * a.n;
+  const long long* keys = pk + (long long)b * total;
+  const int* places = pi + (long long)b * total;
+  long long k[E];
+  int p[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int e = tid + 256 * i;
+    k[i] = keys[e < total ? e : 0];
+    p[i] = places[e < total ? e : 0];
+  }
   // 2^g_log2 lanes a beam
   const int g = 1 << g_log2, j = tid & (g - 1);
   for (int w0 = 0; w0 < a.W; w0 += 256 >> g_log2) {
@@ -542,15 +660,12 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
     const long long f = a.forced ? a.forced[row] : -1;
     const float score = a.scores[row];
     double top = -INFINITY, sum = 0.0;
-    if (f < 0) {
-      const SlicePart* q = part + row * splits;
+    const SlicePart* q = part + row * splits;
+    if (f < 0)
       for (int i = j; i < splits; i += g) top = fmax(top, q[i].top);
-    }
     top = group_max(top, g);
-    if (f < 0) {
-      const SlicePart* q = part + row * splits;
+    if (f < 0)
       for (int i = j; i < splits; i += g) sum += q[i].top == -INFINITY ? q[i].sum : q[i].sum * exp_neg(q[i].top - top);
-    }
     sum = group_sum(sum, g);
     if (live && j == 0) {
       lse[w] = top + log(sum);
@@ -560,43 +675,49 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
   }
   if (tid == 0) rc = 0;
   __syncthreads();
-  // entry r of list l, whose key is kx, as a candidate's key
-  auto candidate = [&](int l, int r, long long kx) -> long long {
-    const int w = l / splits;
-    const bool first = r == 0 && l == w * splits;
-    if (fc[w] >= 0) return first && !(sc[w] == -INFINITY) ? key_of((double)sc[w]) : KEY_NONE;
-    if (broken((double)sc[w], lse[w])) return first ? KEY_NAN : KEY_NONE;
-    if (kx == KEY_NONE) return KEY_NONE;
-    const double c = (double)sc[w] + (value_of(kx) - lse[w]);
-    return c == -INFINITY ? KEY_NONE : key_of(c);
+  // entry e (depth e / lists of list e % lists) with key kx and place px becomes a candidate
+  auto candidate = [&](int e, long long& kx, int& px) {
+    if (e >= total) {
+      kx = KEY_NONE;
+      return;
+    }
+    const int r = e / lists, l = e - r * lists, w = l / splits;
+    const bool head = r == 0 && l == w * splits;
+    if (fc[w] >= 0) {
+      kx = head && !(sc[w] == -INFINITY) ? key_of((double)sc[w]) : KEY_NONE;
+      px = w * a.V + fc[w];
+    } else if (broken((double)sc[w], lse[w])) {
+      kx = head ? KEY_NAN : KEY_NONE;
+      px = w * a.V;
+    } else if (kx != KEY_NONE) {
+      const double c = (double)sc[w] + (value_of(kx) - lse[w]);
+      kx = c == -INFINITY ? KEY_NONE : key_of(c);
+      px += w * a.V;
+    }
   };
-  auto place_of = [&](int l, int px) -> int {
-    const int w = l / splits;
-    if (fc[w] >= 0) return w * a.V + fc[w];
-    return w * a.V + (broken((double)sc[w], lse[w]) ? 0 : px);
-  };
-  long long best = tid < lists ? candidate(tid, 0, head) : KEY_NONE;
-  for (int l = tid + 256; l < lists; l += 256) {
-    const long long k = candidate(l, 0, keys[(long long)l * a.n]);
-    best = k > best ? k : best;
+  unsigned u[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    candidate(tid + 256 * i, k[i], p[i]);
+    u[i] = k[i] == KEY_NONE ? 0u : (unsigned)(k[i] >> 32) ^ 0x80000000u;
   }
-  wave_bounds((unsigned)(best >> 32) ^ 0x80000000u, a.n, false, ru);
-  __syncthreads();
-  const unsigned T = block_bound(a.n, false, ru);
-  for (int l = tid; l < lists; l += 256) {
-    bool more = true;
-    for (int r0 = 0; r0 < a.n && more; r0 += 4) {
-      long long k[4];
+  const unsigned T = block_kth<E>(u, a.n, ct);
+  auto collect = [&](long long kx, int px) {
+    const int q = atomicAdd(&rc, 1);
+    if (q < SEL_CAP) { lk[q] = kx; li[q] = px; }
+  };
 #pragma unroll
-      for (int i = 0; i < 4; ++i) k[i] = keys[(long long)l * a.n + (r0 + i < a.n ? r0 + i : 0)];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const long long ke = r0 + i < a.n ? candidate(l, r0 + i, k[i]) : KEY_NONE;
-        more = more && ke != KEY_NONE && ((unsigned)(ke >> 32) ^ 0x80000000u) >= T;
-        if (more) {
-          const int q = atomicAdd(&rc, 1);
-          if (q < SEL_CAP) { lk[q] = ke; li[q] = place_of(l, places[(long long)l * a.n + r0 + i]); }
-        }
+  for (int i = 0; i < E; ++i)
+    if (k[i] != KEY_NONE && u[i] >= T) collect(k[i], p[i]);
+  if (total > 256 * E) {
+    for (int l = tid; l < lists; l += 256) {
+      // list l's first entry beyond the registers
+      for (int e = l < 256 * E ? l + ((256 * E - 1 - l) / lists + 1) * lists : l; e < total; e += lists) {
+        long long kx = keys[e];
+        int px = places[e];
+        candidate(e, kx, px);
+        if (kx == KEY_NONE || ((unsigned)(kx >> 32) ^ 0x80000000u) < T) break;
+        collect(kx, px);
       }
     }
   }
@@ -615,12 +736,11 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
   for (int r = 0; r < a.n; ++r) {
     long long kb = KEY_NONE;
     int pb = 0x7fffffff;
-    for (int e = tid; e < lists * a.n; e += 256) {
-      const int l = e / a.n;
-      const long long ke = candidate(l, e - l * a.n, keys[e]);
-      if (ke == KEY_NONE) continue;
-      const int pe = place_of(l, places[e]);
-      if (better(prev, place, ke, pe) && better(ke, pe, kb, pb)) { kb = ke; pb = pe; }
+    for (int e = tid; e < total; e += 256) {
+      long long ke = keys[e];
+      int pe = places[e];
+      candidate(e, ke, pe);
+      if (ke != KEY_NONE && better(prev, place, ke, pe) && better(ke, pe, kb, pb)) { kb = ke; pb = pe; }
     }
     block_best(kb, pb, sk, sp);
     if (tid == 0) {
@@ -632,10 +752,11 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
 }
 
 // How a call is split: one wave a group up to 8 candidates a lane (64 x 16 x 21), one workgroup of four waves up to 32 (three
-// beams or more, so that the waves have work), else slices of 256 u logits and a second pass.
+// beams or more, so that the waves have work), else slices of 256 u logits and a second pass: u = 32 where that gives every
+// CU four workgroups, 8 below (32 x 8 x 131072 fp32: 58 us with 32, 63 with 16).
 struct SelectPlan {
   int waves, g_log2, m;  // waves a group, 0 = slices; 2^g_log2 lanes a beam; candidates a lane
-  int u, splits;         // slices
+  int u, splits;         // slices: values a thread holds, slices a beam
 };
 inline SelectPlan select_plan(long long B, int W, int V, int item) {
   SelectPlan p = {};
@@ -650,10 +771,8 @@ inline SelectPlan select_plan(long long B, int W, int V, int item) {
       return p;
     }
   }
-  // 16 values a thread once that gives every CU four workgroups, 8 below (32 x 8 x 131072: 78 us with 16, 86 with 32 - the
-  // registers let four waves a SIMD run instead of six - and 102 with 8, twice the per-slice work)
   const int ve = 16 / item;
-  p.u = B * W * ((V + ve - 1 + 4095LL) / 4096) < 1024 ? 8 : 16;
+  p.u = B * W * ((V + 256LL * SEL_U - 1) / (256LL * SEL_U)) < 1024 ? 8 : SEL_U;
   p.splits = (int)((V + ve - 1 + 256LL * p.u - 1) / (256LL * p.u));
   return p;
 }
@@ -685,7 +804,7 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
     else hipLaunchKernelGGL((k_select_slice<T, U, false>), grid, block, 0, st, a, p.splits, part, pk, pi);       \
   } while (0)
   if (p.u == 8) MPNN_SLICE(8);
-  else MPNN_SLICE(16);
+  else MPNN_SLICE(SEL_U);
 #undef MPNN_SLICE
   int gl = 0;                               // lanes that share a beam's slices
   while (gl < 6 && (1 << gl) < p.splits && (long long)a.W << (gl + 1) <= 256) ++gl;
@@ -986,7 +1105,8 @@ extern "C" int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int
     MPNN_CHECK_ARG(s.data && s.n_mid > 0 && s.run > 0 && (n_beams == 1 || s.stride_beam != 0) &&
                        (n_groups == 1 || s.stride_group != 0) && (s.n_mid == 1 || s.stride_mid != 0),
                    "mpnn_beam_reorder: a state is empty or its rows share memory");
-    MPNN_CHECK_ARG(s.run < (1LL << 31) && ((unsigned long long)(s.run >> state_vec_log2(s, n_beams)) * s.n_mid + 63) / 64 < (1ULL << 31),
+    const int vl = state_vec_log2(s, n_beams);
+    MPNN_CHECK_ARG((s.run >> vl) < (1LL << 32) && ((unsigned long long)(s.run >> vl) * s.n_mid + 63) / 64 < (1ULL << 31),
                    "mpnn_beam_reorder: a state is too large for one launch");
   }
   for (int i0 = 0; i0 < n; i0 += RO_MAX) {

@@ -38,7 +38,7 @@ def test_bad_arguments_are_refused_by_the_library():
         return lib.mpnn_beam_reorder(n, (_lib.BeamState * 1)(_lib.BeamState(**s)), parent, B, W, length_all, None, rank, None)
 
     for kw in (dict(n=0), dict(B=0), dict(B=70000), dict(W=0), dict(W=257), dict(parent=None), dict(rank=P), dict(data=None),
-               dict(stride_beam=0), dict(B=2, stride_group=0), dict(n_mid=3), dict(run=0), dict(run=1 << 31), dict(n_mid=0)):
+               dict(stride_beam=0), dict(B=2, stride_group=0), dict(n_mid=3), dict(run=0), dict(run=1 << 41), dict(n_mid=0)):
         assert reorder(**kw) == -1 and b"mpnn_beam_reorder" in lib.mpnn_last_error(), kw
 
 

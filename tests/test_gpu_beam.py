@@ -148,6 +148,85 @@ def test_select_strides():
         _check(got, orc.select(rep, scores, bias=rep[0, 0]))
 
 
+def test_offsets_beyond_32_bits():
+    """Rows that lie 2^31 elements and more apart: logits of a selection, states of more than 4 GiB."""
+    import mpnn_amd
+    from oracle import beam_oracle as orc
+
+    V, far = 2100, 2**31 + 5
+    buf = torch.zeros(far + V, device="cuda", dtype=torch.float16)
+    rows = buf.as_strided((1, 2, V), (2 * far, far, 1))
+    small = torch.randn(1, 2, V, generator=torch.Generator().manual_seed(2)).half()
+    rows.copy_(small)
+    scores = torch.tensor([[-0.5, -0.25]])
+    _check(mpnn_amd.beam_select(rows, scores.cuda(), n_out=7), orc.select(small, scores, n_out=7))
+    _check(mpnn_amd.beam_select(rows[..., :30], scores.cuda(), n_out=7), orc.select(small[..., :30], scores, n_out=7))
+    del buf, rows
+    n = 2**31 + 64
+    state = torch.zeros(1, 3, n, device="cuda", dtype=torch.uint8)
+    ends = torch.randint(1, 255, (1, 3, 96), generator=torch.Generator().manual_seed(3)).to(torch.uint8)
+    state[..., :32] = ends[..., :32].cuda()
+    state[..., -64:] = ends[..., 32:].cuda()
+    parent = torch.tensor([[2, 0, 0]])
+    mpnn_amd.beam_reorder(state, parent.cuda())
+    want = orc.reorder(ends, parent)
+    assert torch.equal(state[..., :32].cpu(), want[..., :32]) and torch.equal(state[..., -64:].cpu(), want[..., 32:])
+    state = state.view(1, 3, -1, 64)                       # positions of 64 bytes, the last ones alone move back
+    rank = torch.arange(state.shape[2], device="cuda", dtype=torch.int32).flip(0)[None]
+    mpnn_amd.beam_reorder(state, torch.tensor([[1, 2, 1]]).cuda(), length=1, rank=rank)
+    last = orc.reorder(want[..., 32:], torch.tensor([[1, 2, 1]]))
+    assert torch.equal(state[:, :, -1].cpu(), last) and torch.equal(state[:, :, 0, :32].cpu(), want[..., :32])
+
+
+def test_inference_tensors_and_grad_mode():
+    import mpnn_amd
+    from oracle import beam_oracle as orc
+
+    logits, scores, bias, forced = _case(2, 3, 40, torch.float32, 14, "each", 0.2)
+    with torch.inference_mode():
+        dev = [x.cuda() for x in (logits, scores, bias, forced)]
+        out = mpnn_amd.beam_select(*dev)
+        state = torch.arange(2 * 3 * 4.0).view(2, 3, 4)
+        gpu = state.cuda()
+        mpnn_amd.beam_reorder(gpu, out[1])
+    want = orc.select(logits, scores, bias, forced)
+    _check(out, want)
+    assert torch.equal(gpu.cpu(), orc.reorder(state, want[1]))
+    leaf = logits.cuda().requires_grad_()
+    out = mpnn_amd.beam_select(leaf * 1.0, scores.cuda(), bias.cuda(), forced.cuda())
+    assert not out[0].requires_grad
+    _check(out, want)
+
+
+def test_select_refusals():
+    import mpnn_amd
+
+    z = lambda *s: torch.zeros(s, device="cuda")   # noqa: E731
+    ok = dict(logits=z(2, 3, 5), scores=z(2, 3))
+    mpnn_amd.beam_select(**ok)
+    for bad in (dict(logits=z(2, 5)), dict(logits=z(2, 3, 5).double()), dict(logits=z(2, 3, 0)), dict(logits=z(2, 0, 5), scores=z(2, 0)),
+                dict(scores=z(3, 2)), dict(scores=z(2, 3).double()), dict(bias=z(4)), dict(bias=z(5).half()), dict(bias=z(1)[0]),
+                dict(forced=z(2, 3)), dict(n_out=0), dict(n_out=257), dict(logits=z(1, 257, 2), scores=z(1, 257))):
+        with pytest.raises(ValueError, match="beam_select"):
+            mpnn_amd.beam_select(**{**ok, **bad})
+    for bad in (dict(bias=torch.zeros(5)), dict(forced=torch.zeros(2, 3, dtype=torch.int64)), dict(scores=torch.zeros(2, 3)),
+                dict(bias=z(3, 2, 5)), dict(forced=z(4).long())):
+        with pytest.raises(RuntimeError):
+            mpnn_amd.beam_select(**{**ok, **bad})
+    with pytest.raises(TypeError):
+        mpnn_amd.beam_select([1], z(2, 3))
+    parent = torch.zeros(2, 3, device="cuda", dtype=torch.int64)
+    for bad in (dict(states=z(3, 2, 4)), dict(states=z(2)), dict(parent=parent[0]), dict(parent=z(2, 3)), dict(rank=parent),
+                dict(length=3, states=z(2, 3)), dict(length=3, states=[z(2, 3, 4), z(2, 3, 5)]), dict(length=parent[0]),
+                dict(length=3, rank=parent), dict(length=3, rank=z(2, 4))):
+        with pytest.raises(ValueError, match="beam_reorder"):
+            mpnn_amd.beam_reorder(**{**dict(states=z(2, 3, 4), parent=parent), **bad})
+    with pytest.raises(TypeError):
+        mpnn_amd.beam_reorder(7, parent)
+    with pytest.raises(TypeError):
+        mpnn_amd.beam_reorder(z(2, 3, 4), parent, length="x")
+
+
 def test_select_empty_batch_and_repeat():
     import mpnn_amd
 

@@ -280,6 +280,72 @@ def test_step_counts_of_parameters_that_join_later():
     assert all(torch.equal(p, q) for p, q in zip(ps, other))
 
 
+def test_function_in_a_graph_and_on_another_stream():
+    """A captured step is the step (its number, hence its rounding, is the captured one); two graphs share nothing."""
+    from mpnn_amd.optim import adamw_step
+
+    sizes = [5000, 70, 64 * 300]
+    runs = []
+    for captured in (False, True):
+        sets = [Tensors(sizes, 20 + k, lambda n: n > 100) for k in range(2)]
+        grads = [[torch.empty(n, device="cuda") for n in sizes] for _ in range(2)]
+        steps = [lambda t=t, g=g, k=k: adamw_step(t.p, g, t.m, t.v, t.a, t.b, step=3 + k, seed=k, max_grad_norm=0.5)
+                 for k, (t, g) in enumerate(zip(sets, grads))]
+        if captured:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            scratch = Tensors(sizes, 99, lambda n: n > 100)
+            with torch.cuda.stream(side):          # warm-up on tensors of its own, on another stream
+                adamw_step(scratch.p, grads[0], scratch.m, scratch.v, scratch.a, scratch.b, step=1, max_grad_norm=0.5)
+            torch.cuda.current_stream().wait_stream(side)
+            graphs, norms = [], []
+            for f in steps:
+                graphs.append(torch.cuda.CUDAGraph())
+                with torch.cuda.graph(graphs[-1]):
+                    norms.append(f())
+        seen = []
+        for k in range(4):
+            for i in (0, 1):
+                for dst, src in zip(grads[i], _grads(sizes, 60 + 2 * k + i)):
+                    dst.copy_(src)
+                if captured:
+                    graphs[i].replay()
+                    seen.append(float(norms[i]))
+                else:
+                    seen.append(float(steps[i]()))
+        runs.append((seen, [x for t in sets for x in t.lists()]))
+    assert runs[0][0] == runs[1][0]
+    for x, y in zip(runs[0][1], runs[1][1]):
+        for u, v in zip(x, y):
+            assert u is v is None or np.array_equal(u, v)
+
+
+def test_elements_beyond_32_bits_of_offset():
+    """2^31 + 192 elements: addresses pass 2^33 bytes, element numbers 2^31."""
+    from mpnn_amd.optim import adamw_step
+    from oracle import adamw_oracle as orc
+
+    n = 2**31 + 192
+    p, g = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    m, v = (torch.zeros(n, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+    a, b = torch.ones(n // 64, device="cuda"), torch.ones(n // 64, device="cuda")
+    ends = (slice(0, 128), slice(n - 256, n))
+    for s in ends:
+        g[s] = _grads([s.stop - s.start], 70)[0]
+    adamw_step([p], [g], [m], [v], [a], [b], step=1, seed=5, weight_decay=0.0)
+    key = int(orc.random_bits([0], int(orc.random_bits([1], 5)[0]))[0])
+    for s in ends:
+        r = orc.random_bits(np.arange(s.start, s.stop, dtype=np.uint64), key)
+        x = g[s].cpu().double().numpy()
+        for got, scale, want, u, pos in ((m, a, (1.0 - 0.9) * x, r & np.uint32(0xFFFF), False),
+                                         (v, b, (1.0 - 0.999) * (x * x), r >> np.uint32(16), True)):
+            codes, sc = orc.store(want, u / 65536.0, pos)
+            np.testing.assert_array_equal(got[s].cpu().float().double().numpy(), codes)
+            np.testing.assert_array_equal(scale[s.start // 64:s.stop // 64].cpu().double().numpy(), sc)
+        assert bool(((p[s] != 0) == (g[s] != 0)).all())
+    assert int((p != 0).sum()) == sum(int((g[s] != 0).sum()) for s in ends), "nothing else moved"
+
+
 def test_refusals():
     from mpnn_amd.optim import AdamW, adamw_step
 
