@@ -539,8 +539,9 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
   if ((tid & 63) == 0) rd[4 + wave] = sum;
   __syncthreads();                         // the list is complete too
   if (tid == 0) {
-    part[blockIdx.x].top = top;
-    part[blockIdx.x].sum = top == -INFINITY ? 0.0 : (rd[4] + rd[5]) + (rd[6] + rd[7]);
+    const double all = (rd[4] + rd[5]) + (rd[6] + rd[7]);
+    part[blockIdx.x].top = top;            // -inf with a NaN for the sum where the slice holds nothing but NaN
+    part[blockIdx.x].sum = top == -INFINITY && all == all ? 0.0 : all;
   }
   const int cnt = rc;
   if (cnt <= SEL_CAP) {

@@ -119,6 +119,19 @@ def test_select_not_finite(W, V):
     _run(logits, scores, forced=torch.tensor([[1] * W, [-1] * W, [2] * W, [-1] * W]))
 
 
+def test_select_nan_alone_in_its_part_of_the_row():
+    """A long row is read in parts: one that holds a NaN and nothing else that counts breaks its beam all the same."""
+    for V, where in ((2 * 2048 + 1, slice(4096, None)), (3 * 2048, slice(2048, 4096)), (3001, slice(0, 3001))):
+        logits, scores, _, _ = _case(3, 2, V, torch.float32, 13, dead=False)
+        logits[1, 1, where] = math.nan
+        bias = torch.zeros(3, 2, V)
+        bias[1, 1, where] = NEG
+        bias[1, 1, where.start] = 0.0
+        _run(logits, scores)
+        _run(logits, scores, bias)
+        _run(logits.bfloat16(), scores)
+
+
 def test_select_large_magnitudes():
     logits, scores, _, _ = _case(2, 4, 21, torch.float32, 11)
     _run(logits * 1e30, scores)
