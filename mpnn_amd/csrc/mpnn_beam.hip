@@ -336,7 +336,9 @@ k_select_small(SelectArgs a, int g_log2) {
 
 // ---------------------------------------------------------------------------------------------------------------
 // Large vocabularies, first pass: a workgroup reads a slice of 256 U logits of one beam once, keeps it in registers,
-// and leaves the slice's maximum, its sum of exponentials and its n best logits.
+// and leaves the slice's maximum, its sum of exponentials and its `depth` best logits, n + 1 of them where n < 256.  (One
+// more than can be kept: logits that differ may become equal scores, of which the lowest tokens are wanted.  By the entry
+// behind the n-th the second pass sees whether the slice may hold such tokens beside its list.)
 // ---------------------------------------------------------------------------------------------------------------
 struct SlicePart {
   double top, sum;
@@ -482,7 +484,8 @@ struct Logits {
 
 template <typename T, int U, bool BIAS>
 __global__ void __launch_bounds__(256)
-k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long* __restrict__ pk, int* __restrict__ pi) {
+k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part, long long* __restrict__ pk,
+               int* __restrict__ pi) {
   __shared__ double rd[8];
   __shared__ unsigned ru[4];
   __shared__ int rc;
@@ -494,7 +497,7 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
   const int b = row / a.W, w = row % a.W, tid = threadIdx.x, wave = tid >> 6;
   // a group's lists lie side by side: entry r of its list l at r * lists + l
   const int lists = a.W * splits;
-  const long long mine = (long long)b * lists * a.n + w * splits + split;
+  const long long mine = (long long)b * lists * depth + w * splits + split;
   if (a.forced && a.forced[row] >= 0) return;     // the second pass knows the row's one candidate
   const T* lrow = (const T*)a.logits + (long long)b * a.sb + (long long)w * a.sw;
   const float* brow = BIAS ? a.bias + (long long)b * a.bb + (long long)w * a.bw : nullptr;
@@ -511,13 +514,13 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
     nan |= x[i] != x[i];
   }
   const bool full = base >= 0 && base + 256 * U <= a.V;
-  wave_bounds(Order<X>::bits(tmax, nan), a.n, full, ru);
+  wave_bounds(Order<X>::bits(tmax, nan), depth, full, ru);
   double top = group_max((double)tmax, 64);
   if ((tid & 63) == 0) rd[wave] = top;
   if (tid == 0) rc = 0;
   __syncthreads();
   top = fmax(fmax(rd[0], rd[1]), fmax(rd[2], rd[3]));
-  const X least = Order<X>::least(block_bound(a.n, full, ru));
+  const X least = Order<X>::least(block_bound(depth, full, ru));
   const double from = top == -INFINITY ? 0.0 : top;
   double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
@@ -545,11 +548,11 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
   }
   const int cnt = rc;
   if (cnt <= SEL_CAP) {
-    rank_collected(lk, li, cnt, a.n, [&](int r, long long k, int p) {
+    rank_collected(lk, li, cnt, depth, [&](int r, long long k, int p) {
       pk[mine + (long long)r * lists] = k;
       pi[mine + (long long)r * lists] = p;
     });
-    for (int r = cnt + tid; r < a.n; r += 256) pk[mine + (long long)r * lists] = KEY_NONE;
+    for (int r = cnt + tid; r < depth; r += 256) pk[mine + (long long)r * lists] = KEY_NONE;
     return;
   }
   // more equal logits than the list holds: one after the other
@@ -557,7 +560,7 @@ k_select_slice(SelectArgs a, int splits, SlicePart* __restrict__ part, long long
   int place = -1;
   __shared__ long long sk[4];
   __shared__ int sp[4];
-  for (int r = 0; r < a.n; ++r) {
+  for (int r = 0; r < depth; ++r) {
     long long k = KEY_NONE;
     int p = 0x7fffffff;
 #pragma unroll
@@ -625,23 +628,78 @@ __device__ __forceinline__ unsigned block_kth(const unsigned (&u)[E], int q, uns
   return T;
 }
 
+// The last score kept, `kth`, may belong to more candidates than the slices' lists hold.  From slot `slot` on (those before it
+// hold larger scores): the group's candidates of exactly this score, in order, from the logits, up to the last slot.  found: 4
+// words of LDS.
+template <typename T>
+__device__ __forceinline__ void repair_ties(const SelectArgs& a, int b, long long kth, int slot, const double* lse,
+                                            const float* sc, const int* fc, int* found) {
+  constexpr int R = 4;                       // tokens of a thread's turn
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int w = 0; w < a.W && slot < a.n; ++w) {
+    if (fc[w] >= 0 || broken((double)sc[w], lse[w])) {   // one candidate
+      const long long key = fc[w] < 0 ? KEY_NAN : sc[w] == -INFINITY ? KEY_NONE : key_of((double)sc[w]);
+      if (key == kth) {
+        if (tid == 0) write_slot(a, b, slot, key, w * a.V + (fc[w] < 0 ? 0 : fc[w]));
+        ++slot;
+      }
+      continue;
+    }
+    const T* row = (const T*)a.logits + (long long)b * a.sb + (long long)w * a.sw;
+    const float* bias = a.bias ? a.bias + (long long)b * a.bb + (long long)w * a.bw : nullptr;
+    for (int v0 = 0; v0 < a.V && slot < a.n; v0 += 256 * R) {
+      float raw[R], add[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int v = v0 + 256 * i + tid;
+        raw[i] = to_f(row[v < a.V ? v : a.V - 1]);
+        add[i] = bias ? bias[v < a.V ? v : a.V - 1] : 0.f;
+      }
+      unsigned hits = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const double x = add[i] == -INFINITY ? -INFINITY : (double)raw[i] + (double)add[i];
+        const bool in = v0 + 256 * i + tid < a.V && !(x == -INFINITY);
+        hits |= in && key_of((double)sc[w] + (x - lse[w])) == kth ? 1u << i : 0u;
+      }
+      if (!__syncthreads_or((int)hits)) continue;
+      for (int i = 0; i < R; ++i) {
+        const bool hit = hits >> i & 1;
+        const unsigned long long m = __ballot(hit);
+        if (lane == 0) found[wave] = __popcll(m);
+        __syncthreads();
+        int at = slot + __popcll(m & ((1ull << lane) - 1)), all = 0;
+        for (int q = 0; q < 4; ++q) {
+          at += q < wave ? found[q] : 0;
+          all += found[q];
+        }
+        if (hit && at < a.n) write_slot(a, b, at, kth, w * a.V + v0 + 256 * i + tid);
+        slot += all;
+        __syncthreads();
+      }
+    }
+  }
+}
+
 // Second pass, one workgroup a group: the beams' log-sum-exps from the slices', then the n best of the slices' lists.  The
 // lists are sorted; the first 256 E entries by depth (all lists' best, all lists' second ...) are in registers before
 // anything else is done and give the bound, and a list goes on beyond them only where its entries still reach it.  A chain
 // of latencies, 7-8 us (with the lists' heads alone as the bound 120 us at 32 beams x 2 slices, 32 kept).
+template <typename T>
 __global__ void __launch_bounds__(256)
-k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict__ part, const long long* __restrict__ pk,
+k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart* __restrict__ part, const long long* __restrict__ pk,
                const int* __restrict__ pi) {
   constexpr int E = 4;
   __shared__ double lse[SEL_MAX_N];
   __shared__ float sc[SEL_MAX_N];
   __shared__ int fc[SEL_MAX_N];
   __shared__ unsigned ct[5][4];
-  __shared__ int rc;
+  __shared__ int rc, above;
+  __shared__ long long deep, kth;            // best of the lists' last entries; the last score kept
   __shared__ long long lk[SEL_CAP];
   __shared__ int li[SEL_CAP];
   const int b = blockIdx.x, tid = threadIdx.x;
-  const int lists = a.W * splits, total = lists * a.n;
+  const int lists = a.W * splits, total = lists * depth;
   const long long* keys = pk + (long long)b * total;
   const int* places = pi + (long long)b * total;
   long long k[E];
@@ -674,7 +732,10 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
       fc[w] = f < 0 ? -1 : (f < a.V ? (int)f : a.V - 1);
     }
   }
-  if (tid == 0) rc = 0;
+  if (tid == 0) {
+    rc = above = 0;
+    deep = kth = KEY_NONE;
+  }
   __syncthreads();
   // entry e (depth e / lists of list e % lists) with key kx and place px becomes a candidate
   auto candidate = [&](int e, long long& kx, int& px) {
@@ -702,14 +763,15 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
     candidate(tid + 256 * i, k[i], p[i]);
     u[i] = k[i] == KEY_NONE ? 0u : (unsigned)(k[i] >> 32) ^ 0x80000000u;
   }
-  const unsigned T = block_kth<E>(u, a.n, ct);
-  auto collect = [&](long long kx, int px) {
+  const unsigned bound = block_kth<E>(u, a.n, ct);
+  auto collect = [&](int e, long long kx, int px) {
+    if (e >= total - lists) atomicMax(&deep, kx);
     const int q = atomicAdd(&rc, 1);
     if (q < SEL_CAP) { lk[q] = kx; li[q] = px; }
   };
 #pragma unroll
   for (int i = 0; i < E; ++i)
-    if (k[i] != KEY_NONE && u[i] >= T) collect(k[i], p[i]);
+    if (k[i] != KEY_NONE && u[i] >= bound) collect(tid + 256 * i, k[i], p[i]);
   if (total > 256 * E) {
     for (int l = tid; l < lists; l += 256) {
       // list l's first entry beyond the registers
@@ -717,40 +779,58 @@ k_select_merge(SelectArgs a, int splits, int g_log2, const SlicePart* __restrict
         long long kx = keys[e];
         int px = places[e];
         candidate(e, kx, px);
-        if (kx == KEY_NONE || ((unsigned)(kx >> 32) ^ 0x80000000u) < T) break;
-        collect(kx, px);
+        if (kx == KEY_NONE || ((unsigned)(kx >> 32) ^ 0x80000000u) < bound) break;
+        collect(e, kx, px);
       }
     }
   }
   __syncthreads();
   const int cnt = rc;
+  long long last = KEY_NONE;                 // the last score kept and the first slot that holds it
+  int first = 0;
   if (cnt <= SEL_CAP) {
-    rank_collected(lk, li, cnt, a.n, [&](int r, long long ke, int pe) { write_slot(a, b, r, ke, pe); });
+    rank_collected(lk, li, cnt, a.n, [&](int r, long long ke, int pe) {
+      write_slot(a, b, r, ke, pe);
+      if (r == a.n - 1) kth = ke;
+    });
     for (int r = cnt + tid; r < a.n; r += 256) write_dead_slot(a, b, r);
-    return;
-  }
-  // more ties than the list holds: one after the other
-  long long prev = KEY_NAN;
-  int place = -1;
-  __shared__ long long sk[4];
-  __shared__ int sp[4];
-  for (int r = 0; r < a.n; ++r) {
-    long long kb = KEY_NONE;
-    int pb = 0x7fffffff;
-    for (int e = tid; e < total; e += 256) {
-      long long ke = keys[e];
-      int pe = places[e];
-      candidate(e, ke, pe);
-      if (ke != KEY_NONE && better(prev, place, ke, pe) && better(ke, pe, kb, pb)) { kb = ke; pb = pe; }
+    if (deep == KEY_NONE) return;
+    __syncthreads();
+    last = kth;
+    if (deep < last) return;
+    for (int e = tid; e < cnt; e += 256)
+      if (lk[e] > last) atomicAdd(&above, 1);
+    __syncthreads();
+    first = above;
+  } else {
+    // more ties than the list holds: one after the other
+    long long prev = KEY_NAN;
+    int place = -1;
+    __shared__ long long sk[4];
+    __shared__ int sp[4];
+    for (int r = 0; r < a.n; ++r) {
+      long long kb = KEY_NONE;
+      int pb = 0x7fffffff;
+      for (int e = tid; e < total; e += 256) {
+        long long ke = keys[e];
+        int pe = places[e];
+        candidate(e, ke, pe);
+        if (ke != KEY_NONE && better(prev, place, ke, pe) && better(ke, pe, kb, pb)) { kb = ke; pb = pe; }
+      }
+      block_best(kb, pb, sk, sp);
+      if (tid == 0) {
+        if (kb != KEY_NONE) write_slot(a, b, r, kb, pb); else write_dead_slot(a, b, r);
+      }
+      first = kb == prev ? first : r;
+      prev = kb;
+      place = pb;
     }
-    block_best(kb, pb, sk, sp);
-    if (tid == 0) {
-      if (kb != KEY_NONE) write_slot(a, b, r, kb, pb); else write_dead_slot(a, b, r);
-    }
-    prev = kb;
-    place = pb;
+    last = prev;
   }
+  if (last != KEY_NONE && deep >= last) repair_ties<T>(a, b, last, first, lse, sc, fc, (int*)ct);
 }
+
+inline int list_depth(int n) { return n < SEL_MAX_N ? n + 1 : SEL_MAX_N; }   // entries of a slice's list
 
 // How a call is split: one wave a group up to 8 candidates a lane (64 x 16 x 21), one workgroup of four waves up to 32 (three
 // beams or more, so that the waves have work), else slices of 256 u logits and a second pass: u = 32 where that gives every
@@ -797,19 +877,20 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
   const long long parts = (long long)a.B * a.W * p.splits;
   SlicePart* part = (SlicePart*)ws;
   long long* pk = (long long*)(part + parts);
-  int* pi = (int*)(pk + parts * a.n);
+  const int depth = list_depth(a.n);
+  int* pi = (int*)(pk + parts * depth);
   const dim3 grid((unsigned)parts), block(256);
-#define MPNN_SLICE(U)                                                                                            \
-  do {                                                                                                           \
-    if (a.bias) hipLaunchKernelGGL((k_select_slice<T, U, true>), grid, block, 0, st, a, p.splits, part, pk, pi); \
-    else hipLaunchKernelGGL((k_select_slice<T, U, false>), grid, block, 0, st, a, p.splits, part, pk, pi);       \
+#define MPNN_SLICE(U)                                                                                                   \
+  do {                                                                                                                  \
+    if (a.bias) hipLaunchKernelGGL((k_select_slice<T, U, true>), grid, block, 0, st, a, p.splits, depth, part, pk, pi); \
+    else hipLaunchKernelGGL((k_select_slice<T, U, false>), grid, block, 0, st, a, p.splits, depth, part, pk, pi);       \
   } while (0)
   if (p.u == 8) MPNN_SLICE(8);
   else MPNN_SLICE(SEL_U);
 #undef MPNN_SLICE
   int gl = 0;                               // lanes that share a beam's slices
   while (gl < 6 && (1 << gl) < p.splits && (long long)a.W << (gl + 1) <= 256) ++gl;
-  hipLaunchKernelGGL(k_select_merge, dim3(a.B), block, 0, st, a, p.splits, gl, part, pk, pi);
+  hipLaunchKernelGGL((k_select_merge<T>), dim3(a.B), block, 0, st, a, p.splits, depth, gl, part, pk, pi);
   MPNN_LAUNCH_CHECK();
 }
 
@@ -1067,7 +1148,7 @@ extern "C" long long mpnn_beam_select_workspace(int dtype, int n_groups, int n_b
   if (dtype < 0 || dtype > 2 || n_groups <= 0 || n_beams <= 0 || n_tokens <= 0 || n_out <= 0 || n_out > SEL_MAX_N) return -1;
   const SelectPlan p = select_plan(n_groups, n_beams, n_tokens, dtype == 0 ? 4 : 2);
   if (p.waves) return 0;
-  return (long long)n_groups * n_beams * p.splits * ((long long)sizeof(SlicePart) + 12LL * n_out);
+  return (long long)n_groups * n_beams * p.splits * ((long long)sizeof(SlicePart) + 12LL * list_depth(n_out));
 }
 
 extern "C" int mpnn_beam_select(const void* logits, int dtype, long long stride_group, long long stride_beam,
@@ -1086,7 +1167,7 @@ extern "C" int mpnn_beam_select(const void* logits, int dtype, long long stride_
                  "mpnn_beam_select: workspace missing, too small (mpnn_beam_select_workspace) or not 16-byte aligned");
   const SelectPlan p = select_plan(n_groups, n_beams, n_tokens, dtype == 0 ? 4 : 2);
   MPNN_CHECK_ARG((long long)n_groups * n_beams * (p.waves ? 1 : p.splits) < (1LL << 31) &&
-                     (long long)n_beams * (p.waves ? 1 : p.splits) * n_out < (1LL << 31),
+                     (long long)n_beams * (p.waves ? 1 : p.splits) * list_depth(n_out) < (1LL << 31),
                  "mpnn_beam_select: too many groups for one launch");
   SelectArgs a = {logits, stride_group, stride_beam, scores, bias, bias_group, bias_beam, (const long long*)forced,
                   n_groups, n_beams, n_tokens, n_out, out_scores, (long long*)parent, (long long*)token};

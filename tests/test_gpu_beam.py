@@ -132,6 +132,24 @@ def test_select_nan_alone_in_its_part_of_the_row():
         _run(logits.bfloat16(), scores)
 
 
+@pytest.mark.parametrize("W,V", [(4, 21), (2, 64), (1, 5000), (3, 9001), (2, 300)])
+@pytest.mark.parametrize("n_out", [1, 3, 70, 255, 256])
+def test_select_unequal_logits_of_equal_scores(W, V, n_out):
+    """Scores that fp64 cannot tell apart tie, whatever their logits: the lowest tokens are kept."""
+    g = torch.Generator().manual_seed(14)
+    tiny = 1e-25 * torch.randn(2, W, V, generator=g)          # every score is score - log V
+    _run(tiny, torch.zeros(2, W), n_out=n_out)
+    _run(tiny.bfloat16(), -torch.rand(2, W, generator=g), n_out=n_out)
+    few = torch.where(torch.rand(2, W, V, generator=g) < 0.02, tiny, -10.0 - torch.rand(2, W, V, generator=g))
+    _run(few, torch.zeros(2, W), n_out=n_out)                 # a few such tokens above all others
+    _run(few, torch.zeros(2, W), torch.where(torch.rand(V, generator=g) < 0.5, torch.tensor(NEG), torch.tensor(0.0)), n_out=n_out)
+    _run(few, torch.zeros(2, W), forced=torch.tensor([[0] + [-1] * (W - 1)] * 2), n_out=n_out)
+    # scores of 2^40: fp64's step there is 2^-12, so neighbouring logits share one.  Whole quarters with a distance of 2^-14:
+    # all rounding of x - lse (1e-11 at most) stays on its side unless lse lies within that of an odd 2^-13
+    logits = torch.randint(-20, 20, (2, W, V), generator=g) / 4 + torch.randint(0, 3, (2, W, V), generator=g) * 2.0**-14
+    _run(logits, torch.full((2, W), -2.0**40), n_out=n_out)
+
+
 def test_select_large_magnitudes():
     logits, scores, _, _ = _case(2, 4, 21, torch.float32, 11)
     _run(logits * 1e30, scores)
