@@ -765,7 +765,8 @@ int mpnn_mask_self(const int64_t* chain_encoding_all, int B, int L, float* mask_
  * A slot that no candidate is left for gets the score -inf and keeps its beam: parent = slot % n_beams, token = that
  * beam's forced token or 0.  A beam with NaN or +inf among its logits that are not out, or in its score, offers one
  * candidate: token 0, score NaN, ranked first.  Outputs are fully determined by the inputs (no atomics decide anything).
- * n_beams, n_out <= 256, n_tokens <= 2^22.  workspace: mpnn_beam_select_workspace bytes (0: none needed), 16-byte
+ * n_beams, n_out <= 256, n_tokens <= 2^22, n_groups < 2^24 (and n_groups * n_beams slices of long rows: refused where they
+ * do not fit one launch).  workspace: mpnn_beam_select_workspace bytes (0: none needed), 16-byte
  * aligned, overwritten; calls that may overlap need one each.  The outputs may not overlap the inputs. */
 int mpnn_beam_select(const void* logits, int dtype, long long stride_group, long long stride_beam, const float* scores,
                      const float* bias, long long bias_group, long long bias_beam, const int64_t* forced, int n_groups,
@@ -786,7 +787,8 @@ typedef struct mpnn_beam_state {
  * parent outside [0, n_beams) leaves its row as it is.  With a length - length [n_groups] on the device, or length_all >= 0
  * for all groups - only the positions m with rank[b][m] < length move (rank [n_groups][n_mid]; NULL: rank = m), and n_mid
  * is the number of positions of every state; the other positions are not touched.  No two states (and no two rows of one)
- * may share memory.  At most 256 beams and 65535 groups. */
+ * may share memory.  At most 256 beams and 65535 groups, and 2^32 columns of a row (16 bytes where addresses, strides and run
+ * are multiples of 16; one byte where they are odd). */
 int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int64_t* parent, int n_groups, int n_beams,
                       int length_all, const int32_t* length, const int32_t* rank, void* stream);
 

@@ -1166,7 +1166,9 @@ extern "C" int mpnn_beam_select(const void* logits, int dtype, long long stride_
   MPNN_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                  "mpnn_beam_select: workspace missing, too small (mpnn_beam_select_workspace) or not 16-byte aligned");
   const SelectPlan p = select_plan(n_groups, n_beams, n_tokens, dtype == 0 ? 4 : 2);
-  MPNN_CHECK_ARG((long long)n_groups * n_beams * (p.waves ? 1 : p.splits) < (1LL << 31) &&
+  // a launch has less than 2^32 threads; entries of a group's lists are counted in 32 bits
+  MPNN_CHECK_ARG((long long)n_groups < (1LL << 32) / (p.waves == 1 ? 64 : 256) &&
+                     (p.waves || (long long)n_groups * n_beams * p.splits < (1LL << 24)) &&
                      (long long)n_beams * (p.waves ? 1 : p.splits) * list_depth(n_out) < (1LL << 31),
                  "mpnn_beam_select: too many groups for one launch");
   SelectArgs a = {logits, stride_group, stride_beam, scores, bias, bias_group, bias_beam, (const long long*)forced,
@@ -1188,7 +1190,7 @@ extern "C" int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int
                        (n_groups == 1 || s.stride_group != 0) && (s.n_mid == 1 || s.stride_mid != 0),
                    "mpnn_beam_reorder: a state is empty or its rows share memory");
     const int vl = state_vec_log2(s, n_beams);
-    MPNN_CHECK_ARG((s.run >> vl) < (1LL << 32) && ((unsigned long long)(s.run >> vl) * s.n_mid + 63) / 64 < (1ULL << 31),
+    MPNN_CHECK_ARG((s.run >> vl) < (1LL << 32) && ((unsigned long long)(s.run >> vl) * s.n_mid + 63) / 64 < (1ULL << 26),
                    "mpnn_beam_reorder: a state is too large for one launch");
   }
   for (int i0 = 0; i0 < n; i0 += RO_MAX) {

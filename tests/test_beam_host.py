@@ -26,7 +26,8 @@ def test_bad_arguments_are_refused_by_the_library():
         return lib.mpnn_beam_select(logits, dtype, W * V, V, P, None, 0, 0, None, B, W, V, n, P, P, P, ws, size, None)
 
     for kw in (dict(logits=None), dict(dtype=3), dict(B=0), dict(W=0), dict(W=257), dict(V=0), dict(V=(1 << 22) + 1), dict(n=0),
-               dict(n=257), dict(V=100000), dict(V=100000, ws=P, size=64), dict(V=100000, ws=ctypes.c_void_p(4104), size=1 << 30)):
+               dict(n=257), dict(V=100000), dict(V=100000, ws=P, size=64), dict(V=100000, ws=ctypes.c_void_p(4104), size=1 << 30),
+               dict(B=1 << 26), dict(B=1 << 24, W=64), dict(B=1 << 20, W=8, V=9000, ws=P, size=1 << 60)):
         assert select(**kw) == -1 and b"mpnn_beam_select" in lib.mpnn_last_error(), kw
     assert lib.mpnn_beam_select_workspace(0, 4, 4, 21, 4) == 0
     assert lib.mpnn_beam_select_workspace(0, 4, 4, 100000, 4) > 0
@@ -38,7 +39,7 @@ def test_bad_arguments_are_refused_by_the_library():
         return lib.mpnn_beam_reorder(n, (_lib.BeamState * 1)(_lib.BeamState(**s)), parent, B, W, length_all, None, rank, None)
 
     for kw in (dict(n=0), dict(B=0), dict(B=70000), dict(W=0), dict(W=257), dict(parent=None), dict(rank=P), dict(data=None),
-               dict(stride_beam=0), dict(B=2, stride_group=0), dict(n_mid=3), dict(run=0), dict(run=1 << 41), dict(n_mid=0)):
+               dict(stride_beam=0), dict(B=2, stride_group=0), dict(n_mid=3), dict(run=0), dict(run=1 << 41), dict(run=(1 << 32) + 1, stride_beam=1 << 33), dict(n_mid=0)):
         assert reorder(**kw) == -1 and b"mpnn_beam_reorder" in lib.mpnn_last_error(), kw
 
 
