@@ -442,13 +442,13 @@ struct Logits {
   typedef typename std::conditional<BIAS, double, float>::type X;
   unsigned q[WORDS];
   float add[BIAS ? U : 1];
-  // elements base .. base + 256 U of a row (base may lie below 0); what is outside counts as -inf
+  // elements base .. base + 256 U of a row; what is outside counts as -inf
   __device__ __forceinline__ void load(const T* row, const float* bias, int base, int V) {
-    if (base >= 0 && base + 256 * U <= V) {
+    if (base + 256 * U <= V) {
 #pragma unroll
       for (int it = 0; it < U / VE; ++it) {
         const int e0 = base + (it * 256 + (int)threadIdx.x) * VE;
-        __builtin_memcpy(q + 4 * it, __builtin_assume_aligned(row + e0, 16), 16);
+        __builtin_memcpy(q + 4 * it, row + e0, 16);   // of any alignment
         if (BIAS) __builtin_memcpy(add + it * VE, bias + e0, 4 * VE);
       }
       return;
@@ -459,7 +459,7 @@ struct Logits {
 #pragma unroll
       for (int h = 0; h < PER; ++h) {
         const int e = place(base, PER * i + h);
-        const bool in = e >= 0 && e < V;
+        const bool in = e < V;
         q[i] |= (in ? bits_of(row[e]) : minus_inf()) << (16 * h);
         if (BIAS) add[BIAS ? PER * i + h : 0] = in ? bias[e] : 0.f;
       }
@@ -501,8 +501,8 @@ k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part
   if (a.forced && a.forced[row] >= 0) return;     // the second pass knows the row's one candidate
   const T* lrow = (const T*)a.logits + (long long)b * a.sb + (long long)w * a.sw;
   const float* brow = BIAS ? a.bias + (long long)b * a.bb + (long long)w * a.bw : nullptr;
-  // slices begin at multiples of 16 bytes of memory, not of the row: every full load is aligned
-  const int base = split * (256 * U) - (int)(((uintptr_t)lrow & 15) / sizeof(T));
+  // slices are cut by the row's tokens, not by memory's 16 bytes: beams of equal logits have equal sums, bit for bit, and tie
+  const int base = split * (256 * U);
   In in;
   in.load(lrow, brow, base, a.V);
   X x[U], tmax = (X)-INFINITY;
@@ -513,7 +513,7 @@ k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part
     tmax = max_of(tmax, x[i]);
     nan |= x[i] != x[i];
   }
-  const bool full = base >= 0 && base + 256 * U <= a.V;
+  const bool full = base + 256 * U <= a.V;
   wave_bounds(Order<X>::bits(tmax, nan), depth, full, ru);
   double top = group_max((double)tmax, 64);
   if ((tid & 63) == 0) rd[wave] = top;
@@ -839,7 +839,7 @@ struct SelectPlan {
   int waves, g_log2, m;  // waves a group, 0 = slices; 2^g_log2 lanes a beam; candidates a lane
   int u, splits;         // slices: values a thread holds, slices a beam
 };
-inline SelectPlan select_plan(long long B, int W, int V, int item) {
+inline SelectPlan select_plan(long long B, int W, int V) {
   SelectPlan p = {};
   for (int waves = 1; waves <= 4; waves += 3) {
     int gl = 6;
@@ -852,9 +852,8 @@ inline SelectPlan select_plan(long long B, int W, int V, int item) {
       return p;
     }
   }
-  const int ve = 16 / item;
   p.u = B * W * ((V + 256LL * SEL_U - 1) / (256LL * SEL_U)) < 1024 ? 8 : SEL_U;
-  p.splits = (int)((V + ve - 1 + 256LL * p.u - 1) / (256LL * p.u));
+  p.splits = (int)((V + 256LL * p.u - 1) / (256LL * p.u));
   return p;
 }
 
@@ -1146,7 +1145,7 @@ k_beam_place(PlaceArgs a) {
 
 extern "C" long long mpnn_beam_select_workspace(int dtype, int n_groups, int n_beams, int n_tokens, int n_out) {
   if (dtype < 0 || dtype > 2 || n_groups <= 0 || n_beams <= 0 || n_tokens <= 0 || n_out <= 0 || n_out > SEL_MAX_N) return -1;
-  const SelectPlan p = select_plan(n_groups, n_beams, n_tokens, dtype == 0 ? 4 : 2);
+  const SelectPlan p = select_plan(n_groups, n_beams, n_tokens);
   if (p.waves) return 0;
   return (long long)n_groups * n_beams * p.splits * ((long long)sizeof(SlicePart) + 12LL * list_depth(n_out));
 }
@@ -1165,7 +1164,7 @@ extern "C" int mpnn_beam_select(const void* logits, int dtype, long long stride_
   const long long need = mpnn_beam_select_workspace(dtype, n_groups, n_beams, n_tokens, n_out);
   MPNN_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                  "mpnn_beam_select: workspace missing, too small (mpnn_beam_select_workspace) or not 16-byte aligned");
-  const SelectPlan p = select_plan(n_groups, n_beams, n_tokens, dtype == 0 ? 4 : 2);
+  const SelectPlan p = select_plan(n_groups, n_beams, n_tokens);
   // a launch has less than 2^32 threads; entries of a group's lists are counted in 32 bits
   MPNN_CHECK_ARG((long long)n_groups < (1LL << 32) / (p.waves == 1 ? 64 : 256) &&
                      (p.waves || (long long)n_groups * n_beams * p.splits < (1LL << 24)) &&

@@ -150,6 +150,23 @@ def test_select_unequal_logits_of_equal_scores(W, V, n_out):
     _run(logits, torch.full((2, W), -2.0**40), n_out=n_out)
 
 
+@pytest.mark.parametrize("W,V", [(4, 21), (5, 47), (33, 21), (2, 600), (3, 4999), (5, 20011)])
+def test_select_beams_of_equal_logits_tie(W, V):
+    """Equal beams tie to the last bit, wherever their rows begin in memory: the lowest of them is kept for each token."""
+    import mpnn_amd
+    from oracle import beam_oracle as orc
+
+    g = torch.Generator().manual_seed(15)
+    for dtype in (torch.float32, torch.bfloat16):
+        row = (3 * torch.randn(2, 1, V, generator=g)).to(dtype)
+        apart = torch.cat([row] * W, 1)                                            # rows one after the other
+        padded = torch.cat([torch.zeros(2, W, 3, dtype=dtype), apart], 2)[:, :, 3:]
+        want = orc.select(apart, torch.zeros(2, W), None, None, 2 * W)
+        assert torch.equal(want[1][0], torch.arange(W).repeat(2))
+        for logits in (apart.cuda(), padded.cuda(), row.cuda().expand(2, W, V)):
+            _check(mpnn_amd.beam_select(logits, torch.zeros(2, W, device="cuda"), n_out=2 * W), want)
+
+
 def test_select_large_magnitudes():
     logits, scores, _, _ = _case(2, 4, 21, torch.float32, 11)
     _run(logits * 1e30, scores)
