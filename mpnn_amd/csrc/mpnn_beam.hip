@@ -22,6 +22,7 @@ namespace {
 constexpr int SEL_MAX_N = 256;       // hypotheses kept of a group
 constexpr int SEL_U = 32;            // logits a thread of a long slice holds
 constexpr int SEL_CAP = 1024;        // candidates a workgroup ranks in LDS
+constexpr int SEL_LONG = 1024;       // long slices from this many on
 constexpr long long KEY_NONE = (long long)0x8000000000000000ull;  // below every candidate
 constexpr long long KEY_NAN = 0x7fffffffffffffffll;               // NaN ranks first: a broken beam shows at once
 
@@ -92,6 +93,15 @@ struct Order<double> {
   }
 };
 
+// the least X that is not below d
+template <typename X>
+__device__ __forceinline__ X at_least(double d) {
+  const X x = (X)d;
+  if (std::is_same<X, double>::value || !((double)x < d)) return x;
+  const int b = __float_as_int((float)x);
+  return (X)__int_as_float((float)x == 0.f ? 1 : b < 0 ? b - 1 : b + 1);
+}
+
 // largest and least value of the wave, uniform: rotations within rows of 16 lanes, then one lane of each row
 __device__ __forceinline__ unsigned wave_max_u(unsigned x) {
 #define MPNN_ROR(n)                                                                               \
@@ -139,18 +149,20 @@ __device__ __forceinline__ unsigned wave_kth(unsigned u, int q) {
   return T;
 }
 
-// a bound that the n-th best of a 256-thread workgroup's values is no worse than, from each thread's best (u, 0 = none): the
-// least of the waves' ceil(n / 4)-th best threads where every thread has values (close to the n-th best), else the best of
-// the waves' n-th best threads, which threads without values do not spoil.  ru: 4 words of LDS, written here; the caller's
-// barrier follows, then block_bound reads them.
+// a bound that the n-th best of a workgroup's values is no worse than, from each thread's best (u, 0 = none): the least of
+// the four waves' ceil(n / 4)-th best threads where every thread has values (they share a row: close to the n-th best), else the
+// best of the waves' n-th best threads, which threads without values do not spoil.  ru: 4 words of LDS, written here; the
+// caller's barrier follows, then block_bound reads them.
+template <int WAVES>
 __device__ __forceinline__ void wave_bounds(unsigned u, int n, bool full, unsigned* ru) {
-  const unsigned q = wave_kth(u, full || n > 64 ? (n + 3) / 4 : n);
+  const unsigned q = wave_kth(u, WAVES > 1 && (full || n > 64) ? (n + 3) / 4 : n);
   if ((threadIdx.x & 63) == 0) ru[threadIdx.x >> 6] = q;
 }
+template <int WAVES>
 __device__ __forceinline__ unsigned block_bound(int n, bool full, const unsigned* ru) {
   unsigned lo = ru[0], hi = ru[0];
 #pragma unroll
-  for (int i = 1; i < 4; ++i) {
+  for (int i = 1; i < WAVES; ++i) {
     lo = ru[i] < lo ? ru[i] : lo;
     hi = ru[i] > hi ? ru[i] : hi;
   }
@@ -344,10 +356,60 @@ struct SlicePart {
   double top, sum;
 };
 
-// rank the `cnt` <= SEL_CAP collected candidates and hand the n best to put(slot, key, place)
-template <typename Put>
+// some T that at least q of the workgroup's values u reach, and seldom a quarter more; 0 if fewer than q are above 0
+template <int E, int WAVES = 4>
+__device__ __forceinline__ unsigned block_kth(const unsigned (&u)[E], int q, unsigned (*cnt)[4]) {
+  unsigned largest = 0, least = 0xffffffffu;
+  int some = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    largest = u[i] > largest ? u[i] : largest;
+    least = u[i] && u[i] < least ? u[i] : least;
+    some += __popcll(__ballot(u[i] != 0));
+  }
+  largest = wave_max_u(largest);
+  least = wave_min_u(least);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    cnt[0][wave] = largest;
+    cnt[1][wave] = least;
+    cnt[2][wave] = some;
+  }
+  __syncthreads();
+  some = 0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    largest = cnt[0][i] > largest ? cnt[0][i] : largest;
+    least = cnt[1][i] < least ? cnt[1][i] : least;
+    some += cnt[2][i];
+  }
+  if (some < q) return 0;
+  unsigned T;
+  int bit = common_prefix(least, largest, T), turn = 3;
+#pragma unroll 1
+  for (; bit >= 0; --bit) {
+    const unsigned t = T | (1u << bit);
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) c += __popcll(__ballot(u[i] >= t));
+    if ((threadIdx.x & 63) == 0) cnt[turn][wave] = c;
+    __syncthreads();
+    c = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) c += (int)cnt[turn][i];
+    turn ^= 7;             // 3, 4, 3 ...: written again two barriers from here
+    if (c >= q) {
+      T = t;
+      if (c <= q + (q >> 2)) break;
+    }
+  }
+  return T;
+}
+
+// rank the `cnt` collected candidates and hand the n best to put(slot, key, place)
+template <int WAVES = 4, typename Put>
 __device__ __forceinline__ void rank_collected(const long long* lk, const int* li, int cnt, int n, Put put) {
-  for (int e = threadIdx.x; e < cnt; e += 256) {
+  for (int e = threadIdx.x; e < cnt; e += 64 * WAVES) {
     const long long ke = lk[e];
     const int ie = li[e];
     int r = 0;
@@ -355,6 +417,36 @@ __device__ __forceinline__ void rank_collected(const long long* lk, const int* l
     for (int q = 0; q < cnt; ++q) r += better(lk[q], li[q], ke, ie);
     if (r < n) put(r, ke, ie);
   }
+}
+
+// Ranking compares every collected candidate with every other one.  Where the first bound let many through, the best of
+// those in the list give a closer one: collect(least) puts what is not below `least` into the list again, counting in rc.
+// Returns the list's length; more than CAP where too many are equal.  (256 x 60 beams x 1000 tokens, 60 kept: lists of 600 and
+// 1136 us before, 146 with this.)
+template <int CAP, int WAVES, typename Collect>
+__device__ __forceinline__ int collect_fewer(int q, const long long* lk, int* rc, unsigned (*ct)[4], Collect collect) {
+  constexpr int T = 64 * WAVES;
+  unsigned last = 0;
+  int cnt = *rc;
+#pragma unroll 1
+  while (cnt > 256 && cnt > 2 * q) {
+    unsigned u[CAP / T];
+#pragma unroll
+    for (int i = 0; i < CAP / T; ++i) {
+      const int e = threadIdx.x + T * i;
+      u[i] = e < cnt ? (unsigned)(lk[e] >> 32) ^ 0x80000000u : 0u;
+    }
+    const unsigned bound = block_kth<CAP / T, WAVES>(u, q, ct);
+    if (bound <= last) break;
+    last = bound;
+    __syncthreads();                         // everybody has read the list
+    if (threadIdx.x == 0) *rc = 0;
+    __syncthreads();
+    collect(value_of((long long)((unsigned long long)(bound ^ 0x80000000u) << 32)), bound);
+    __syncthreads();
+    cnt = *rc;
+  }
+  return cnt;
 }
 
 // best of the workgroup's (key, place) pairs; every thread gets it
@@ -380,30 +472,30 @@ __device__ __forceinline__ void block_best(long long& k, int& p, long long* sk, 
 template <typename T, int M>
 __global__ void __launch_bounds__(256)
 k_select_group(SelectArgs a, int g_log2) {
-  __shared__ unsigned ru[4];
+  __shared__ unsigned ct[5][4];
   __shared__ int rc;
   __shared__ long long lk[SEL_CAP];
   __shared__ int li[SEL_CAP];
   const int b = blockIdx.x, tid = threadIdx.x, w = tid >> g_log2, j = tid & ((1 << g_log2) - 1);
   long long k[M];
-  const long long best = lane_candidates<T, M>(a, b, w, j, g_log2, k);
-  const bool full = a.W << g_log2 >= 256;
-  wave_bounds((unsigned)(best >> 32) ^ 0x80000000u, a.n, full, ru);
+  const unsigned best[1] = {(unsigned)(lane_candidates<T, M>(a, b, w, j, g_log2, k) >> 32) ^ 0x80000000u};   // 0: none
   if (tid == 0) rc = 0;
-  __syncthreads();
-  const unsigned T32 = block_bound(a.n, full, ru);
+  const unsigned first = block_kth<1>(best, a.n, ct);   // the n-th best thread, or 0
+  auto collect = [&](double, unsigned bound) {
 #pragma unroll
-  for (int i = 0; i < M; ++i) {
-    if (k[i] != KEY_NONE && ((unsigned)(k[i] >> 32) ^ 0x80000000u) >= T32) {
-      const int q = atomicAdd(&rc, 1);
-      if (q < SEL_CAP) {
-        lk[q] = k[i];
-        li[q] = w * a.V + j + (i << g_log2);
+    for (int i = 0; i < M; ++i) {
+      if (k[i] != KEY_NONE && ((unsigned)(k[i] >> 32) ^ 0x80000000u) >= bound) {
+        const int q = atomicAdd(&rc, 1);
+        if (q < SEL_CAP) {
+          lk[q] = k[i];
+          li[q] = w * a.V + j + (i << g_log2);
+        }
       }
     }
-  }
+  };
+  collect(0.0, first);
   __syncthreads();
-  const int cnt = rc;
+  const int cnt = collect_fewer<SEL_CAP, 4>(a.n, lk, &rc, ct, collect);
   if (cnt <= SEL_CAP) {
     rank_collected(lk, li, cnt, a.n, [&](int r, long long ke, int pe) { write_slot(a, b, r, ke, pe); });
     for (int r = cnt + tid; r < a.n; r += 256) write_dead_slot(a, b, r);
@@ -434,34 +526,33 @@ k_select_group(SelectArgs a, int g_log2) {
 __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
 
-// U logits of a thread on their way: 16-byte loads, VE = 16 / sizeof(T) neighbours each, 256 VE apart.  They stay packed as
+// U logits of a thread on their way: 16-byte loads, VE = 16 / sizeof(T) neighbours each, THREADS VE apart.  They stay packed as
 // they come until they are used: unpacking at the load would wait for each before the next is requested.
-template <typename T, int U, bool BIAS>
+template <typename T, int U, bool BIAS, int THREADS>
 struct Logits {
   static constexpr int VE = 16 / (int)sizeof(T), WORDS = U * (int)sizeof(T) / 4, PER = 4 / (int)sizeof(T);
   typedef typename std::conditional<BIAS, double, float>::type X;
   unsigned q[WORDS];
   float add[BIAS ? U : 1];
-  // elements base .. base + 256 U of a row; what is outside counts as -inf
+  // elements base .. base + THREADS U of a row; what is outside counts as -inf
   __device__ __forceinline__ void load(const T* row, const float* bias, int base, int V) {
-    if (base + 256 * U <= V) {
 #pragma unroll
-      for (int it = 0; it < U / VE; ++it) {
-        const int e0 = base + (it * 256 + (int)threadIdx.x) * VE;
-        __builtin_memcpy(q + 4 * it, row + e0, 16);   // of any alignment
+    for (int it = 0; it < U / VE; ++it) {
+      const int c0 = base + it * THREADS * VE, e0 = c0 + (int)threadIdx.x * VE;   // of the turn, of this thread
+      if (c0 + THREADS * VE <= V) {
+        __builtin_memcpy(q + 4 * it, row + e0, 16);                               // of any alignment
         if (BIAS) __builtin_memcpy(add + it * VE, bias + e0, 4 * VE);
-      }
-      return;
-    }
+      } else {
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i) {
-      q[i] = 0;
+        for (int i = 0; i < 4; ++i) {
+          q[4 * it + i] = 0;
 #pragma unroll
-      for (int h = 0; h < PER; ++h) {
-        const int e = place(base, PER * i + h);
-        const bool in = e < V;
-        q[i] |= (in ? bits_of(row[e]) : minus_inf()) << (16 * h);
-        if (BIAS) add[BIAS ? PER * i + h : 0] = in ? bias[e] : 0.f;
+          for (int h = 0; h < PER; ++h) {
+            const int e = e0 + PER * i + h;
+            q[4 * it + i] |= (e < V ? bits_of(row[e]) : minus_inf()) << (16 * h);
+            if (BIAS) add[BIAS ? it * VE + PER * i + h : 0] = e < V ? bias[e] : 0.f;
+          }
+        }
       }
     }
   }
@@ -479,19 +570,22 @@ struct Logits {
     if (!BIAS) return (X)x;
     return add[BIAS ? i : 0] == -INFINITY ? (X)-INFINITY : (X)x + (X)add[BIAS ? i : 0];
   }
-  static __device__ __forceinline__ int place(int base, int i) { return base + (i / VE * 256 + (int)threadIdx.x) * VE + i % VE; }
+  static __device__ __forceinline__ int place(int base, int i) {
+    return base + (i / VE * THREADS + (int)threadIdx.x) * VE + i % VE;
+  }
 };
 
-template <typename T, int U, bool BIAS>
-__global__ void __launch_bounds__(256)
+template <typename T, int U, bool BIAS, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, U > 8 ? 4 : 1)
 k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part, long long* __restrict__ pk,
                int* __restrict__ pi) {
-  __shared__ double rd[8];
-  __shared__ unsigned ru[4];
+  constexpr int THREADS = 64 * WAVES, CAP = WAVES == 1 ? 64 * U : SEL_CAP;   // one wave's list holds its whole slice
+  __shared__ double rd[2 * WAVES];
+  __shared__ unsigned ru[4], ct[5][4];
   __shared__ int rc;
-  __shared__ long long lk[SEL_CAP];
-  __shared__ int li[SEL_CAP];
-  typedef Logits<T, U, BIAS> In;
+  __shared__ long long lk[CAP];
+  __shared__ int li[CAP];
+  typedef Logits<T, U, BIAS, THREADS> In;
   typedef typename In::X X;
   const int row = blockIdx.x / splits, split = blockIdx.x % splits;
   const int b = row / a.W, w = row % a.W, tid = threadIdx.x, wave = tid >> 6;
@@ -502,7 +596,7 @@ k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part
   const T* lrow = (const T*)a.logits + (long long)b * a.sb + (long long)w * a.sw;
   const float* brow = BIAS ? a.bias + (long long)b * a.bb + (long long)w * a.bw : nullptr;
   // slices are cut by the row's tokens, not by memory's 16 bytes: beams of equal logits have equal sums, bit for bit, and tie
-  const int base = split * (256 * U);
+  const int base = split * (THREADS * U);
   In in;
   in.load(lrow, brow, base, a.V);
   X x[U], tmax = (X)-INFINITY;
@@ -513,48 +607,62 @@ k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part
     tmax = max_of(tmax, x[i]);
     nan |= x[i] != x[i];
   }
-  const bool full = base + 256 * U <= a.V;
-  wave_bounds(Order<X>::bits(tmax, nan), depth, full, ru);
+  const bool full = base + THREADS * U <= a.V;
+  wave_bounds<WAVES>(Order<X>::bits(tmax, nan), depth, full, ru);
   double top = group_max((double)tmax, 64);
   if ((tid & 63) == 0) rd[wave] = top;
   if (tid == 0) rc = 0;
   __syncthreads();
-  top = fmax(fmax(rd[0], rd[1]), fmax(rd[2], rd[3]));
-  const X least = Order<X>::least(block_bound(depth, full, ru));
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) top = fmax(top, rd[i]);
+  const X least = Order<X>::least(block_bound<WAVES>(depth, full, ru));
   const double from = top == -INFINITY ? 0.0 : top;
   double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
   for (int i = 0; i < U; ++i) s[i & 3] += exp_neg((double)x[i] - from);
   double sum = nan || top == INFINITY ? (double)NAN : (s[0] + s[1]) + (s[2] + s[3]);
+  auto put = [&](X xi, int place) {
+    const int p = atomicAdd(&rc, 1);
+    if (p < CAP) {
+      lk[p] = key_of((double)xi);
+      li[p] = place;
+    }
+  };
   if (!(tmax < least) || nan) {            // few threads: one look at the largest instead of one at each
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (!(x[i] < least)) {
-        const int p = atomicAdd(&rc, 1);
-        if (p < SEL_CAP) {
-          lk[p] = key_of((double)x[i]);
-          li[p] = In::place(base, i);
-        }
-      }
-    }
+    for (int i = 0; i < U; ++i)
+      if (!(x[i] < least)) put(x[i], In::place(base, i));
   }
   sum = group_sum(sum, 64);
-  if ((tid & 63) == 0) rd[4 + wave] = sum;
+  if ((tid & 63) == 0) rd[WAVES + wave] = sum;
   __syncthreads();                         // the list is complete too
   if (tid == 0) {
-    const double all = (rd[4] + rd[5]) + (rd[6] + rd[7]);
+    double all = rd[WAVES];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) all += rd[WAVES + i];
     part[blockIdx.x].top = top;            // -inf with a NaN for the sum where the slice holds nothing but NaN
     part[blockIdx.x].sum = top == -INFINITY && all == all ? 0.0 : all;
   }
-  const int cnt = rc;
-  if (cnt <= SEL_CAP) {
-    rank_collected(lk, li, cnt, depth, [&](int r, long long k, int p) {
+  // (a second time from memory: a second use of the logits in registers costs the main path a wave or two a SIMD)
+  const int cnt = collect_fewer<CAP, WAVES>(depth, lk, &rc, ct, [&](double lowest, unsigned) {
+    const X bound = at_least<X>(lowest);
+#pragma unroll 4
+    for (int e = base + tid; e < base + THREADS * U; e += THREADS) {
+      if (e >= a.V) break;
+      X xe = (X)to_f(lrow[e]);
+      if (BIAS) xe = brow[e] == -INFINITY ? (X)-INFINITY : xe + (X)brow[e];
+      if (!(xe < bound)) put(xe, e);
+    }
+  });
+  if (cnt <= CAP) {
+    rank_collected<WAVES>(lk, li, cnt, depth, [&](int r, long long k, int p) {
       pk[mine + (long long)r * lists] = k;
       pi[mine + (long long)r * lists] = p;
     });
-    for (int r = cnt + tid; r < depth; r += 256) pk[mine + (long long)r * lists] = KEY_NONE;
+    for (int r = cnt + tid; r < depth; r += THREADS) pk[mine + (long long)r * lists] = KEY_NONE;
     return;
   }
+  if (WAVES == 1) return;                  // not reached: the list holds the slice
   // more equal logits than the list holds: one after the other
   long long prev = KEY_NAN;
   int place = -1;
@@ -578,54 +686,6 @@ k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part
     prev = k;
     place = p;
   }
-}
-
-// some T that at least q of the workgroup's values u reach, and seldom a quarter more; 0 if fewer than q are above 0
-template <int E>
-__device__ __forceinline__ unsigned block_kth(const unsigned (&u)[E], int q, unsigned (*cnt)[4]) {
-  unsigned largest = 0, least = 0xffffffffu;
-  int some = 0;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    largest = u[i] > largest ? u[i] : largest;
-    least = u[i] && u[i] < least ? u[i] : least;
-    some += __popcll(__ballot(u[i] != 0));
-  }
-  largest = wave_max_u(largest);
-  least = wave_min_u(least);
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) {
-    cnt[0][wave] = largest;
-    cnt[1][wave] = least;
-    cnt[2][wave] = some;
-  }
-  __syncthreads();
-  some = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    largest = cnt[0][i] > largest ? cnt[0][i] : largest;
-    least = cnt[1][i] < least ? cnt[1][i] : least;
-    some += cnt[2][i];
-  }
-  if (some < q) return 0;
-  unsigned T;
-  int bit = common_prefix(least, largest, T), turn = 3;
-#pragma unroll 1
-  for (; bit >= 0; --bit) {
-    const unsigned t = T | (1u << bit);
-    int c = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) c += __popcll(__ballot(u[i] >= t));
-    if ((threadIdx.x & 63) == 0) cnt[turn][wave] = c;
-    __syncthreads();
-    c = (int)(cnt[turn][0] + cnt[turn][1] + cnt[turn][2] + cnt[turn][3]);
-    turn ^= 7;             // 3, 4, 3 ...: written again two barriers from here
-    if (c >= q) {
-      T = t;
-      if (c <= q + (q >> 2)) break;
-    }
-  }
-  return T;
 }
 
 // The last score kept, `kth`, may belong to more candidates than the slices' lists hold.  From slot `slot` on (those before it
@@ -683,7 +743,7 @@ __device__ __forceinline__ void repair_ties(const SelectArgs& a, int b, long lon
 
 // Second pass, one workgroup a group: the beams' log-sum-exps from the slices', then the n best of the slices' lists.  The
 // lists are sorted; the first 256 E entries by depth (all lists' best, all lists' second ...) are in registers before
-// anything else is done and give the bound, and a list goes on beyond them only where its entries still reach it.  A chain
+// anything else is done and give the bound, and lists go on beyond them only where their entries still reach it.  A chain
 // of latencies, 7-8 us (with the lists' heads alone as the bound 120 us at 32 beams x 2 slices, 32 kept).
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -694,7 +754,7 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
   __shared__ float sc[SEL_MAX_N];
   __shared__ int fc[SEL_MAX_N];
   __shared__ unsigned ct[5][4];
-  __shared__ int rc, above;
+  __shared__ int rc, above, reach;           // reach: the last entry collected
   __shared__ long long deep, kth;            // best of the lists' last entries; the last score kept
   __shared__ long long lk[SEL_CAP];
   __shared__ int li[SEL_CAP];
@@ -733,7 +793,7 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
     }
   }
   if (tid == 0) {
-    rc = above = 0;
+    rc = above = reach = 0;
     deep = kth = KEY_NONE;
   }
   __syncthreads();
@@ -763,29 +823,41 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
     candidate(tid + 256 * i, k[i], p[i]);
     u[i] = k[i] == KEY_NONE ? 0u : (unsigned)(k[i] >> 32) ^ 0x80000000u;
   }
-  const unsigned bound = block_kth<E>(u, a.n, ct);
-  auto collect = [&](int e, long long kx, int px) {
+  const unsigned first_bound = block_kth<E>(u, a.n, ct);
+  auto take = [&](int e, long long kx, int px, unsigned bound) {
+    if (kx == KEY_NONE || ((unsigned)(kx >> 32) ^ 0x80000000u) < bound) return;
     if (e >= total - lists) atomicMax(&deep, kx);
+    if (total > 256 * E) atomicMax(&reach, e);
     const int q = atomicAdd(&rc, 1);
     if (q < SEL_CAP) { lk[q] = kx; li[q] = px; }
   };
+  // A list's entry counts only where the one before it, `lists` places earlier, does: entries beyond the registers are looked
+  // at while that may be, 256 E at a time.  (One thread walking down a list: 40 us where one beam of 60 has most of the best.)
+  auto collect = [&](double, unsigned bound) {
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    if (k[i] != KEY_NONE && u[i] >= bound) collect(tid + 256 * i, k[i], p[i]);
-  if (total > 256 * E) {
-    for (int l = tid; l < lists; l += 256) {
-      // list l's first entry beyond the registers
-      for (int e = l < 256 * E ? l + ((256 * E - 1 - l) / lists + 1) * lists : l; e < total; e += lists) {
-        long long kx = keys[e];
-        int px = places[e];
-        candidate(e, kx, px);
-        if (kx == KEY_NONE || ((unsigned)(kx >> 32) ^ 0x80000000u) < bound) break;
-        collect(e, kx, px);
+    for (int i = 0; i < E; ++i) take(tid + 256 * i, k[i], p[i], bound);
+    for (int base = 256 * E; base < total; base += 256 * E) {
+      __syncthreads();
+      if (base > reach + lists) break;
+      __syncthreads();
+      long long kx[E];
+      int px[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int e = base + tid + 256 * i;
+        kx[i] = keys[e < total ? e : 0];
+        px[i] = places[e < total ? e : 0];
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        candidate(base + tid + 256 * i, kx[i], px[i]);
+        take(base + tid + 256 * i, kx[i], px[i], bound);
       }
     }
-  }
+  };
+  collect(0.0, first_bound);
   __syncthreads();
-  const int cnt = rc;
+  const int cnt = collect_fewer<SEL_CAP, 4>(a.n, lk, &rc, ct, collect);
   long long last = KEY_NONE;                 // the last score kept and the first slot that holds it
   int first = 0;
   if (cnt <= SEL_CAP) {
@@ -833,11 +905,12 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
 inline int list_depth(int n) { return n < SEL_MAX_N ? n + 1 : SEL_MAX_N; }   // entries of a slice's list
 
 // How a call is split: one wave a group up to 8 candidates a lane (64 x 16 x 21), one workgroup of four waves up to 32 (three
-// beams or more, so that the waves have work), else slices of 256 u logits and a second pass: u = 32 where that gives every
-// CU four workgroups, 8 below (32 x 8 x 131072 fp32: 58 us with 32, 63 with 16).
+// beams or more, so that the waves have work), else slices and a second pass.  A slice is a row of up to 512 logits for one
+// wave, else 256 u logits for four: u = 32 where that gives every CU SEL_LONG workgroups, 8 below (32 x 8 x 131072 fp32: 58 us
+// with 32, 63 with 16).
 struct SelectPlan {
   int waves, g_log2, m;  // waves a group, 0 = slices; 2^g_log2 lanes a beam; candidates a lane
-  int u, splits;         // slices: values a thread holds, slices a beam
+  int u, per, splits;    // slices: values a thread holds, waves a slice, slices a beam
 };
 inline SelectPlan select_plan(long long B, int W, int V) {
   SelectPlan p = {};
@@ -852,8 +925,9 @@ inline SelectPlan select_plan(long long B, int W, int V) {
       return p;
     }
   }
-  p.u = B * W * ((V + 256LL * SEL_U - 1) / (256LL * SEL_U)) < 1024 ? 8 : SEL_U;
-  p.splits = (int)((V + 256LL * p.u - 1) / (256LL * p.u));
+  p.per = V <= 512 ? 1 : 4;
+  p.u = p.per == 1 || B * W * (V / (256 * SEL_U)) < SEL_LONG ? 8 : SEL_U;
+  p.splits = (V + 64 * p.per * p.u - 1) / (64 * p.per * p.u);
   return p;
 }
 
@@ -879,13 +953,18 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
   const int depth = list_depth(a.n);
   int* pi = (int*)(pk + parts * depth);
   const dim3 grid((unsigned)parts), block(256);
-#define MPNN_SLICE(U)                                                                                                   \
-  do {                                                                                                                  \
-    if (a.bias) hipLaunchKernelGGL((k_select_slice<T, U, true>), grid, block, 0, st, a, p.splits, depth, part, pk, pi); \
-    else hipLaunchKernelGGL((k_select_slice<T, U, false>), grid, block, 0, st, a, p.splits, depth, part, pk, pi);       \
+#define MPNN_SLICE(U, WAVES)                                                                                             \
+  do {                                                                                                                   \
+    if (a.bias)                                                                                                          \
+      hipLaunchKernelGGL((k_select_slice<T, U, true, WAVES>), grid, dim3(64 * WAVES), 0, st, a, p.splits, depth, part,   \
+                         pk, pi);                                                                                        \
+    else                                                                                                                 \
+      hipLaunchKernelGGL((k_select_slice<T, U, false, WAVES>), grid, dim3(64 * WAVES), 0, st, a, p.splits, depth, part,  \
+                         pk, pi);                                                                                        \
   } while (0)
-  if (p.u == 8) MPNN_SLICE(8);
-  else MPNN_SLICE(SEL_U);
+  if (p.per == 1) MPNN_SLICE(8, 1);
+  else if (p.u == 8) MPNN_SLICE(8, 4);
+  else MPNN_SLICE(SEL_U, 4);
 #undef MPNN_SLICE
   int gl = 0;                               // lanes that share a beam's slices
   while (gl < 6 && (1 << gl) < p.splits && (long long)a.W << (gl + 1) <= 256) ++gl;
