@@ -22,7 +22,7 @@ namespace {
 constexpr int SEL_MAX_N = 256;       // hypotheses kept of a group
 constexpr int SEL_U = 32;            // logits a thread of a long slice holds
 constexpr int SEL_CAP = 1024;        // candidates a workgroup ranks in LDS
-constexpr int SEL_LONG = 1024;       // long slices from this many on
+constexpr int SEL_LONG = 300;        // long slices from this many on: about one a CU
 constexpr long long KEY_NONE = (long long)0x8000000000000000ull;  // below every candidate
 constexpr long long KEY_NAN = 0x7fffffffffffffffll;               // NaN ranks first: a broken beam shows at once
 
@@ -131,16 +131,27 @@ __device__ __forceinline__ int common_prefix(unsigned least, unsigned largest, u
   return bit;
 }
 
-// some T that at least q lanes' u reach, and seldom half as many more, 0 if fewer than q are above 0 (uniform): bisection
-// over ballots
-__device__ __forceinline__ unsigned wave_kth(unsigned u, int q) {
-  if (__popcll(__ballot(u != 0)) < q) return 0;
+// some T that at least q of the wave's values u reach, and seldom half as many more, 0 if fewer than q are above 0 (uniform):
+// bisection over ballots
+template <int E>
+__device__ __forceinline__ unsigned wave_kth(const unsigned (&u)[E], int q) {
+  unsigned largest = 0, least = 0xffffffffu;
+  int some = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    largest = u[i] > largest ? u[i] : largest;
+    least = u[i] && u[i] < least ? u[i] : least;
+    some += __popcll(__ballot(u[i] != 0));
+  }
+  if (some < q) return 0;
   unsigned T;
-  int bit = common_prefix(wave_min_u(u ? u : 0xffffffffu), wave_max_u(u), T);
+  int bit = common_prefix(wave_min_u(least), wave_max_u(largest), T);
 #pragma unroll 1
   for (; bit >= 0; --bit) {
     const unsigned t = T | (1u << bit);
-    const int cnt = __popcll(__ballot(u >= t));
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) cnt += __popcll(__ballot(u[i] >= t));
     if (cnt >= q) {
       T = t;
       if (cnt <= q + (q >> 1)) break;
@@ -153,16 +164,14 @@ __device__ __forceinline__ unsigned wave_kth(unsigned u, int q) {
 // the four waves' ceil(n / 4)-th best threads where every thread has values (they share a row: close to the n-th best), else the
 // best of the waves' n-th best threads, which threads without values do not spoil.  ru: 4 words of LDS, written here; the
 // caller's barrier follows, then block_bound reads them.
-template <int WAVES>
 __device__ __forceinline__ void wave_bounds(unsigned u, int n, bool full, unsigned* ru) {
-  const unsigned q = wave_kth(u, WAVES > 1 && (full || n > 64) ? (n + 3) / 4 : n);
+  const unsigned each[1] = {u}, q = wave_kth(each, full || n > 64 ? (n + 3) / 4 : n);
   if ((threadIdx.x & 63) == 0) ru[threadIdx.x >> 6] = q;
 }
-template <int WAVES>
 __device__ __forceinline__ unsigned block_bound(int n, bool full, const unsigned* ru) {
   unsigned lo = ru[0], hi = ru[0];
 #pragma unroll
-  for (int i = 1; i < WAVES; ++i) {
+  for (int i = 1; i < 4; ++i) {
     lo = ru[i] < lo ? ru[i] : lo;
     hi = ru[i] > hi ? ru[i] : hi;
   }
@@ -196,6 +205,47 @@ __device__ __forceinline__ void write_dead_slot(const SelectArgs& a, int b, int 
   a.out_scores[o] = -INFINITY;
   a.parent[o] = w;
   a.token[o] = f < 0 ? 0 : (f < a.V ? f : a.V - 1);
+}
+
+// Rank the `cnt` collected candidates and hand the n best to put(slot, key, place): each is compared with every other one, by 2, 4
+// or 8 neighbouring lanes where there are lanes enough, eight at a time (they are in LDS: one by one, each waits for its read).
+// lk and li have RANK_PAD places behind the candidates.
+constexpr int RANK_PAD = 64;
+template <int WAVES = 4, typename Put>
+__device__ __forceinline__ void rank_collected(long long* lk, const int* li, int cnt, int n, Put put) {
+  constexpr int T = 64 * WAVES;
+  if (threadIdx.x < RANK_PAD) lk[cnt + threadIdx.x] = KEY_NONE;
+  int lp = 0;
+  while (cnt > 32 && lp < 3 && cnt << (lp + 1) <= T) ++lp;
+  const int part = threadIdx.x & ((1 << lp) - 1), step = 1 << lp;
+  auto sum = [&](int v) {
+    if (lp > 0) v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false);    // lane ^ 1
+    if (lp > 1) v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false);    // lane ^ 2
+    if (lp > 2) v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, false);   // mirrored in 8 lanes
+    return v;
+  };
+  __syncthreads();
+  for (int e0 = 0; e0 < cnt; e0 += T >> lp) {
+    const int e = e0 + ((int)threadIdx.x >> lp);
+    const bool in = e < cnt;                 // the same in all lanes of an entry
+    if (!__any(in)) break;
+    const long long ke = lk[in ? e : 0];
+    const int ie = li[in ? e : 0];
+    int r = 0;
+    for (int q0 = 0; q0 < cnt; q0 += 8 * step) {
+      long long kq[8];
+      int iq[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        kq[i] = lk[q0 + i * step + part];
+        iq[i] = li[q0 + i * step + part];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r += better(kq[i], iq[i], ke, ie);
+    }
+    r = sum(r);
+    if (in && part == 0 && r < n) put(r, ke, ie);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -265,7 +315,7 @@ k_select_small(SelectArgs a, int g_log2) {
   // at least n candidates reach the bound that n lanes' best ones do, seldom many more
   int cnt = SMALL_CAP + 1;
   if (a.n <= 64) {
-    const unsigned T32 = wave_kth((unsigned)(best >> 32) ^ 0x80000000u, a.n);
+    const unsigned each[1] = {(unsigned)(best >> 32) ^ 0x80000000u}, T32 = wave_kth(each, a.n);
     const long long bound = T32 ? (long long)((unsigned long long)(T32 ^ 0x80000000u) << 32) : KEY_NONE + 1;
     cnt = 0;
 #pragma unroll
@@ -406,23 +456,10 @@ __device__ __forceinline__ unsigned block_kth(const unsigned (&u)[E], int q, uns
   return T;
 }
 
-// rank the `cnt` collected candidates and hand the n best to put(slot, key, place)
-template <int WAVES = 4, typename Put>
-__device__ __forceinline__ void rank_collected(const long long* lk, const int* li, int cnt, int n, Put put) {
-  for (int e = threadIdx.x; e < cnt; e += 64 * WAVES) {
-    const long long ke = lk[e];
-    const int ie = li[e];
-    int r = 0;
-#pragma unroll 8
-    for (int q = 0; q < cnt; ++q) r += better(lk[q], li[q], ke, ie);
-    if (r < n) put(r, ke, ie);
-  }
-}
-
 // Ranking compares every collected candidate with every other one.  Where the first bound let many through, the best of
 // those in the list give a closer one: collect(least) puts what is not below `least` into the list again, counting in rc.
 // Returns the list's length; more than CAP where too many are equal.  (256 x 60 beams x 1000 tokens, 60 kept: lists of 600 and
-// 1136 us before, 146 with this.)
+// 1136 us before, 146 with this, 95 with one wave a row.)
 template <int CAP, int WAVES, typename Collect>
 __device__ __forceinline__ int collect_fewer(int q, const long long* lk, int* rc, unsigned (*ct)[4], Collect collect) {
   constexpr int T = 64 * WAVES;
@@ -450,6 +487,7 @@ __device__ __forceinline__ int collect_fewer(int q, const long long* lk, int* rc
 }
 
 // best of the workgroup's (key, place) pairs; every thread gets it
+template <int WAVES = 4>
 __device__ __forceinline__ void block_best(long long& k, int& p, long long* sk, int* sp) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
@@ -463,7 +501,7 @@ __device__ __forceinline__ void block_best(long long& k, int& p, long long* sk, 
   k = sk[0];
   p = sp[0];
 #pragma unroll
-  for (int i = 1; i < 4; ++i)
+  for (int i = 1; i < WAVES; ++i)
     if (better(sk[i], sp[i], k, p)) { k = sk[i]; p = sp[i]; }
 }
 
@@ -474,8 +512,8 @@ __global__ void __launch_bounds__(256)
 k_select_group(SelectArgs a, int g_log2) {
   __shared__ unsigned ct[5][4];
   __shared__ int rc;
-  __shared__ long long lk[SEL_CAP];
-  __shared__ int li[SEL_CAP];
+  __shared__ long long lk[SEL_CAP + RANK_PAD];
+  __shared__ int li[SEL_CAP + RANK_PAD];
   const int b = blockIdx.x, tid = threadIdx.x, w = tid >> g_log2, j = tid & ((1 << g_log2) - 1);
   long long k[M];
   const unsigned best[1] = {(unsigned)(lane_candidates<T, M>(a, b, w, j, g_log2, k) >> 32) ^ 0x80000000u};   // 0: none
@@ -579,12 +617,12 @@ template <typename T, int U, bool BIAS, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, U > 8 ? 4 : 1)
 k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part, long long* __restrict__ pk,
                int* __restrict__ pi) {
-  constexpr int THREADS = 64 * WAVES, CAP = WAVES == 1 ? 64 * U : SEL_CAP;   // one wave's list holds its whole slice
+  constexpr int THREADS = 64 * WAVES, CAP = WAVES == 1 ? 512 : SEL_CAP;
   __shared__ double rd[2 * WAVES];
   __shared__ unsigned ru[4], ct[5][4];
   __shared__ int rc;
-  __shared__ long long lk[CAP];
-  __shared__ int li[CAP];
+  __shared__ long long lk[CAP + RANK_PAD];
+  __shared__ int li[CAP + RANK_PAD];
   typedef Logits<T, U, BIAS, THREADS> In;
   typedef typename In::X X;
   const int row = blockIdx.x / splits, split = blockIdx.x % splits;
@@ -608,14 +646,26 @@ k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part
     nan |= x[i] != x[i];
   }
   const bool full = base + THREADS * U <= a.V;
-  wave_bounds<WAVES>(Order<X>::bits(tmax, nan), depth, full, ru);
+  unsigned bound = 0;
+  if (WAVES == 1) {
+    unsigned u[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) u[i] = x[i] == -INFINITY ? 0u : Order<X>::bits(x[i], x[i] != x[i]);
+    bound = wave_kth(u, depth);
+  } else if (full || depth <= 16) {
+    wave_bounds(Order<X>::bits(tmax, nan), depth, full, ru);
+  } else {
+    const unsigned each[1] = {Order<X>::bits(tmax, nan)};
+    bound = block_kth<1>(each, depth, ct);
+  }
   double top = group_max((double)tmax, 64);
   if ((tid & 63) == 0) rd[wave] = top;
   if (tid == 0) rc = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < WAVES; ++i) top = fmax(top, rd[i]);
-  const X least = Order<X>::least(block_bound<WAVES>(depth, full, ru));
+  if (WAVES > 1 && (full || depth <= 16)) bound = block_bound(depth, full, ru);
+  const X least = Order<X>::least(bound);
   const double from = top == -INFINITY ? 0.0 : top;
   double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
@@ -662,7 +712,6 @@ k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part
     for (int r = cnt + tid; r < depth; r += THREADS) pk[mine + (long long)r * lists] = KEY_NONE;
     return;
   }
-  if (WAVES == 1) return;                  // not reached: the list holds the slice
   // more equal logits than the list holds: one after the other
   long long prev = KEY_NAN;
   int place = -1;
@@ -678,7 +727,7 @@ k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part
       const int q = In::place(base, i);
       if (ki != KEY_NONE && better(prev, place, ki, q) && better(ki, q, k, p)) { k = ki; p = q; }
     }
-    block_best(k, p, sk, sp);
+    block_best<WAVES>(k, p, sk, sp);
     if (tid == 0) {
       pk[mine + (long long)r * lists] = k;
       pi[mine + (long long)r * lists] = p;
@@ -754,10 +803,11 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
   __shared__ float sc[SEL_MAX_N];
   __shared__ int fc[SEL_MAX_N];
   __shared__ unsigned ct[5][4];
+  __shared__ int live[SEL_MAX_N];
   __shared__ int rc, above, reach;           // reach: the last entry collected
   __shared__ long long deep, kth;            // best of the lists' last entries; the last score kept
-  __shared__ long long lk[SEL_CAP];
-  __shared__ int li[SEL_CAP];
+  __shared__ long long lk[SEL_CAP + RANK_PAD];
+  __shared__ int li[SEL_CAP + RANK_PAD];
   const int b = blockIdx.x, tid = threadIdx.x;
   const int lists = a.W * splits, total = lists * depth;
   const long long* keys = pk + (long long)b * total;
@@ -774,8 +824,8 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
   const int g = 1 << g_log2, j = tid & (g - 1);
   for (int w0 = 0; w0 < a.W; w0 += 256 >> g_log2) {
     const int w = w0 + (tid >> g_log2);
-    const bool live = w < a.W;
-    const long long row = (long long)b * a.W + (live ? w : 0);
+    const bool in = w < a.W;
+    const long long row = (long long)b * a.W + (in ? w : 0);
     const long long f = a.forced ? a.forced[row] : -1;
     const float score = a.scores[row];
     double top = -INFINITY, sum = 0.0;
@@ -786,7 +836,7 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
     if (f < 0)
       for (int i = j; i < splits; i += g) sum += q[i].top == -INFINITY ? q[i].sum : q[i].sum * exp_neg(q[i].top - top);
     sum = group_sum(sum, g);
-    if (live && j == 0) {
+    if (in && j == 0) {
       lse[w] = top + log(sum);
       sc[w] = score;
       fc[w] = f < 0 ? -1 : (f < a.V ? (int)f : a.V - 1);
@@ -797,60 +847,83 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
     deep = kth = KEY_NONE;
   }
   __syncthreads();
-  // entry e (depth e / lists of list e % lists) with key kx and place px becomes a candidate
-  auto candidate = [&](int e, long long& kx, int& px) {
-    if (e >= total) {
-      kx = KEY_NONE;
-      return;
-    }
-    const int r = e / lists, l = e - r * lists, w = l / splits;
-    const bool head = r == 0 && l == w * splits;
-    if (fc[w] >= 0) {
-      kx = head && !(sc[w] == -INFINITY) ? key_of((double)sc[w]) : KEY_NONE;
-      px = w * a.V + fc[w];
-    } else if (broken((double)sc[w], lse[w])) {
-      kx = head ? KEY_NAN : KEY_NONE;
-      px = w * a.V;
-    } else if (kx != KEY_NONE) {
-      const double c = (double)sc[w] + (value_of(kx) - lse[w]);
-      kx = c == -INFINITY ? KEY_NONE : key_of(c);
-      px += w * a.V;
-    }
+  // beams whose lists count: not dead, no other candidate in place of the list's.  Where the registers do not hold all entries the
+  // other beams' are left out (at a search's first step one beam is alive): else live[w] = w, or -1.
+  const bool listed = tid < a.W && fc[tid] < 0 && !(sc[tid] == -INFINITY) && !broken((double)sc[tid], lse[tid]);
+  int in_use = lists;                        // lists
+  bool all = true;
+  if (total > 256 * E) {
+    const unsigned long long m = __ballot(listed);
+    if ((tid & 63) == 0) ct[0][tid >> 6] = __popcll(m);
+    __syncthreads();
+    int at = __popcll(m & ((1ull << (tid & 63)) - 1));
+    for (int i = 0; i < tid >> 6; ++i) at += ct[0][i];
+    if (listed) live[at] = tid;
+    in_use = (int)(ct[0][0] + ct[0][1] + ct[0][2] + ct[0][3]) * splits;
+    all = in_use == lists;
+  } else if (tid < a.W) {
+    live[tid] = listed ? tid : -1;
+  }
+  __syncthreads();
+  const int used = in_use * depth;           // entries
+  // entry e: depth e / in_use of list e % in_use, the candidate (kx, px)
+  auto fetch = [&](int e, bool load, long long& kx, int& px, int& w) {
+    const int r = e / in_use, l = e - r * in_use, i = l / splits;
+    w = live[i];
+    if (!load) return;
+    const int o = r * lists + w * splits + (l - i * splits);
+    kx = keys[o];
+    px = places[o];
+  };
+  auto candidate = [&](int w, long long& kx, int& px) {
+    if (w < 0) kx = KEY_NONE;
+    if (kx == KEY_NONE) return;
+    const double c = (double)sc[w] + (value_of(kx) - lse[w]);
+    kx = c == -INFINITY ? KEY_NONE : key_of(c);
+    px += w * a.V;
   };
   unsigned u[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) {
-    candidate(tid + 256 * i, k[i], p[i]);
+    const int e = tid + 256 * i;
+    int w = -1;
+    if (e < used) fetch(e, !all, k[i], p[i], w);
+    candidate(w, k[i], p[i]);
     u[i] = k[i] == KEY_NONE ? 0u : (unsigned)(k[i] >> 32) ^ 0x80000000u;
   }
   const unsigned first_bound = block_kth<E>(u, a.n, ct);
   auto take = [&](int e, long long kx, int px, unsigned bound) {
     if (kx == KEY_NONE || ((unsigned)(kx >> 32) ^ 0x80000000u) < bound) return;
-    if (e >= total - lists) atomicMax(&deep, kx);
-    if (total > 256 * E) atomicMax(&reach, e);
+    if (e >= used - in_use) atomicMax(&deep, kx);
+    if (used > 256 * E) atomicMax(&reach, e);
     const int q = atomicAdd(&rc, 1);
     if (q < SEL_CAP) { lk[q] = kx; li[q] = px; }
   };
-  // A list's entry counts only where the one before it, `lists` places earlier, does: entries beyond the registers are looked
+  auto alone = [&]() {                       // the one candidate of a forced or broken beam
+    if (fc[tid] < 0) return broken((double)sc[tid], lse[tid]) ? KEY_NAN : KEY_NONE;
+    return sc[tid] == -INFINITY ? KEY_NONE : key_of((double)sc[tid]);
+  };
+  // A list's entry counts only where the one before it, `in_use` places earlier, does: entries beyond the registers are looked
   // at while that may be, 256 E at a time.  (One thread walking down a list: 40 us where one beam of 60 has most of the best.)
   auto collect = [&](double, unsigned bound) {
 #pragma unroll
     for (int i = 0; i < E; ++i) take(tid + 256 * i, k[i], p[i], bound);
-    for (int base = 256 * E; base < total; base += 256 * E) {
+    if (tid < a.W && !listed) take(-1, alone(), tid * a.V + (fc[tid] < 0 ? 0 : fc[tid]), bound);
+    for (int base = 256 * E; base < used; base += 256 * E) {
       __syncthreads();
-      if (base > reach + lists) break;
+      if (base > reach + in_use) break;
       __syncthreads();
       long long kx[E];
-      int px[E];
+      int px[E], w[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const int e = base + tid + 256 * i;
-        kx[i] = keys[e < total ? e : 0];
-        px[i] = places[e < total ? e : 0];
+        fetch(e < used ? e : base, true, kx[i], px[i], w[i]);
+        if (e >= used) kx[i] = KEY_NONE;
       }
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        candidate(base + tid + 256 * i, kx[i], px[i]);
+        candidate(w[i], kx[i], px[i]);
         take(base + tid + 256 * i, kx[i], px[i], bound);
       }
     }
@@ -883,12 +956,17 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
     for (int r = 0; r < a.n; ++r) {
       long long kb = KEY_NONE;
       int pb = 0x7fffffff;
-      for (int e = tid; e < total; e += 256) {
-        long long ke = keys[e];
-        int pe = places[e];
-        candidate(e, ke, pe);
+      auto look = [&](long long ke, int pe) {
         if (ke != KEY_NONE && better(prev, place, ke, pe) && better(ke, pe, kb, pb)) { kb = ke; pb = pe; }
+      };
+      for (int e = tid; e < used; e += 256) {
+        long long ke;
+        int pe, w;
+        fetch(e, true, ke, pe, w);
+        candidate(w, ke, pe);
+        look(ke, pe);
       }
+      if (tid < a.W && !listed) look(alone(), tid * a.V + (fc[tid] < 0 ? 0 : fc[tid]));
       block_best(kb, pb, sk, sp);
       if (tid == 0) {
         if (kb != KEY_NONE) write_slot(a, b, r, kb, pb); else write_dead_slot(a, b, r);
@@ -905,9 +983,10 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
 inline int list_depth(int n) { return n < SEL_MAX_N ? n + 1 : SEL_MAX_N; }   // entries of a slice's list
 
 // How a call is split: one wave a group up to 8 candidates a lane (64 x 16 x 21), one workgroup of four waves up to 32 (three
-// beams or more, so that the waves have work), else slices and a second pass.  A slice is a row of up to 512 logits for one
-// wave, else 256 u logits for four: u = 32 where that gives every CU SEL_LONG workgroups, 8 below (32 x 8 x 131072 fp32: 58 us
-// with 32, 63 with 16).
+// beams or more, so that the waves have work), else slices and a second pass.  A slice is a row of up to 512 or 1024 logits for
+// one wave (250 x 16 x 700, 16 kept: 28 us, with four waves 33), else 256 u logits for four: u = 32 where rows hold two such
+// slices and there are 300 (512 rows of 31839 fp32: 33 us with 32, 44 with 8; 32 rows: 15.6 and 14.0; 2048 rows of 9000
+// bf16: 75 and 53).
 struct SelectPlan {
   int waves, g_log2, m;  // waves a group, 0 = slices; 2^g_log2 lanes a beam; candidates a lane
   int u, per, splits;    // slices: values a thread holds, waves a slice, slices a beam
@@ -925,8 +1004,9 @@ inline SelectPlan select_plan(long long B, int W, int V) {
       return p;
     }
   }
-  p.per = V <= 512 ? 1 : 4;
-  p.u = p.per == 1 || B * W * (V / (256 * SEL_U)) < SEL_LONG ? 8 : SEL_U;
+  p.per = V <= 1024 ? 1 : 4;
+  if (p.per == 1) p.u = V <= 512 ? 8 : 16;
+  else p.u = V >= 2 * 256 * SEL_U && B * W * (V / (256 * SEL_U)) >= SEL_LONG ? SEL_U : 8;
   p.splits = (V + 64 * p.per * p.u - 1) / (64 * p.per * p.u);
   return p;
 }
@@ -962,7 +1042,8 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
       hipLaunchKernelGGL((k_select_slice<T, U, false, WAVES>), grid, dim3(64 * WAVES), 0, st, a, p.splits, depth, part,  \
                          pk, pi);                                                                                        \
   } while (0)
-  if (p.per == 1) MPNN_SLICE(8, 1);
+  if (p.per == 1 && p.u == 8) MPNN_SLICE(8, 1);
+  else if (p.per == 1) MPNN_SLICE(16, 1);
   else if (p.u == 8) MPNN_SLICE(8, 4);
   else MPNN_SLICE(SEL_U, 4);
 #undef MPNN_SLICE
