@@ -29,7 +29,10 @@ constexpr int AW_BLOCK = 64;     // elements that share a scale: 16 lanes of fou
 constexpr int AW_PARTS = 256;    // workgroups (and partial sums) of the norm, over all launches of a call
 constexpr int NT_THREADS = 1024;
 constexpr int NT_CHUNK = 4 * NT_THREADS * 4;   // elements of a workgroup's turn in the norm
-constexpr int NT_MAX = 128;      // tensors of a launch of the norm
+constexpr int NT_MAX = 128;      // tensors of a launch of the norm, by pointers
+constexpr int NT_NEAR = 320;     // by distances
+constexpr int FEW = 16;          // tensors whose table is a launch's smallest: 3.1 us a launch with 640 bytes of arguments, 2.7 with
+                                 // 64, 4.1-4.9 with 1.5 to 4 KB
 
 // A tensor's six addresses as distances from those of the first tensor of its kind, in units of four bytes: 32 bytes a
 // tensor, where pointers take 56 and two launches for the model's 118 tensors.  A tensor that lies 8 GB away from the first
@@ -37,20 +40,35 @@ constexpr int NT_MAX = 128;      // tensors of a launch of the norm
 struct Origin {
   char *p, *g, *m, *v, *ms, *vs;
 };
+template <int N>
 struct AdamTable {
+  static constexpr int MAX = N;
   Origin origin[2];              // of 32-bit moments, of 8-bit ones
-  int p[AW_MAX], g[AW_MAX], m[AW_MAX], v[AW_MAX], ms[AW_MAX], vs[AW_MAX];   // ms: NO_SCALE for 32-bit moments
-  unsigned numel[AW_MAX];
-  int chunk0[AW_MAX + 1];        // first chunk of each tensor
+  int p[N], g[N], m[N], v[N], ms[N], vs[N];   // ms: NO_SCALE for 32-bit moments
+  unsigned numel[N];
+  int chunk0[N + 1];             // first chunk of each tensor
   int n;
 };
 constexpr int NO_SCALE = (int)0x80000000;
 
-struct NormTable {
-  const float* g[NT_MAX];
-  long long numel[NT_MAX];
+// the norm's: distances in units of four bytes from the first, as above, or pointers where those do not reach
+template <int N>
+struct NearTable {
+  static constexpr int MAX = N;
+  const float* origin;
+  int at[N];
+  unsigned numel[N];
+  int chunk0[N + 1];
+  int n;
+  __device__ const float* grad(int i) const { return origin + at[i]; }
+};
+struct FarTable {
+  static constexpr int MAX = NT_MAX;
+  const float* at[NT_MAX];
+  unsigned numel[NT_MAX];
   int chunk0[NT_MAX + 1];
   int n;
+  __device__ const float* grad(int i) const { return at[i]; }
 };
 
 struct AdamHyper {
@@ -97,13 +115,14 @@ __device__ __forceinline__ double block_sum(double s, double* sh) {
   return s;
 }
 
+template <typename Table>
 __global__ void __launch_bounds__(NT_THREADS)
-k_grad_sumsq_parts(NormTable t, double* __restrict__ parts) {
+k_grad_sumsq_parts(Table t, double* __restrict__ parts) {
   __shared__ double sh[NT_THREADS / 64];
   double s = 0.0;
   for (int chunk = blockIdx.x; chunk < t.chunk0[t.n]; chunk += gridDim.x) {
     const int ti = tensor_of(t, chunk);
-    const float* __restrict__ g = t.g[ti];
+    const float* __restrict__ g = t.grad(ti);
     const long long n = t.numel[ti], i = (long long)(chunk - t.chunk0[ti]) * NT_CHUNK + threadIdx.x * 4;
     constexpr int ROW = 4 * NT_THREADS;
     if (((uintptr_t)g & 15) == 0 && i + NT_CHUNK - ROW + 4 <= n) {   // this thread's last four included
@@ -199,7 +218,8 @@ struct Four {
   f32x4 pv, gv, mv, vv;          // 8-bit moments: four codes in mv[0], vv[0], the scale in mv[1], vv[1]
 };
 
-__device__ __forceinline__ void load_four(const AdamTable& t, const AdamHyper& h, int chunk, Four& c) {
+template <typename Table>
+__device__ __forceinline__ void load_four(const Table& t, const AdamHyper& h, int chunk, Four& c) {
   const int ti = tensor_of(t, chunk);
   const long long n = t.numel[ti], i = (long long)(chunk - t.chunk0[ti]) * AW_CHUNK + threadIdx.x * 4;
   const bool eight = t.ms[ti] != NO_SCALE;
@@ -337,8 +357,9 @@ __device__ __forceinline__ void finish_four(const AdamHyper& h, double coef, Fou
   }
 }
 
+template <typename Table>
 __global__ void __launch_bounds__(256)
-k_adamw_mixed(AdamTable t, AdamHyper h) {
+k_adamw_mixed(Table t, AdamHyper h) {
   __shared__ double sh[4];
   const int total = t.chunk0[t.n];
   int chunk = blockIdx.x;
@@ -363,26 +384,46 @@ k_adamw_mixed(AdamTable t, AdamHyper h) {
 
 }  // namespace
 
-extern "C" int mpnn_grad_sumsq_parts(int n, const float* const* grads, const long long* numel, double* parts, void* stream) {
-  MPNN_CHECK_ARG(n > 0 && n <= AW_PARTS * NT_MAX && grads && numel && parts, "mpnn_grad_sumsq_parts: bad arguments");
-  for (int j = 0; j < n; ++j)
-    MPNN_CHECK_ARG(grads[j] && numel[j] > 0 && numel[j] < (1LL << 32), "mpnn_grad_sumsq_parts: null, empty or oversized tensor");
-  const int launches = (n + NT_MAX - 1) / NT_MAX, share = AW_PARTS / launches;
+static void place(FarTable& t, int j, const float* const* grads, int k0) { t.at[j] = grads[k0 + j]; }
+template <int N>
+static void place(NearTable<N>& t, int j, const float* const* grads, int k0) {
+  t.origin = grads[0];
+  t.at[j] = (int)(grads[k0 + j] - grads[0]);
+}
+
+template <typename Table>
+static void launch_parts(int n, const float* const* grads, const long long* numel, double* parts, hipStream_t st) {
+  const int launches = (n + Table::MAX - 1) / Table::MAX, share = AW_PARTS / launches;
   for (int l = 0; l < launches; ++l) {
-    NormTable t;
-    const int k0 = l * NT_MAX;
-    t.n = n - k0 < NT_MAX ? n - k0 : NT_MAX;
-    long long chunks = 0;                            // at most 128 * 2^18
+    Table t;
+    const int k0 = l * Table::MAX;
+    t.n = n - k0 < Table::MAX ? n - k0 : Table::MAX;
+    long long chunks = 0;                            // at most 320 * 2^18
     for (int j = 0; j < t.n; ++j) {
-      t.g[j] = grads[k0 + j];
-      t.numel[j] = numel[k0 + j];
+      place(t, j, grads, k0);
+      t.numel[j] = (unsigned)numel[k0 + j];
       t.chunk0[j] = (int)chunks;
       chunks += (numel[k0 + j] + NT_CHUNK - 1) / NT_CHUNK;
     }
     t.chunk0[t.n] = (int)chunks;
     const int wgs = l + 1 < launches ? share : AW_PARTS - share * (launches - 1);   // every part is written
-    hipLaunchKernelGGL(k_grad_sumsq_parts, dim3(wgs), dim3(NT_THREADS), 0, (hipStream_t)stream, t, parts + (long long)share * l);
+    hipLaunchKernelGGL((k_grad_sumsq_parts<Table>), dim3(wgs), dim3(NT_THREADS), 0, st, t, parts + (long long)share * l);
   }
+}
+
+extern "C" int mpnn_grad_sumsq_parts(int n, const float* const* grads, const long long* numel, double* parts, void* stream) {
+  MPNN_CHECK_ARG(n > 0 && n <= AW_PARTS * NT_MAX && grads && numel && parts, "mpnn_grad_sumsq_parts: bad arguments");
+  bool near = true;
+  for (int j = 0; j < n; ++j) {
+    MPNN_CHECK_ARG(grads[j] && ((uintptr_t)grads[j] & 3) == 0 && numel[j] > 0 && numel[j] < (1LL << 32),
+                   "mpnn_grad_sumsq_parts: null, misaligned, empty or oversized tensor");
+    const long long d = ((const char*)grads[j] - (const char*)grads[0]) / 4;
+    near &= d > -(1LL << 31) && d < (1LL << 31);
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (!near) launch_parts<FarTable>(n, grads, numel, parts, st);
+  else if (n <= FEW) launch_parts<NearTable<FEW>>(n, grads, numel, parts, st);
+  else launch_parts<NearTable<NT_NEAR>>(n, grads, numel, parts, st);
   MPNN_LAUNCH_CHECK();
 }
 
@@ -391,6 +432,51 @@ static bool offset(const void* x, const char* origin, int& out) {
   const long long d = (const char*)x - origin;
   out = (int)(d / 4);
   return d % 4 == 0 && d / 4 > -(1LL << 31) && d / 4 < (1LL << 31);
+}
+
+struct AdamLists {
+  int n, first;
+  float* const* params;
+  const float* const* grads;
+  void* const* exp_avg;
+  void* const* exp_avg_sq;
+  float* const* exp_avg_scale;
+  float* const* exp_avg_sq_scale;
+  const long long* numel;
+};
+
+template <typename Table>
+static void launch_adamw(const AdamLists& q, AdamHyper h, hipStream_t st) {
+  for (int k0 = 0; k0 < q.n;) {
+    Table t;
+    t.origin[0] = t.origin[1] = Origin{};
+    long long chunks = 0;
+    int j = 0;
+    for (; j < Table::MAX && k0 + j < q.n; ++j) {
+      const int k = k0 + j;
+      const bool eight = q.exp_avg_scale[k] != nullptr;
+      Origin& o = t.origin[eight];
+      if (!o.p)
+        o = Origin{(char*)q.params[k], (char*)q.grads[k], (char*)q.exp_avg[k], (char*)q.exp_avg_sq[k], (char*)q.exp_avg_scale[k],
+                   (char*)q.exp_avg_sq_scale[k]};
+      const long long more = (q.numel[k] + AW_CHUNK - 1) / AW_CHUNK;
+      t.ms[j] = t.vs[j] = NO_SCALE;
+      if (!offset(q.params[k], o.p, t.p[j]) || !offset(q.grads[k], o.g, t.g[j]) || !offset(q.exp_avg[k], o.m, t.m[j]) ||
+          !offset(q.exp_avg_sq[k], o.v, t.v[j]) ||
+          (eight && (!offset(q.exp_avg_scale[k], o.ms, t.ms[j]) || !offset(q.exp_avg_sq_scale[k], o.vs, t.vs[j]))) ||
+          chunks + more >= (1LL << 31) - 65536)
+        break;                                       // never the first: it is an origin
+      t.numel[j] = (unsigned)q.numel[k];
+      t.chunk0[j] = (int)chunks;
+      chunks += more;
+    }
+    t.n = j;
+    t.chunk0[j] = (int)chunks;
+    h.tensor0 = (unsigned)(q.first + k0);
+    hipLaunchKernelGGL((k_adamw_mixed<Table>), dim3((unsigned)(chunks < AW_WGS ? chunks : AW_WGS)), dim3(256), 0, st, t, h);
+    h.sumsq = nullptr;
+    k0 += j;
+  }
 }
 
 extern "C" int mpnn_adamw_mixed(int n, float* const* params, const float* const* grads, void* const* exp_avg,
@@ -424,35 +510,8 @@ extern "C" int mpnn_adamw_mixed(int n, float* const* params, const float* const*
   h.parts = max_norm > 0 ? sumsq_parts : nullptr;
   h.key = hash_bits((unsigned)step, seed);
   h.sumsq = grad_sumsq;
-  for (int k0 = 0; k0 < n;) {
-    AdamTable t;
-    t.origin[0] = t.origin[1] = Origin{};
-    long long chunks = 0;
-    int j = 0;
-    for (; j < AW_MAX && k0 + j < n; ++j) {
-      const int k = k0 + j;
-      const bool eight = exp_avg_scale[k] != nullptr;
-      Origin& o = t.origin[eight];
-      if (!o.p)
-        o = Origin{(char*)params[k], (char*)grads[k], (char*)exp_avg[k], (char*)exp_avg_sq[k], (char*)exp_avg_scale[k],
-                   (char*)exp_avg_sq_scale[k]};
-      const long long more = (numel[k] + AW_CHUNK - 1) / AW_CHUNK;
-      t.ms[j] = t.vs[j] = NO_SCALE;
-      if (!offset(params[k], o.p, t.p[j]) || !offset(grads[k], o.g, t.g[j]) || !offset(exp_avg[k], o.m, t.m[j]) ||
-          !offset(exp_avg_sq[k], o.v, t.v[j]) ||
-          (eight && (!offset(exp_avg_scale[k], o.ms, t.ms[j]) || !offset(exp_avg_sq_scale[k], o.vs, t.vs[j]))) ||
-          chunks + more >= (1LL << 31) - 65536)
-        break;                                       // never the first: it is an origin
-      t.numel[j] = (unsigned)numel[k];
-      t.chunk0[j] = (int)chunks;
-      chunks += more;
-    }
-    t.n = j;
-    t.chunk0[j] = (int)chunks;
-    h.tensor0 = (unsigned)(first + k0);
-    hipLaunchKernelGGL(k_adamw_mixed, dim3((unsigned)(chunks < AW_WGS ? chunks : AW_WGS)), dim3(256), 0, (hipStream_t)stream, t, h);
-    h.sumsq = nullptr;
-    k0 += j;
-  }
+  const AdamLists lists = {n, first, params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, numel};
+  if (n <= FEW) launch_adamw<AdamTable<FEW>>(lists, h, (hipStream_t)stream);
+  else launch_adamw<AdamTable<AW_MAX>>(lists, h, (hipStream_t)stream);
   MPNN_LAUNCH_CHECK();
 }
