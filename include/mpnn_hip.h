@@ -765,7 +765,7 @@ int mpnn_mask_self(const int64_t* chain_encoding_all, int B, int L, float* mask_
  * A slot that no candidate is left for gets the score -inf and keeps its beam: parent = slot % n_beams, token = that
  * beam's forced token or 0.  A beam with NaN or +inf among its logits that are not out, or in its score, offers one
  * candidate: token 0, score NaN, ranked first.  Outputs are fully determined by the inputs (no atomics decide anything).
- * n_beams, n_out <= 256, n_tokens <= 2^22, n_groups < 2^24 (and n_groups * n_beams slices of long rows: refused where they
+ * n_beams, n_out <= 256, n_tokens <= 2^22, n_groups < 2^22 (and n_groups * n_beams slices of long rows: refused where they
  * do not fit one launch).  workspace: mpnn_beam_select_workspace bytes (0: none needed), 16-byte
  * aligned, overwritten; calls that may overlap need one each.  The outputs may not overlap the inputs. */
 int mpnn_beam_select(const void* logits, int dtype, long long stride_group, long long stride_beam, const float* scores,

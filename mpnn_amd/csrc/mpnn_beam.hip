@@ -408,7 +408,7 @@ struct SlicePart {
 
 // some T that at least q of the workgroup's values u reach, and seldom a quarter more; 0 if fewer than q are above 0
 template <int E, int WAVES = 4>
-__device__ __forceinline__ unsigned block_kth(const unsigned (&u)[E], int q, unsigned (*cnt)[4]) {
+__device__ __forceinline__ unsigned block_kth(const unsigned (&u)[E], int q, unsigned (*cnt)[WAVES]) {
   unsigned largest = 0, least = 0xffffffffu;
   int some = 0;
 #pragma unroll
@@ -461,7 +461,7 @@ __device__ __forceinline__ unsigned block_kth(const unsigned (&u)[E], int q, uns
 // Returns the list's length; more than CAP where too many are equal.  (256 x 60 beams x 1000 tokens, 60 kept: lists of 600 and
 // 1136 us before, 146 with this, 95 with one wave a row.)
 template <int CAP, int WAVES, typename Collect>
-__device__ __forceinline__ int collect_fewer(int q, const long long* lk, int* rc, unsigned (*ct)[4], Collect collect) {
+__device__ __forceinline__ int collect_fewer(int q, const long long* lk, int* rc, unsigned (*ct)[WAVES], Collect collect) {
   constexpr int T = 64 * WAVES;
   unsigned last = 0;
   int cnt = *rc;
@@ -505,12 +505,13 @@ __device__ __forceinline__ void block_best(long long& k, int& p, long long* sk, 
     if (better(sk[i], sp[i], k, p)) { k = sk[i]; p = sp[i]; }
 }
 
-// Middling groups: four waves hold a group's candidates in registers, as one wave does for small ones, and rank those that
-// reach the bound in LDS.  64 beams x 21 letters, 64 kept: 6.2 us, where one wave took 16-21.
-template <typename T, int M>
-__global__ void __launch_bounds__(256)
+// Middling groups: 4 to 16 waves hold a group's candidates in registers, as one wave does for small ones, and rank those that
+// reach the bound in LDS.  64 beams x 21 letters, 64 kept: 6.2 us with 4, where one wave took 16-21; 21 x 9 x 468, 18 kept: 13
+// us with 16, 18 with 4; 205 x 61 x 131, 64 kept: 20 us, as slices 69.
+template <typename T, int M, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
 k_select_group(SelectArgs a, int g_log2) {
-  __shared__ unsigned ct[5][4];
+  __shared__ unsigned ct[5][WAVES];
   __shared__ int rc;
   __shared__ long long lk[SEL_CAP + RANK_PAD];
   __shared__ int li[SEL_CAP + RANK_PAD];
@@ -518,7 +519,7 @@ k_select_group(SelectArgs a, int g_log2) {
   long long k[M];
   const unsigned best[1] = {(unsigned)(lane_candidates<T, M>(a, b, w, j, g_log2, k) >> 32) ^ 0x80000000u};   // 0: none
   if (tid == 0) rc = 0;
-  const unsigned first = block_kth<1>(best, a.n, ct);   // the n-th best thread, or 0
+  const unsigned first = block_kth<1, WAVES>(best, a.n, ct);   // the n-th best thread, or 0
   auto collect = [&](double, unsigned bound) {
 #pragma unroll
     for (int i = 0; i < M; ++i) {
@@ -533,17 +534,17 @@ k_select_group(SelectArgs a, int g_log2) {
   };
   collect(0.0, first);
   __syncthreads();
-  const int cnt = collect_fewer<SEL_CAP, 4>(a.n, lk, &rc, ct, collect);
+  const int cnt = collect_fewer<SEL_CAP, WAVES>(a.n, lk, &rc, ct, collect);
   if (cnt <= SEL_CAP) {
-    rank_collected(lk, li, cnt, a.n, [&](int r, long long ke, int pe) { write_slot(a, b, r, ke, pe); });
-    for (int r = cnt + tid; r < a.n; r += 256) write_dead_slot(a, b, r);
+    rank_collected<WAVES>(lk, li, cnt, a.n, [&](int r, long long ke, int pe) { write_slot(a, b, r, ke, pe); });
+    for (int r = cnt + tid; r < a.n; r += 64 * WAVES) write_dead_slot(a, b, r);
     return;
   }
   // more ties than the list holds: one after the other
   long long prev = KEY_NAN;
   int place = -1;
-  __shared__ long long sk[4];
-  __shared__ int sp[4];
+  __shared__ long long sk[WAVES];
+  __shared__ int sp[WAVES];
   for (int r = 0; r < a.n; ++r) {
     long long kb = KEY_NONE;
     int pb = 0x7fffffff;
@@ -552,7 +553,7 @@ k_select_group(SelectArgs a, int g_log2) {
       const int pe = w * a.V + j + (i << g_log2);
       if (k[i] != KEY_NONE && better(prev, place, k[i], pe) && better(k[i], pe, kb, pb)) { kb = k[i]; pb = pe; }
     }
-    block_best(kb, pb, sk, sp);
+    block_best<WAVES>(kb, pb, sk, sp);
     if (tid == 0) {
       if (kb != KEY_NONE) write_slot(a, b, r, kb, pb); else write_dead_slot(a, b, r);
     }
@@ -619,7 +620,7 @@ k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part
                int* __restrict__ pi) {
   constexpr int THREADS = 64 * WAVES, CAP = WAVES == 1 ? 512 : SEL_CAP;
   __shared__ double rd[2 * WAVES];
-  __shared__ unsigned ru[4], ct[5][4];
+  __shared__ unsigned ru[4], ct[5][WAVES];
   __shared__ int rc;
   __shared__ long long lk[CAP + RANK_PAD];
   __shared__ int li[CAP + RANK_PAD];
@@ -982,22 +983,22 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
 
 inline int list_depth(int n) { return n < SEL_MAX_N ? n + 1 : SEL_MAX_N; }   // entries of a slice's list
 
-// How a call is split: one wave a group up to 8 candidates a lane (64 x 16 x 21), one workgroup of four waves up to 32 (three
-// beams or more, so that the waves have work), else slices and a second pass.  A slice is a row of up to 512 or 1024 logits for
-// one wave (250 x 16 x 700, 16 kept: 28 us, with four waves 33), else 256 u logits for four: u = 32 where rows hold two such
-// slices and there are 300 (512 rows of 31839 fp32: 33 us with 32, 44 with 8; 32 rows: 15.6 and 14.0; 2048 rows of 9000
-// bf16: 75 and 53).
+// How a call is split: one wave a group up to 8 candidates a lane (64 x 16 x 21); a beam's lanes are at most a wave, so three or
+// four beams take one workgroup of four waves up to 32 a lane, more of them four waves up to 8, else 8 or (more than four, more than
+// eight beams) 16 waves up to 16 (8 x 6 x 882: 12 us with 8 waves, 15 with 16, 14 with 4); else slices and a second pass.  A slice is a row of up to 512 or 1024 logits for one wave (250 x 16 x 700, 16 kept: 28 us, with four waves
+// 33), else 256 u logits for four: u = 32 where rows hold two such slices and there are 300 (512 rows of 31839 fp32: 33 us with
+// 32, 44 with 8; 32 rows: 15.6 and 14.0; 2048 rows of 9000 bf16: 75 and 53).
 struct SelectPlan {
   int waves, g_log2, m;  // waves a group, 0 = slices; 2^g_log2 lanes a beam; candidates a lane
   int u, per, splits;    // slices: values a thread holds, waves a slice, slices a beam
 };
 inline SelectPlan select_plan(long long B, int W, int V) {
   SelectPlan p = {};
-  for (int waves = 1; waves <= 4; waves += 3) {
+  for (int waves : {1, 4, 8, 16}) {
     int gl = 6;
     while (gl > 0 && ((64 * waves) >> gl) < W) --gl;
-    const int m = (V + (1 << gl) - 1) >> gl;
-    if (((64 * waves) >> gl) >= W && m <= (waves == 1 ? 8 : W > 2 ? 32 : 0)) {
+    const int m = (V + (1 << gl) - 1) >> gl, most = waves == 1 ? 8 : waves == 4 ? (W <= 2 ? 0 : W <= 4 ? 32 : 8) : W <= waves / 2 ? 0 : 16;
+    if (((64 * waves) >> gl) >= W && m <= most) {
       p.waves = waves;
       p.g_log2 = gl;
       p.m = m;
@@ -1020,11 +1021,15 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
     else hipLaunchKernelGGL((k_select_small<T, 8>), grid, block, 0, st, a, p.g_log2);
     MPNN_LAUNCH_CHECK();
   }
-  if (p.waves == 4) {
-    const dim3 grid(a.B), block(256);
-    if (p.m <= 8) hipLaunchKernelGGL((k_select_group<T, 8>), grid, block, 0, st, a, p.g_log2);
-    else if (p.m <= 16) hipLaunchKernelGGL((k_select_group<T, 16>), grid, block, 0, st, a, p.g_log2);
-    else hipLaunchKernelGGL((k_select_group<T, 32>), grid, block, 0, st, a, p.g_log2);
+  if (p.waves) {
+    const dim3 grid(a.B), block(64 * p.waves);
+    if (p.waves == 16 && p.m <= 8) hipLaunchKernelGGL((k_select_group<T, 8, 16>), grid, block, 0, st, a, p.g_log2);
+    else if (p.waves == 8 && p.m <= 8) hipLaunchKernelGGL((k_select_group<T, 8, 8>), grid, block, 0, st, a, p.g_log2);
+    else if (p.waves == 8) hipLaunchKernelGGL((k_select_group<T, 16, 8>), grid, block, 0, st, a, p.g_log2);
+    else if (p.waves == 16) hipLaunchKernelGGL((k_select_group<T, 16, 16>), grid, block, 0, st, a, p.g_log2);
+    else if (p.m <= 8) hipLaunchKernelGGL((k_select_group<T, 8, 4>), grid, block, 0, st, a, p.g_log2);
+    else if (p.m <= 16) hipLaunchKernelGGL((k_select_group<T, 16, 4>), grid, block, 0, st, a, p.g_log2);
+    else hipLaunchKernelGGL((k_select_group<T, 32, 4>), grid, block, 0, st, a, p.g_log2);
     MPNN_LAUNCH_CHECK();
   }
   const long long parts = (long long)a.B * a.W * p.splits;
@@ -1326,7 +1331,7 @@ extern "C" int mpnn_beam_select(const void* logits, int dtype, long long stride_
                  "mpnn_beam_select: workspace missing, too small (mpnn_beam_select_workspace) or not 16-byte aligned");
   const SelectPlan p = select_plan(n_groups, n_beams, n_tokens);
   // a launch has less than 2^32 threads; entries of a group's lists are counted in 32 bits
-  MPNN_CHECK_ARG((long long)n_groups < (1LL << 32) / (p.waves == 1 ? 64 : 256) &&
+  MPNN_CHECK_ARG((long long)n_groups < (1LL << 32) / (p.waves ? 64 * p.waves : 256) &&
                      (p.waves || (long long)n_groups * n_beams * p.splits < (1LL << 24)) &&
                      (long long)n_beams * (p.waves ? 1 : p.splits) * list_depth(n_out) < (1LL << 31),
                  "mpnn_beam_select: too many groups for one launch");
