@@ -805,7 +805,8 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
   __shared__ int fc[SEL_MAX_N];
   __shared__ unsigned ct[5][4];
   __shared__ int live[SEL_MAX_N];
-  __shared__ int rc, above, reach;           // reach: the last entry collected
+  __shared__ short open[256 * E];            // lists that go on beyond the registers
+  __shared__ int rc, above, n_open, reach;   // reach: the last entry collected there
   __shared__ long long deep, kth;            // best of the lists' last entries; the last score kept
   __shared__ long long lk[SEL_CAP + RANK_PAD];
   __shared__ int li[SEL_CAP + RANK_PAD];
@@ -844,7 +845,8 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
     }
   }
   if (tid == 0) {
-    rc = above = reach = 0;
+    rc = above = n_open = 0;
+    reach = -1;
     deep = kth = KEY_NONE;
   }
   __syncthreads();
@@ -867,9 +869,9 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
   }
   __syncthreads();
   const int used = in_use * depth;           // entries
-  // entry e: depth e / in_use of list e % in_use, the candidate (kx, px)
-  auto fetch = [&](int e, bool load, long long& kx, int& px, int& w) {
-    const int r = e / in_use, l = e - r * in_use, i = l / splits;
+  // the entry at depth r of list l; e = r in_use + l
+  auto fetch = [&](int r, int l, bool load, long long& kx, int& px, int& w) {
+    const int i = l / splits;
     w = live[i];
     if (!load) return;
     const int o = r * lists + w * splits + (l - i * splits);
@@ -888,15 +890,29 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
   for (int i = 0; i < E; ++i) {
     const int e = tid + 256 * i;
     int w = -1;
-    if (e < used) fetch(e, !all, k[i], p[i], w);
+    if (e < used) fetch(e / in_use, e % in_use, !all, k[i], p[i], w);
     candidate(w, k[i], p[i]);
     u[i] = k[i] == KEY_NONE ? 0u : (unsigned)(k[i] >> 32) ^ 0x80000000u;
   }
   const unsigned first_bound = block_kth<E>(u, a.n, ct);
-  auto take = [&](int e, long long kx, int px, unsigned bound) {
+  // Entries beyond the registers: of the lists whose entry in the registers' last whole row reaches the bound (of all lists, if
+  // there is no whole row), row by row as far as one of them does.  (One thread walking down a list: 40 us where one beam of 60
+  // has most of the best; all lists row by row: 50 us for 16 x 64 x 20000, 64 kept.)
+  const int rows = used > 256 * E ? 256 * E / in_use : 0;
+  if (rows) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int e = tid + 256 * i - (rows - 1) * in_use;
+      if (e >= 0 && e < in_use && u[i] && u[i] >= first_bound) open[atomicAdd(&n_open, 1)] = (short)e;
+    }
+    __syncthreads();
+  }
+  const int wide = rows ? n_open : in_use, more = used > 256 * E ? wide * (depth - rows) : 0;
+  // e: place among the entries beyond the registers, -1 for others
+  auto take = [&](int e, bool at_end, long long kx, int px, unsigned bound) {
     if (kx == KEY_NONE || ((unsigned)(kx >> 32) ^ 0x80000000u) < bound) return;
-    if (e >= used - in_use) atomicMax(&deep, kx);
-    if (used > 256 * E) atomicMax(&reach, e);
+    if (at_end) atomicMax(&deep, kx);
+    if (e >= 0) atomicMax(&reach, e);
     const int q = atomicAdd(&rc, 1);
     if (q < SEL_CAP) { lk[q] = kx; li[q] = px; }
   };
@@ -904,28 +920,31 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
     if (fc[tid] < 0) return broken((double)sc[tid], lse[tid]) ? KEY_NAN : KEY_NONE;
     return sc[tid] == -INFINITY ? KEY_NONE : key_of((double)sc[tid]);
   };
-  // A list's entry counts only where the one before it, `in_use` places earlier, does: entries beyond the registers are looked
-  // at while that may be, 256 E at a time.  (One thread walking down a list: 40 us where one beam of 60 has most of the best.)
   auto collect = [&](double, unsigned bound) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) take(tid + 256 * i, k[i], p[i], bound);
-    if (tid < a.W && !listed) take(-1, alone(), tid * a.V + (fc[tid] < 0 ? 0 : fc[tid]), bound);
-    for (int base = 256 * E; base < used; base += 256 * E) {
+    for (int i = 0; i < E; ++i) take(-1, tid + 256 * i >= used - in_use, k[i], p[i], bound);
+    if (tid < a.W && !listed) take(-1, false, alone(), tid * a.V + (fc[tid] < 0 ? 0 : fc[tid]), bound);
+    for (int base = 0; base < more; base += 256 * E) {
       __syncthreads();
-      if (base > reach + in_use) break;
+      if (base > reach + wide) break;
       __syncthreads();
       long long kx[E];
-      int px[E], w[E];
+      int px[E], w[E], r[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const int e = base + tid + 256 * i;
-        fetch(e < used ? e : base, true, kx[i], px[i], w[i]);
-        if (e >= used) kx[i] = KEY_NONE;
+        const int e = base + tid + 256 * i < more ? base + tid + 256 * i : base, l = rows ? open[e % wide] : e % wide;
+        r[i] = rows + e / wide;
+        fetch(r[i], l, true, kx[i], px[i], w[i]);
+        if (base + tid + 256 * i >= more) kx[i] = KEY_NONE;
+        else if (r[i] * in_use + l < 256 * E) {      // is in the registers
+          kx[i] = KEY_NONE;
+          atomicMax(&reach, e);
+        }
       }
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         candidate(w[i], kx[i], px[i]);
-        take(base + tid + 256 * i, kx[i], px[i], bound);
+        take(base + tid + 256 * i, r[i] == depth - 1, kx[i], px[i], bound);
       }
     }
   };
@@ -963,7 +982,7 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
       for (int e = tid; e < used; e += 256) {
         long long ke;
         int pe, w;
-        fetch(e, true, ke, pe, w);
+        fetch(e / in_use, e % in_use, true, ke, pe, w);
         candidate(w, ke, pe);
         look(ke, pe);
       }
