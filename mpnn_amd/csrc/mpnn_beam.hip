@@ -154,7 +154,7 @@ __device__ __forceinline__ unsigned wave_kth(const unsigned (&u)[E], int q) {
     for (int i = 0; i < E; ++i) cnt += __popcll(__ballot(u[i] >= t));
     if (cnt >= q) {
       T = t;
-      if (cnt <= q + (q >> 1)) break;
+      if (cnt <= (E > 1 && q > 42 ? (q <= 64 ? 64 : q + (q >> 2)) : q + (q >> 1))) break;   // 64 are ranked in one turn
     }
   }
   return T;
@@ -216,8 +216,6 @@ __device__ __forceinline__ void rank_collected(long long* lk, const int* li, int
   constexpr int T = 64 * WAVES;
   if (threadIdx.x < RANK_PAD) lk[cnt + threadIdx.x] = KEY_NONE;
   int lp = 0;
-  while (cnt > 32 && lp < 3 && cnt << (lp + 1) <= T) ++lp;
-  const int part = threadIdx.x & ((1 << lp) - 1), step = 1 << lp;
   auto sum = [&](int v) {
     if (lp > 0) v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, false);    // lane ^ 1
     if (lp > 1) v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, false);    // lane ^ 2
@@ -226,6 +224,9 @@ __device__ __forceinline__ void rank_collected(long long* lk, const int* li, int
   };
   __syncthreads();
   for (int e0 = 0; e0 < cnt; e0 += T >> lp) {
+    lp = 0;
+    while (cnt > 32 && lp < 3 && (cnt - e0) << (lp + 1) <= T) ++lp;
+    const int part = threadIdx.x & ((1 << lp) - 1), step = 1 << lp;
     const int e = e0 + ((int)threadIdx.x >> lp);
     const bool in = e < cnt;                 // the same in all lanes of an entry
     if (!__any(in)) break;
@@ -459,7 +460,7 @@ __device__ __forceinline__ unsigned block_kth(const unsigned (&u)[E], int q, uns
 // Ranking compares every collected candidate with every other one.  Where the first bound let many through, the best of
 // those in the list give a closer one: collect(least) puts what is not below `least` into the list again, counting in rc.
 // Returns the list's length; more than CAP where too many are equal.  (256 x 60 beams x 1000 tokens, 60 kept: lists of 600 and
-// 1136 us before, 146 with this, 95 with one wave a row.)
+// 1136 us before; 82 with one wave a row.)
 template <int CAP, int WAVES, typename Collect>
 __device__ __forceinline__ int collect_fewer(int q, const long long* lk, int* rc, unsigned (*ct)[WAVES], Collect collect) {
   constexpr int T = 64 * WAVES;
@@ -1002,11 +1003,12 @@ k_select_merge(SelectArgs a, int splits, int depth, int g_log2, const SlicePart*
 
 inline int list_depth(int n) { return n < SEL_MAX_N ? n + 1 : SEL_MAX_N; }   // entries of a slice's list
 
-// How a call is split: one wave a group up to 8 candidates a lane (64 x 16 x 21); a beam's lanes are at most a wave, so three or
-// four beams take one workgroup of four waves up to 32 a lane, more of them four waves up to 8, else 8 or (more than four, more than
-// eight beams) 16 waves up to 16 (8 x 6 x 882: 12 us with 8 waves, 15 with 16, 14 with 4); else slices and a second pass.  A slice is a row of up to 512 or 1024 logits for one wave (250 x 16 x 700, 16 kept: 28 us, with four waves
-// 33), else 256 u logits for four: u = 32 where rows hold two such slices and there are 300 (512 rows of 31839 fp32: 33 us with
-// 32, 44 with 8; 32 rows: 15.6 and 14.0; 2048 rows of 9000 bf16: 75 and 53).
+// How a call is split.  One wave a group up to 8 candidates a lane (64 x 16 x 21).  A beam's lanes are at most a wave: three or
+// four beams take one workgroup of four waves, up to 32 a lane; more of them four waves up to 8, else 8 or (more than eight beams)
+// 16 waves up to 16 (8 x 6 x 882: 12 us with 8 waves, 15 with 16, 14 with 4).  Else slices and a second pass: a row of up to 512 or
+// 1024 logits for one wave (250 x 20 x 700 and more; 250 x 16 x 700 took 28 us so, with four waves 33), or 256 u logits for four:
+// u = 32 where rows hold two such slices and there are 300 (512 rows of 31839 fp32: 33 us with 32, 44 with 8; 32 rows: 15.6 and
+// 14.0; 2048 rows of 9000 bf16: 75 and 53).
 struct SelectPlan {
   int waves, g_log2, m;  // waves a group, 0 = slices; 2^g_log2 lanes a beam; candidates a lane
   int u, per, splits;    // slices: values a thread holds, waves a slice, slices a beam
