@@ -44,6 +44,18 @@ def select(logits, scores, bias=None, forced=None, n_out=None):
     return out, parent, token
 
 
+def select_large(logits, scores, n):
+    """select() without bias and forced tokens, for finite inputs and scores of -inf, by a stable sort of whole groups."""
+    B, W, V = logits.shape
+    x = logits.double()
+    c = scores.double()[..., None] + (x - torch.logsumexp(x, -1, keepdim=True))
+    s, i = torch.sort(c.view(B, -1), dim=1, descending=True, stable=True)
+    s, i = s[:, :n], i[:, :n]
+    slot = torch.arange(n).expand(B, n) % W
+    dead = s == -math.inf
+    return s, torch.where(dead, slot, i // V), torch.where(dead, torch.zeros_like(i), i % V)
+
+
 def reorder(state, parent, length=None, rank=None):
     """A new tensor: state[b, j] = old state[b, parent[b, j]], at the positions that move."""
     out = state.clone()

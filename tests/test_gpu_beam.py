@@ -60,6 +60,25 @@ def test_select(B, W, V, dtype):
     _run(*_case(B, W, V, dtype, seed=V + W))
 
 
+@pytest.mark.parametrize("B,W,V,n", [(3, 17, 174, 17), (2, 9, 468, 18), (2, 6, 882, 6), (3, 64, 250, 64), (2, 256, 60, 256),
+                                     (3, 2, 700, 2), (2, 1, 1024, 9), (3, 40, 600, 40), (2, 70, 900, 64), (2, 100, 130, 100),
+                                     (2, 64, 20000, 64), (1, 64, 131072, 64), (2, 200, 3000, 200), (2, 3, 40000, 256),
+                                     (40, 20, 17000, 20)])
+@pytest.mark.parametrize("values", ["fp32", "bf16", "coarse"])
+def test_select_ways_of_splitting(B, W, V, n, values):
+    """Sizes on each side of the rules that split a call; the last group is at a search's first step (one beam alive)."""
+    import mpnn_amd
+    from oracle import beam_oracle as orc
+
+    g = torch.Generator().manual_seed(W + V)
+    logits = 2.5 * torch.randn(B, W, V, generator=g)
+    logits = logits.bfloat16() if values == "bf16" else (4 * logits).round() / 4 if values == "coarse" else logits
+    scores = -torch.cumsum(torch.rand(B, W, generator=g), 1)
+    scores[B - 1, 1:] = NEG
+    got = mpnn_amd.beam_select(logits.cuda(), scores.cuda(), n_out=n)
+    _check(got, orc.select_large(logits, scores, n))
+
+
 @pytest.mark.parametrize("bias", ["shared", "group", "beam", "each"])
 @pytest.mark.parametrize("B,W,V", [(4, 4, 21), (2, 16, 21), (3, 5, 700), (2, 3, 9001)])
 def test_select_bias_and_forced(B, W, V, bias):
@@ -74,7 +93,7 @@ def test_select_numbers_kept(B, W, V, n_out):
     _run(*_case(B, W, V, torch.bfloat16, 8), n_out=n_out)
 
 
-@pytest.mark.parametrize("W,V", [(3, 21), (4, 32), (2, 1300), (2, 5000)])
+@pytest.mark.parametrize("W,V", [(3, 21), (4, 32), (2, 1300), (2, 5000), (2, 600), (1, 1000), (60, 400), (9, 900)])
 def test_select_ties(W, V):
     """Constant logits: every token of a beam ties, and with equal scores the beams do too."""
     for scores in (torch.zeros(2, W), -torch.arange(2.0 * W).view(2, W) / 8):
