@@ -335,6 +335,12 @@ void check_dense(const at::Tensor& t, const char* what) {
                   " must be contiguous fp32 tensors on a ROCm device (the HIP path has no CPU fallback)");
 }
 
+at::Tensor sumsq_parts(Py_ssize_t n, const float* const* p, const long long* numel, const c10::Device& dev) {
+  at::Tensor parts = at::empty({kParts}, at::TensorOptions().device(dev).dtype(at::kDouble));
+  check_rc(f_parts((int)n, p, numel, parts.data_ptr<double>(), stream_of(dev)), "mpnn_grad_sumsq_parts");
+  return parts;
+}
+
 // grad_sumsq_parts(grads) -> float64 [256]
 at::Tensor sumsq_parts(const Items& grads) {
   std::vector<const float*> p(grads.n);
@@ -349,9 +355,7 @@ at::Tensor sumsq_parts(const Items& grads) {
     numel[i] = g.numel();
   }
   const c10::OptionalDeviceGuard guard(dev);
-  at::Tensor parts = at::empty({kParts}, at::TensorOptions().device(dev).dtype(at::kDouble));
-  check_rc(f_parts((int)grads.n, p.data(), numel.data(), parts.data_ptr<double>(), stream_of(dev)), "mpnn_grad_sumsq_parts");
-  return parts;
+  return sumsq_parts(grads.n, p.data(), numel.data(), dev);
 }
 
 PyObject* py_parts(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -425,7 +429,7 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     // a parameter listed twice would be stepped by two workgroups at once
     order.resize(n);
     for (Py_ssize_t i = 0; i < n; ++i) order[i] = {p[i], p[i] + numel[i]};
-    std::sort(order.begin(), order.end());
+    if (!std::is_sorted(order.begin(), order.end())) std::sort(order.begin(), order.end());
     for (Py_ssize_t i = 1; i < n; ++i)
       if (order[i].first < order[i - 1].second) value_error("mpnn_amd.optim.adamw_step: two parameters share memory");
     const double max_norm = number(a[14]);
@@ -437,7 +441,7 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (parts.numel() != kParts || parts.scalar_type() != at::kDouble || !parts.is_contiguous())
           value_error("mpnn_amd.optim.adamw_step: parts come from grad_sumsq_parts");
       } else {
-        parts = sumsq_parts(G);
+        parts = sumsq_parts(n, g.data(), numel.data(), dev);
       }
       sumsq = at::empty({1}, at::TensorOptions().device(dev).dtype(at::kFloat));
     }
