@@ -9,8 +9,8 @@
 // rounding to nearest would freeze it; rounded up with the probability of the part cut off, the stored moment follows the
 // exact one in the mean.  The bits come from a hash of (seed, step, tensor, element): a step is the same on every run.  v
 // above zero is never stored as zero (m / eps would follow).  A power of two scales without a rounding of its own, so the
-// stored value has one error only, and moments are fp64 up to it (the fp64 vector rate is the fp32 one): which code an element gets does not hang
-// on the order of operations.  Memory-bound: 16.25 bytes an element of an 8-bit tensor (28 with 32-bit moments), and 4 more
+// stored value has one error only, and moments are fp64 up to it (the fp64 vector rate is the fp32 one): which code an element
+// gets does not hang on the order of operations.  Memory-bound: 16.25 bytes an element of an 8-bit tensor (28 with 32-bit moments), and 4 more
 // where the norm is needed.
 #include <hip/hip_runtime.h>
 #include <math.h>
