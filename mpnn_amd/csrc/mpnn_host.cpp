@@ -294,23 +294,38 @@ PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (begin < s.end && s.begin < end) return t.clone();
       return t;
     };
-    int length_all = -1;
+    long long all = -1;
     at::Tensor lengths, rank;
     if (positions) {
       if (THPVariable_Check(a[2])) {
-        const at::Tensor& t = on_gpu(a[2], what, "length", &dev);
-        if (t.dim() != 1 || t.size(0) != B || !whole(t))
+        lengths = on_gpu(a[2], what, "length", &dev);
+        if (lengths.dim() != 1 || lengths.size(0) != B || !whole(lengths))
           value_error("mpnn_amd.beam_reorder: length must be an int or integers [" + std::to_string(B) + "]");
-        lengths = beside_states(t.to(at::kInt).contiguous());
       } else {
-        length_all = (int)std::max(0LL, std::min(integer(a[2]), 0x7fffffffLL));
+        all = integer(a[2]);
       }
     }
     if (a[3] != Py_None) {
-      const at::Tensor& t = on_gpu(a[3], what, "rank", &dev);
-      if (!whole(t) || (L >= 0 && (t.dim() != 2 || t.size(0) != B || t.size(1) != L)))
+      rank = on_gpu(a[3], what, "rank", &dev);
+      if (!whole(rank) || (L >= 0 && (rank.dim() != 2 || rank.size(0) != B || rank.size(1) != L)))
         value_error("mpnn_amd.beam_reorder: rank must be integers [" + std::to_string(B) + ", " + std::to_string(L) + "]");
-      rank = beside_states(t.to(at::kInt).contiguous());
+    }
+    // The library compares in 32 bits.  Positions without a rank are below 2^31, so clamping a length changes nothing; where a
+    // rank, or the length it is compared with, has 64 bits, the comparison's result takes its place: 0 < 1 moves, 1 < 1 stays.
+    constexpr long long most = 0x7fffffff;
+    int length_all = -1;
+    if (positions && !table.empty()) {
+      if (rank.defined() && (rank.scalar_type() == at::kLong ||
+                             (lengths.defined() ? lengths.scalar_type() == at::kLong : all < 0 || all > most))) {
+        rank = (lengths.defined() ? rank.ge(lengths.unsqueeze(1)) : rank.to(at::kLong).ge(all)).to(at::kInt).contiguous();
+        lengths.reset();
+        length_all = 1;
+      } else {
+        if (rank.defined()) rank = beside_states(rank.contiguous());
+        if (!lengths.defined()) length_all = (int)std::max(0LL, std::min(all, most));
+        else if (lengths.scalar_type() == at::kLong) lengths = lengths.clamp(0, most).to(at::kInt);
+        else lengths = beside_states(lengths.contiguous());
+      }
     }
     if (!table.empty()) {
       const at::Tensor parent = beside_states(given.to(at::kLong).contiguous());
