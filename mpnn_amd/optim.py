@@ -223,9 +223,11 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Checkpoints of 8-bit and of 32-bit moments (this optimizer's, torch's) load into an optimizer of either width.  With
-        8-bit moments the state is copied: codes and scales of two optimizers may not get out of step."""
+        8-bit moments the state is copied: codes, scales and counts of two optimizers may not get out of step."""
         super().load_state_dict(state_dict)
         for p, st in self.state.items():
+            if self.state_bits == 8 and torch.is_tensor(st.get("step")):
+                st["step"] = st["step"].clone()   # torch hands on the source's own, which its owner may add to in place
             if "exp_avg" not in st:
                 continue
             wide = self.state_bits == 8 and p.numel() >= self.min_8bit_numel
