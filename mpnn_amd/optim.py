@@ -116,7 +116,7 @@ class AdamW(torch.optim.Optimizer):
                                       fused=None, decoupled_weight_decay=True))
         self.max_grad_norm = float(max_grad_norm)
         self.state_bits, self.min_8bit_numel, self.seed = state_bits, int(min_8bit_numel), int(seed)
-        self._zero = torch.tensor(0.0)  # the step count of parameters without a step (8-bit moments)
+        self._counts, self._steps, self._at = None, [], {}  # 8-bit moments: see _gather_counts
         self.last_grad_sumsq = None  # device scalar of the last step (its square root is the unclipped gradient norm)
 
     @torch.no_grad()
@@ -171,7 +171,7 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _new_state(self, p):
-        st = {"step": self._zero}
+        st = {"step": torch.tensor(0.0)}
         if p.numel() < self.min_8bit_numel:
             st["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
             st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
@@ -188,30 +188,45 @@ class AdamW(torch.optim.Optimizer):
         parts, self.last_grad_sumsq = None, None
         if self.max_grad_norm > 0.0:
             parts = host_call("mpnn_grad_sumsq_parts", "grad_sumsq_parts", [p.grad for p in every])
-        first = 0
-        # parameters that took the same steps share one `step` tensor (adding to each of 118 cost more than the kernels): the
-        # next count is a new tensor, parameters without a gradient keep the old one
-        counted, shared = {}, {}
-        for group, ps in zip(self.param_groups, live):
-            by_step = {}
-            for p in ps:
-                st = self.state[p]
-                if not st:
-                    st.update(self._new_state(p))
-                old = st["step"]
-                if id(old) not in counted:
-                    counted[id(old)] = int(old) + 1
-                by_step.setdefault(counted[id(old)], []).append((p, st))
-            for k, sel in sorted(by_step.items(), key=lambda x: x[0]):
-                lists = [[st.get(n) for _, st in sel] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
-                ss = host_call("mpnn_adamw_mixed", "adamw", [p for p, _ in sel], [p.grad for p, _ in sel], *lists, k, group["lr"],
+        states = [[self.state[p] for p in ps] for ps in live]
+        places = lambda: [[self._at.get(id(st.get("step"))) for st in sts] for sts in states]   # noqa: E731
+        at_of = places()
+        if any(None in at for at in at_of):
+            for ps, sts in zip(live, states):
+                for p, st in zip(ps, sts):
+                    if not st:
+                        st.update(self._new_state(p))
+            self._gather_counts()
+            at_of = places()
+        counts, first = self._counts.tolist(), 0
+        for group, ps, sts, at in zip(self.param_groups, live, states, at_of):
+            taken = [counts[i] for i in at]
+            for k in sorted(set(taken)):
+                sel = (ps, sts, at)
+                if taken.count(k) < len(taken):
+                    sel = [[x for x, c in zip(xs, taken) if c == k] for xs in sel]
+                lists = [[st.get(n) for st in sel[1]] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
+                ss = host_call("mpnn_adamw_mixed", "adamw", sel[0], [p.grad for p in sel[0]], *lists, int(k) + 1, group["lr"],
                                group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"],
                                self.seed & 0xFFFFFFFF, first, self.max_grad_norm, parts)
                 self.last_grad_sumsq = ss if ss is not None else self.last_grad_sumsq
-                first += len(sel)
-                now = shared.setdefault(k, torch.tensor(float(k)))
-                for _, st in sel:
-                    st["step"] = now
+                first += len(sel[0])
+                i, n = sel[2][0], len(sel[2])
+                if sel[2] == list(range(i, i + n)):
+                    self._counts[i:i + n] += 1
+                else:
+                    self._counts[sel[2]] += 1
+
+    def _gather_counts(self):
+        """Make every parameter's `step` an element of one tensor: an operation counts for all (adding to each of 118 tensors
+        costs more than the kernels), and a program that writes one of them restarts that parameter alone.  Done whenever a
+        state holds a `step` that is not such an element (a new parameter, a loaded state, one that a program put there)."""
+        states = [st for st in self.state.values() if "step" in st]
+        self._counts = torch.tensor([float(st["step"]) for st in states], dtype=torch.float32, device="cpu")
+        self._steps = [self._counts[i] for i in range(len(states))]   # kept: their ids are the keys of _at
+        self._at = {id(s): i for i, s in enumerate(self._steps)}
+        for st, s in zip(states, self._steps):
+            st["step"] = s
 
     def state_dict(self):
         """As torch's; with 8-bit moments every parameter gets a `step` tensor of its own (an optimizer that adds to them in
@@ -226,8 +241,6 @@ class AdamW(torch.optim.Optimizer):
         8-bit moments the state is copied: codes, scales and counts of two optimizers may not get out of step."""
         super().load_state_dict(state_dict)
         for p, st in self.state.items():
-            if self.state_bits == 8 and torch.is_tensor(st.get("step")):
-                st["step"] = st["step"].clone()   # torch hands on the source's own, which its owner may add to in place
             if "exp_avg" not in st:
                 continue
             wide = self.state_bits == 8 and p.numel() >= self.min_8bit_numel
@@ -242,3 +255,5 @@ class AdamW(torch.optim.Optimizer):
                     st[name], st[name + "_scale"] = st[name].to(torch.float8_e4m3fn), scale.clone()
                 else:
                     st[name] = unpack_moment(st[name], scale)
+        if self.state_bits == 8:
+            self._gather_counts()   # torch hands on the source's own `step` tensors, which their owner may add to in place
