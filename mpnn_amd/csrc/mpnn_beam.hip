@@ -1133,7 +1133,7 @@ __device__ __forceinline__ void reorder_through_lds(char* data, long long sw, in
       needed[m] |= (unsigned long long)lo | (unsigned long long)hi << 32;
     }
   }
-  if (!live) return;
+  // a lane without a column (or whose position stays) goes on with the others: it holds parents that they ask it for
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     for (int w0 = 64 * k; w0 < W && w0 < 64 * k + 64; w0 += 8) {   // eight rows in flight
@@ -1142,10 +1142,10 @@ __device__ __forceinline__ void reorder_through_lds(char* data, long long sw, in
       V r[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (bits >> i & 1) r[i] = *(const V*)(data + (w0 + i) * sw);
+        if ((bits >> i & 1) && live) r[i] = *(const V*)(data + (w0 + i) * sw);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (bits >> i & 1) lds[(w0 + i) * 64 + lane] = r[i];
+        if ((bits >> i & 1) && live) lds[(w0 + i) * 64 + lane] = r[i];
     }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -1159,7 +1159,7 @@ __device__ __forceinline__ void reorder_through_lds(char* data, long long sw, in
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (f[i] >= 0) *(V*)(data + (w0 + i) * sw) = r[i];
+        if (f[i] >= 0 && live) *(V*)(data + (w0 + i) * sw) = r[i];
     }
 }
 

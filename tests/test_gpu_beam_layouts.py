@@ -1,4 +1,4 @@
-"""beam_reorder: ranks and lengths of 64 bits."""
+"""beam_reorder: ranks and lengths of 64 bits, and waves with few columns."""
 import pytest
 import torch
 
@@ -75,3 +75,23 @@ def test_64_bit_rank_in_a_graph():
         graph.replay()
         same = torch.equal(state.cpu(), orc.reorder(*cpu))
         assert same
+
+
+@pytest.mark.parametrize("W", [65, 66, 100, 128, 129, 200, 255, 256])
+@pytest.mark.parametrize("columns", [1, 3, 63, 64, 65, 130])
+def test_waves_with_few_columns(W, columns):
+    """Beyond 64 beams every lane holds the parents of its beams, also a lane without a column, or whose position stays."""
+    import mpnn_amd
+    from oracle import beam_oracle as orc
+
+    g = torch.Generator().manual_seed(W + columns)
+    parent = torch.randint(0, W, (2, W), generator=g)
+    cpu = torch.randn(2, W, columns, generator=g)
+    dev = cpu.cuda()
+    mpnn_amd.beam_reorder(dev, parent.cuda())
+    want = orc.reorder(cpu, parent)
+    assert torch.equal(dev.cpu(), want)
+    rank = torch.argsort(torch.rand(2, columns, generator=g), 1).to(torch.int32)
+    length = torch.tensor([1, columns // 2])
+    mpnn_amd.beam_reorder(dev, parent.cuda(), length.cuda(), rank.cuda())
+    assert torch.equal(dev.cpu(), orc.reorder(want, parent, length, rank))
