@@ -33,5 +33,6 @@ def beam_reorder(states, parent, length=None, rank=None):
     dimension of such runs (a [B, W, heads, :t, D] prefix is).  parent: integers [B, W]; a parent outside [0, W) leaves its
     row as it is.  length: an int, or integers [B]: only the positions p < length[b] of dimension 2 move, the others are not
     touched.  rank: integers [B, L], with `length`: position p moves where rank[b, p] < length[b] (a decoding order other
-    than left to right; 64-bit integers compare as such).  At most 256 beams.  No two states may share memory."""
+    than left to right; 64-bit integers compare as such).  At most 256 beams.  No two states may share memory
+    (rows of one may lie between the other's: keys and values of one [B, W, 2, heads, T, D] buffer)."""
     return host_call("mpnn_beam_reorder", "beam_reorder", states, parent, length, rank)

@@ -13,7 +13,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <climits>
+#include <memory>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "mpnn_hip.h"
@@ -217,23 +220,63 @@ long long state_span(const at::Tensor& x) {
   return extent;
 }
 
+// a state's rows: runs of bytes at up to three strides, the widest first, each at least what lies inside it spans (state_span)
+struct Rows {
+  int n = 0;
+  long long stride[3], count[3], extent[4];   // extent[i]: bytes from level i's first to behind its last; [n]: the run
+};
 struct Span {
   long long begin, end;               // bytes
-  long long stride[3];
-  long long run;
+  Rows rows;
 };
 
+Span state_rows(const at::Tensor& x, const Layout& l, long long extent) {
+  const long long item = x.element_size(), begin = (long long)x.const_data_ptr();
+  std::pair<long long, long long> dims[3] = {{x.stride(0), x.size(0)}, {x.stride(1), x.size(1)}, {l.stride_mid, l.n_mid}};
+  std::sort(dims, dims + 3, [](const auto& a, const auto& b) { return a.first > b.first; });
+  Span s = {begin, begin + extent * item, {}};
+  Rows& r = s.rows;
+  for (const auto& d : dims)
+    if (d.second > 1) {
+      r.stride[r.n] = d.first * item;
+      r.count[r.n++] = d.second;
+    }
+  r.extent[r.n] = l.run * item;
+  for (int i = r.n - 1; i >= 0; --i) r.extent[i] = r.stride[i] * (r.count[i] - 1) + r.extent[i + 1];
+  return s;
+}
+
+long long floor_div(long long x, long long y) { return x / y - (x % y < 0); }
+
+// a's rows from level i on, b's from level j on d bytes behind them: do they share a byte?  The level with the wider stride is
+// taken apart (both, if they are equal: what counts is then the distance of two blocks); `left`: steps until it says yes.
+bool meet(const Rows& a, int i, const Rows& b, int j, long long d, int& left) {
+  if (d >= a.extent[i] || -d >= b.extent[j]) return false;
+  if ((i == a.n && j == b.n) || --left < 0) return true;
+  const long long sa = i < a.n ? a.stride[i] : 0, sb = j < b.n ? b.stride[j] : 0, s = std::max(sa, sb);
+  const int da = sa == s, db = sb == s;
+  const long long lo = std::max(da ? 1 - a.count[i] : 0, floor_div(-b.extent[j + db] - d, s) + 1);
+  const long long hi = std::min(db ? b.count[j] - 1 : 0, -floor_div(d - a.extent[i + da], s) - 1);
+  for (long long k = lo; k <= hi; ++k)
+    if (meet(a, i + da, b, j + db, d + k * s, left)) return true;
+  return false;
+}
+
 // two states share no byte though their ranges meet: rows of one lie between those of the other
-bool apart(const Span& a, const Span& b) {
-  long long m = 0;
-  for (int i = 0; i < 3; ++i)
-    for (long long s : {a.stride[i], b.stride[i]})
-      if (s && (!m || s < m)) m = s;
-  if (!m) return false;
-  for (int i = 0; i < 3; ++i)
-    if (a.stride[i] % m || b.stride[i] % m) return false;
-  const long long d = (b.begin - a.begin) % m;
-  return d >= a.run && d + b.run <= m;
+bool apart(const Span& x, const Span& y) {
+  const Rows &a = x.rows, &b = y.rows;
+  const long long d = y.begin - x.begin;
+  // all strides are multiples of the smallest, and the runs lie side by side in it
+  const long long m = std::min(a.n ? a.stride[a.n - 1] : LLONG_MAX, b.n ? b.stride[b.n - 1] : LLONG_MAX);
+  bool even = m < LLONG_MAX;
+  for (int i = 0; i < a.n; ++i) even &= a.stride[i] % m == 0;
+  for (int i = 0; i < b.n; ++i) even &= b.stride[i] % m == 0;
+  if (even) {
+    const long long r = d - floor_div(d, m) * m;
+    if (r >= a.extent[a.n] && r + b.extent[b.n] <= m) return true;
+  }
+  int left = 4096;
+  return !meet(a, 0, b, 0, d, left);
 }
 
 PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -280,7 +323,7 @@ PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       const long long sb = B > 1 ? x.stride(0) * item : 0, sw = W > 1 ? x.stride(1) * item : 0, sm = lay.stride_mid * item;
       char* data = (char*)x.data_ptr();
       table.push_back({data, sb, sw, sm, lay.run * item, (int)lay.n_mid});
-      spans.push_back({(long long)data, (long long)data + extent * item, {sb, sw, lay.n_mid > 1 ? sm : 0}, lay.run * item});
+      spans.push_back(state_rows(x, lay, extent));
     }
     std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.begin < y.begin; });
     for (size_t i = 0; i < spans.size(); ++i)
@@ -506,6 +549,23 @@ PyObject* py_span(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// whether beam_reorder may move the two states in one call: None where one of them is refused by itself
+PyObject* py_apart(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 3) type_error("states_apart: three arguments");
+    Span s[2];
+    for (int i = 0; i < 2; ++i) {
+      const at::Tensor& t = tensor(a[i], "states_apart", "state");
+      const Layout l = state_layout(t, PyObject_IsTrue(a[2]) == 1);
+      const long long extent = state_span(t);
+      if (!l.regular || !extent || !t.numel()) Py_RETURN_NONE;
+      s[i] = state_rows(t, l, extent);
+    }
+    const Span &x = s[0].begin <= s[1].begin ? s[0] : s[1], &y = s[0].begin <= s[1].begin ? s[1] : s[0];
+    return PyBool_FromLong(y.begin >= x.end || apart(x, y));
+  });
+}
+
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)(void))py_bind, METH_FASTCALL, "addresses of the HIP library's functions"},
     {"beam_select", (PyCFunction)(void (*)(void))py_select, METH_FASTCALL, "mpnn_amd.beam_select, arguments in order"},
@@ -513,6 +573,7 @@ PyMethodDef methods[] = {
     {"grad_sumsq_parts", (PyCFunction)(void (*)(void))py_parts, METH_FASTCALL, "partial sums of squares over gradients"},
     {"adamw", (PyCFunction)(void (*)(void))py_adamw, METH_FASTCALL, "mpnn_amd.optim.adamw_step, arguments in order"},
     {"state_layout", (PyCFunction)(void (*)(void))py_layout, METH_FASTCALL, "layout of a state behind its beams"},
+    {"states_apart", (PyCFunction)(void (*)(void))py_apart, METH_FASTCALL, "whether two states share no byte"},
     {"state_span", (PyCFunction)(void (*)(void))py_span, METH_FASTCALL, "elements a state spans"},
     {nullptr, nullptr, 0, nullptr}};
 

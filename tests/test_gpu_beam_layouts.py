@@ -1,4 +1,4 @@
-"""beam_reorder: ranks and lengths of 64 bits, and waves with few columns."""
+"""beam_reorder: ranks and lengths of 64 bits, states that lie between each other in one buffer, and waves with few columns."""
 import pytest
 import torch
 
@@ -95,3 +95,43 @@ def test_waves_with_few_columns(W, columns):
     length = torch.tensor([1, columns // 2])
     mpnn_amd.beam_reorder(dev, parent.cuda(), length.cuda(), rank.cuda())
     assert torch.equal(dev.cpu(), orc.reorder(want, parent, length, rank))
+
+
+PACKED = {   # views of one buffer that share no byte
+    "keys_values_prefix": ((2, 3, 2, 4, 9, 8), lambda x: [x[:, :, 0, :, :5], x[:, :, 1, :, :5]], None),
+    "keys_values": ((2, 3, 2, 4, 9, 8), lambda x: [x[:, :, 1], x[:, :, 0]], None),
+    "behind_heads": ((2, 3, 4, 2, 9, 8), lambda x: [x[:, :, :, 0, :5], x[:, :, :, 1, :5]], None),
+    "layers": ((2, 3, 3, 2, 9, 8), lambda x: [x[:, :, i, j, :6] for i in range(3) for j in range(2)], None),
+    "different_lengths": ((2, 3, 2, 4, 9, 8), lambda x: [x[:, :, 0, :, :5], x[:, :, 1, :, :7], x[:, :, 0, :, 5:], x[:, :, 1, :, 7:]], None),
+    "different_types_of_rows": ((2, 3, 40), lambda x: [x[:, :, :8], x[:, :, 8:40].view(2, 3, 4, 8)[..., :5], x[:, :, 13]], None),
+    "positions": ((2, 3, 2, 9, 8), lambda x: [x[:, :, 0], x[:, :, 1]], 4),
+    "beams_first": ((3, 2, 2, 4, 9, 8), lambda x: [x.transpose(0, 1)[:, :, k, :, :5] for k in (0, 1)], None),
+}
+
+
+@pytest.mark.parametrize("name", list(PACKED))
+def test_states_packed_into_one_buffer(name):
+    import mpnn_amd
+    from oracle import beam_oracle as orc
+
+    shape, views, length = PACKED[name]
+    buf = torch.randn(shape, generator=torch.Generator().manual_seed(3))
+    parent = torch.tensor([[2, 0, 0], [1, 2, 1]])
+    dev = buf.cuda()
+    mpnn_amd.beam_reorder(views(dev), parent.cuda(), length)
+    want = buf.clone()
+    for x, y in zip(views(want), views(buf)):
+        x.copy_(orc.reorder(y, parent, length))
+    same = torch.equal(dev.cpu(), want)
+    assert same
+
+
+def test_states_that_share_a_byte_of_one_buffer_are_refused():
+    import mpnn_amd
+
+    x = torch.zeros(2, 3, 2, 4, 9, 8, device="cuda")
+    parent = torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    for pair in ([x[:, :, 0, :, :5], x[:, :, :, 3]], [x[:, :, 0, :, :5], x[:, :, 0, :, 4:]], [x[:, :, 0], x[:, :, 0, 1]],
+                 [x[:, :, 1, :, :5], x[:, :, 1, :, :5]], [x[:, :, :, 0], x[:, :, 1, :, :2]]):
+        with pytest.raises(ValueError, match="share memory"):
+            mpnn_amd.beam_reorder(pair, parent)
