@@ -233,7 +233,7 @@ int mpnn_adamw_step(int n, float* const* params, const float* const* grads, floa
  * sumsq_parts != NULL and max_norm > 0: gradients are scaled by min(1, max_norm / (norm + 1e-6)), norm^2 = the sum of the
  * 256 doubles that mpnn_grad_sumsq_parts wrote (all of them, from any number of tensors; fp64, fixed order); grad_sumsq
  * (may be NULL) gets norm^2.  Moments are fp64 up to their rounding, the update is fp32.  step >= 1.  numel < 2^32.  No
- * two tensors may share memory.  At most 32768 tensors in mpnn_grad_sumsq_parts. */
+ * two tensors may share memory, but for gradients among themselves (not checked here).  At most 32768 tensors in mpnn_grad_sumsq_parts. */
 int mpnn_grad_sumsq_parts(int n, const float* const* grads, const long long* numel, double* parts, void* stream);
 int mpnn_adamw_mixed(int n, float* const* params, const float* const* grads, void* const* exp_avg, void* const* exp_avg_sq,
                      float* const* exp_avg_scale, float* const* exp_avg_sq_scale, const long long* numel, double lr,

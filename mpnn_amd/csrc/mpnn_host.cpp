@@ -386,6 +386,140 @@ PyObject* py_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 // ---- optimizer ----
 constexpr int kBlock = 64, kParts = 256;
 
+// Tensors cut from a few buffers, or made one after the other, first: lists are a few ascending runs, and where no two runs meet, no
+// two tensors do.  (300 tensors with their state: 0.5 us; 5-6 with Ranges, which takes any.)
+struct Runs {
+  static constexpr int kMost = 24;
+  static constexpr long long kGap = 16384;   // a larger one may hold another list
+  const char *begin[kMost], *end[kMost];
+  int n = 0;
+  // false: more runs than this holds
+  bool add(const void* p, long long bytes) {
+    const char* b = (const char*)p;
+    if (n && b >= end[n - 1] && b - end[n - 1] <= kGap) {
+      end[n - 1] = b + bytes;
+      return true;
+    }
+    if (n == kMost) return false;
+    begin[n] = b;
+    end[n++] = b + bytes;
+    return true;
+  }
+  // whether some run of this one meets another, or one of `read`
+  bool meet(const Runs& read) const {
+    for (int i = 0; i < n; ++i) {
+      for (int j = 0; j < i; ++j)
+        if (begin[i] < end[j] && begin[j] < end[i]) return true;
+      for (int j = 0; j < read.n; ++j)
+        if (begin[i] < read.end[j] && read.begin[j] < end[i]) return true;
+    }
+    return false;
+  }
+};
+
+// Any tensors: their byte ranges, kept as ascending runs, merged into one.
+struct Ranges {
+  using Range = std::pair<const char*, const char*>;
+  std::vector<Range> at;
+  std::vector<size_t> run;            // where each run begins
+  void add(const void* p, long long bytes) {
+    const char* begin = (const char*)p;
+    if (at.empty() || begin < at.back().second) run.push_back(at.size());
+    at.emplace_back(begin, begin + bytes);
+  }
+  // into one ascending run; false if two share a byte
+  bool sort() {
+    std::vector<std::pair<size_t, size_t>> part;   // begin, end of the runs
+    for (size_t i = 0; i < run.size(); ++i) part.emplace_back(run[i], i + 1 < run.size() ? run[i + 1] : at.size());
+    std::sort(part.begin(), part.end(), [&](const auto& x, const auto& y) { return at[x.first].first < at[y.first].first; });
+    std::vector<Range> out;
+    std::vector<size_t> edge = {0};
+    out.reserve(at.size());
+    for (const auto& x : part) {
+      out.insert(out.end(), at.begin() + x.first, at.begin() + x.second);
+      edge.push_back(out.size());
+    }
+    for (; edge.size() > 2;) {
+      std::vector<size_t> next = {0};
+      for (size_t i = 0; i + 1 < edge.size(); i += 2) {
+        const size_t end = edge[std::min(i + 2, edge.size() - 1)];
+        if (edge[i + 1] < end && out[edge[i + 1]].first < out[edge[i + 1] - 1].second)
+          std::inplace_merge(out.begin() + edge[i], out.begin() + edge[i + 1], out.begin() + end);
+        next.push_back(end);
+      }
+      edge.swap(next);
+    }
+    at.swap(out);
+    run.assign(at.empty() ? 0 : 1, 0);
+    for (size_t i = 1; i < at.size(); ++i)
+      if (at[i].first < at[i - 1].second) return false;
+    return true;
+  }
+  // of a sorted one: whether any range of `r` shares a byte with it
+  bool meets(const Ranges& r) const {
+    for (size_t i = 0; i < r.run.size(); ++i) {
+      const size_t end = i + 1 < r.run.size() ? r.run[i + 1] : r.at.size();
+      auto w = std::upper_bound(at.begin(), at.end(), r.at[r.run[i]].first,
+                                [](const char* x, const Range& y) { return x < y.second; });   // the first to end behind it
+      if (w == at.end() || w->first >= r.at[end - 1].second) continue;
+      for (size_t j = r.run[i]; j < end; ++j) {
+        while (w != at.end() && w->second <= r.at[j].first) ++w;
+        if (w == at.end()) break;
+        if (w->first < r.at[j].second) return true;
+      }
+    }
+    return false;
+  }
+};
+
+// the addresses of an optimizer step; ms[i] and vs[i] NULL where the moments have no scales
+struct StepLists {
+  Py_ssize_t n;
+  float* const* p;
+  const float* const* g;
+  void* const* m;
+  void* const* v;
+  float* const* ms;
+  float* const* vs;
+  const long long* numel;
+  long long bytes(Py_ssize_t i) const { return (ms[i] ? 1 : 4) * numel[i]; }
+  long long scale_bytes(Py_ssize_t i) const { return (numel[i] + kBlock - 1) / kBlock * 4; }
+};
+
+// whether a look at runs shows that no tensors of a step meet
+bool plainly_apart(const StepLists& l) {
+  Runs read, written;
+  for (Py_ssize_t i = 0; i < l.n; ++i)
+    if (!read.add(l.g[i], 4 * l.numel[i])) return false;
+  for (Py_ssize_t i = 0; i < l.n; ++i)
+    if (!written.add(l.p[i], 4 * l.numel[i])) return false;
+  for (const auto x : {l.m, l.v})
+    for (Py_ssize_t i = 0; i < l.n; ++i)
+      if (!written.add(x[i], l.bytes(i))) return false;
+  for (const auto x : {l.ms, l.vs})
+    for (Py_ssize_t i = 0; i < l.n; ++i)
+      if (x[i] && !written.add(x[i], l.scale_bytes(i))) return false;
+  return !written.meet(read);
+}
+
+// What a step writes would otherwise be written, or read as a gradient, by two workgroups at once.  NULL, or what is wrong.
+const char* shared_memory(const StepLists& l) {
+  if (plainly_apart(l)) return nullptr;
+  Ranges writes, reads;
+  writes.at.reserve(5 * l.n);
+  for (Py_ssize_t i = 0; i < l.n; ++i) writes.add(l.p[i], 4 * l.numel[i]);
+  for (const auto x : {l.m, l.v})
+    for (Py_ssize_t i = 0; i < l.n; ++i) writes.add(x[i], l.bytes(i));
+  for (const auto x : {l.ms, l.vs})
+    for (Py_ssize_t i = 0; i < l.n; ++i)
+      if (x[i]) writes.add(x[i], l.scale_bytes(i));
+  reads.at.reserve(l.n);
+  for (Py_ssize_t i = 0; i < l.n; ++i) reads.add(l.g[i], 4 * l.numel[i]);
+  if (!writes.sort()) return "two parameters, moments or scales share memory";
+  if (writes.meets(reads)) return "a gradient shares memory with what the step writes";
+  return nullptr;
+}
+
 void check_dense(const at::Tensor& t, const char* what) {
   const c10::TensorImpl* x = t.unsafeGetTensorImpl();
   if (!x->is_cuda() || x->dtype() != caffe2::TypeMeta::fromScalarType(at::kFloat) || !x->is_contiguous())
@@ -441,7 +575,6 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     std::vector<const float*> g(n);
     std::vector<void*> m(n), v(n);
     std::vector<long long> numel(n);
-    std::vector<std::pair<const float*, const float*>> order;
     const c10::Device dev = tensor(P.at[0], "optim", "parameters").device();
     const char* name = "optim.adamw_step";
     const auto fp32 = caffe2::TypeMeta::fromScalarType(at::kFloat), fp8 = caffe2::TypeMeta::fromScalarType(at::kFloat8_e4m3fn);
@@ -484,12 +617,8 @@ PyObject* py_adamw(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         vs[i] = (float*)ts.data_ptr();
       }
     }
-    // a parameter listed twice would be stepped by two workgroups at once
-    order.resize(n);
-    for (Py_ssize_t i = 0; i < n; ++i) order[i] = {p[i], p[i] + numel[i]};
-    if (!std::is_sorted(order.begin(), order.end())) std::sort(order.begin(), order.end());
-    for (Py_ssize_t i = 1; i < n; ++i)
-      if (order[i].first < order[i - 1].second) value_error("mpnn_amd.optim.adamw_step: two parameters share memory");
+    if (const char* refusal = shared_memory({n, p.data(), g.data(), m.data(), v.data(), ms.data(), vs.data(), numel.data()}))
+      value_error(std::string("mpnn_amd.optim.adamw_step: ") + refusal);
     const double max_norm = number(a[14]);
     const c10::OptionalDeviceGuard guard(dev);
     at::Tensor parts, sumsq;
@@ -566,6 +695,28 @@ PyObject* py_apart(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// shared_memory of tensors on any device (unit tests without a GPU): params, grads, exp_avgs, exp_avg_sqs, scales, sq_scales
+PyObject* py_share(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 6) type_error("shared_memory: six arguments");
+    std::vector<void*> at[6];
+    std::vector<long long> numel;
+    for (int k = 0; k < 6; ++k) {
+      const Items l(a[k]);
+      if (k && (size_t)l.n != at[0].size()) value_error("shared_memory: lists of different lengths");
+      for (Py_ssize_t i = 0; i < l.n; ++i) {
+        const at::Tensor* t = l.at[i] == Py_None ? nullptr : &tensor(l.at[i], "shared_memory", "tensors");
+        at[k].push_back(t ? t->data_ptr() : nullptr);
+        if (k == 0) numel.push_back(t->numel());
+      }
+    }
+    const char* refusal = shared_memory({(Py_ssize_t)numel.size(), (float**)at[0].data(), (const float**)at[1].data(), at[2].data(),
+                                         at[3].data(), (float**)at[4].data(), (float**)at[5].data(), numel.data()});
+    if (!refusal) Py_RETURN_NONE;
+    return PyUnicode_FromString(refusal);
+  });
+}
+
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)(void))py_bind, METH_FASTCALL, "addresses of the HIP library's functions"},
     {"beam_select", (PyCFunction)(void (*)(void))py_select, METH_FASTCALL, "mpnn_amd.beam_select, arguments in order"},
@@ -573,6 +724,7 @@ PyMethodDef methods[] = {
     {"grad_sumsq_parts", (PyCFunction)(void (*)(void))py_parts, METH_FASTCALL, "partial sums of squares over gradients"},
     {"adamw", (PyCFunction)(void (*)(void))py_adamw, METH_FASTCALL, "mpnn_amd.optim.adamw_step, arguments in order"},
     {"state_layout", (PyCFunction)(void (*)(void))py_layout, METH_FASTCALL, "layout of a state behind its beams"},
+    {"shared_memory", (PyCFunction)(void (*)(void))py_share, METH_FASTCALL, "why an optimizer step over these tensors is refused"},
     {"states_apart", (PyCFunction)(void (*)(void))py_apart, METH_FASTCALL, "whether two states share no byte"},
     {"state_span", (PyCFunction)(void (*)(void))py_span, METH_FASTCALL, "elements a state spans"},
     {nullptr, nullptr, 0, nullptr}};

@@ -95,7 +95,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_
     fp32 moments; the others hold float8_e4m3fn codes and fp32 scales (see the module's docstring; zeros and ones to begin
     with).  step: 1 for the first.  seed, step, the place in the list and the element decide the rounding of 8-bit moments.
     max_grad_norm > 0 clips by the norm over all gradients.  Returns the squared norm (a device scalar) then, else None.
-    No two tensors may share memory.  A replayed HIP graph of this call repeats its step and its hyper-parameters."""
+    No two tensors may share memory, but for gradients among themselves.  A replayed HIP graph of this call repeats its step and its hyper-parameters."""
     return host_call("mpnn_adamw_mixed", "adamw", params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step,
                      lr, betas[0], betas[1], eps, weight_decay, int(seed) & 0xFFFFFFFF, 0, max_grad_norm, None)
 
@@ -186,8 +186,9 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("mpnn_amd.optim.AdamW(state_bits=8): a step counts on the host and cannot be captured into a HIP "
                                "graph")
         parts, self.last_grad_sumsq = None, None
+        grads = [[p.grad for p in ps] for ps in live]
         if self.max_grad_norm > 0.0:
-            parts = host_call("mpnn_grad_sumsq_parts", "grad_sumsq_parts", [p.grad for p in every])
+            parts = host_call("mpnn_grad_sumsq_parts", "grad_sumsq_parts", [g for gs in grads for g in gs])
         states = [[self.state[p] for p in ps] for ps in live]
         places = lambda: [[self._at.get(id(st.get("step"))) for st in sts] for sts in states]   # noqa: E731
         at_of = places()
@@ -199,23 +200,24 @@ class AdamW(torch.optim.Optimizer):
             self._gather_counts()
             at_of = places()
         counts, first = self._counts.tolist(), 0
-        for group, ps, sts, at in zip(self.param_groups, live, states, at_of):
+        for group, *own, at in zip(self.param_groups, live, grads, states, at_of):
             taken = [counts[i] for i in at]
             for k in sorted(set(taken)):
-                sel = (ps, sts, at)
+                sel = (*own, at)
                 if taken.count(k) < len(taken):
                     sel = [[x for x, c in zip(xs, taken) if c == k] for xs in sel]
-                lists = [[st.get(n) for st in sel[1]] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
-                ss = host_call("mpnn_adamw_mixed", "adamw", sel[0], [p.grad for p in sel[0]], *lists, int(k) + 1, group["lr"],
-                               group["betas"][0], group["betas"][1], group["eps"], group["weight_decay"],
-                               self.seed & 0xFFFFFFFF, first, self.max_grad_norm, parts)
+                ps, gs, sts, places_k = sel
+                lists = [[st.get(n) for st in sts] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
+                ss = host_call("mpnn_adamw_mixed", "adamw", ps, gs, *lists, int(k) + 1, group["lr"], group["betas"][0],
+                               group["betas"][1], group["eps"], group["weight_decay"], self.seed & 0xFFFFFFFF, first,
+                               self.max_grad_norm, parts)
                 self.last_grad_sumsq = ss if ss is not None else self.last_grad_sumsq
-                first += len(sel[0])
-                i, n = sel[2][0], len(sel[2])
-                if sel[2] == list(range(i, i + n)):
-                    self._counts[i:i + n] += 1
+                first += len(ps)
+                i = places_k[0]
+                if places_k == list(range(i, i + len(ps))):
+                    self._counts[i:i + len(ps)] += 1
                 else:
-                    self._counts[sel[2]] += 1
+                    self._counts[places_k] += 1
 
     def _gather_counts(self):
         """Make every parameter's `step` an element of one tensor: an operation counts for all (adding to each of 118 tensors
