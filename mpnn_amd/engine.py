@@ -31,6 +31,18 @@ def _require_device(t: torch.Tensor, name: str):
                            "the HIP path has no CPU fallback")
 
 
+def _require_batch(what, X, mask, **others):
+    """Inputs whose bare addresses go to the kernels, which would read what is elsewhere, or smaller, all the same: mask [B, L], X
+    with 12 coordinates a residue, and others like the mask, on X's device."""
+    if mask.dim() != 2 or X.shape[:2] != mask.shape or X.numel() != 12 * mask.numel():
+        raise ValueError(f"mpnn_amd.{what}: X must be [B, L, 4, 3] and mask [B, L] (got {list(X.shape)}, {list(mask.shape)})")
+    for name, t in dict(mask=mask, **others).items():
+        if t.device != X.device:
+            raise RuntimeError(f"mpnn_amd.{what}: `{name}` is on {t.device}, X on {X.device}")
+        if t.shape != mask.shape:
+            raise ValueError(f"mpnn_amd.{what}: `{name}` must be {list(mask.shape)} (got {list(t.shape)})")
+
+
 def _f32(t):
     return t.detach().to(torch.float32).contiguous()
 
@@ -949,6 +961,9 @@ def beam_search(model, X, mask, chain_M, residue_idx, chain_encoding_all, S_true
     W = int(beam_width)
     if not 1 <= W <= 64:
         raise ValueError("mpnn_amd.beam_search: beam_width must lie in 1..64")
+    _require_batch("beam_search", X, mask, residue_idx=residue_idx, chain_encoding_all=chain_encoding_all)
+    if backbone_noise is not None and (backbone_noise.shape != X.shape or backbone_noise.device != X.device):
+        raise ValueError("mpnn_amd.beam_search: backbone_noise must be like X")
     guard = numerics_guard(model, X.device)
     guard.poll()
     _lib.set_precision(getattr(model, "precision", "fp32"))

@@ -189,3 +189,25 @@ def test_nothing_designed_and_f16_and_refusals():
         other = model.beam_search(*args, beam_width=4, seed=1)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(full[k], other[k]) for k in full)
+
+
+def test_inputs_elsewhere_or_of_another_size_are_refused():
+    """Before anything is launched: the kernels take bare addresses."""
+    model = build(dict(k_neighbors=16))
+    b, args = inputs(dict(B=2, L=30, seed=4, design_fraction=1.0))
+    given = dict(X=args[0], mask=args[1], residue_idx=args[3], chain_encoding_all=args[4])
+    rest = dict(chain_M=args[2], S_true=b["S"], fix_order=model.beam_search(*args, beam_width=1)["order"], beam_width=2)
+    for name in given:
+        for bad, error in ((given[name].cpu(), RuntimeError), (given[name][:, :29], ValueError), (given[name][:1], ValueError)):
+            with pytest.raises(error):
+                model.beam_search(**{**given, name: bad}, **rest)
+    for name in ("chain_M", "S_true", "fix_order"):
+        with pytest.raises((RuntimeError, ValueError)):
+            model.beam_search(**given, **{**rest, name: rest[name].cpu()})
+        with pytest.raises((RuntimeError, ValueError)):
+            model.beam_search(**given, **{**rest, name: rest[name][:, :29]})
+    for noise in (torch.zeros(2, 29, 4, 3, device="cuda"), torch.zeros(2, 30, 4, 3)):
+        from mpnn_amd import engine
+        with pytest.raises(ValueError):
+            engine.beam_search(model, *args, beam_width=2, backbone_noise=noise)
+    assert model.beam_search(**given, **rest)["S"].shape == (2, 2, 30)
