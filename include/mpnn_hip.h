@@ -233,7 +233,8 @@ int mpnn_adamw_step(int n, float* const* params, const float* const* grads, floa
  * sumsq_parts != NULL and max_norm > 0: gradients are scaled by min(1, max_norm / (norm + 1e-6)), norm^2 = the sum of the
  * 256 doubles that mpnn_grad_sumsq_parts wrote (all of them, from any number of tensors; fp64, fixed order); grad_sumsq
  * (may be NULL) gets norm^2.  Moments are fp64 up to their rounding, the update is fp32.  step >= 1.  numel < 2^32.  No
- * two tensors may share memory, but for gradients among themselves (not checked here).  At most 32768 tensors in mpnn_grad_sumsq_parts. */
+ * two tensors may share memory, but for gradients among themselves (not checked here; optim.adamw_step does).  At most 32768
+ * tensors in mpnn_grad_sumsq_parts. */
 int mpnn_grad_sumsq_parts(int n, const float* const* grads, const long long* numel, double* parts, void* stream);
 int mpnn_adamw_mixed(int n, float* const* params, const float* const* grads, void* const* exp_avg, void* const* exp_avg_sq,
                      float* const* exp_avg_scale, float* const* exp_avg_sq_scale, const long long* numel, double lr,
@@ -787,7 +788,7 @@ typedef struct mpnn_beam_state {
  * parent outside [0, n_beams) leaves its row as it is.  With a length - length [n_groups] on the device, or length_all >= 0
  * for all groups - only the positions m with rank[b][m] < length move (rank [n_groups][n_mid]; NULL: rank = m), and n_mid
  * is the number of positions of every state; the other positions are not touched.  No two states (and no two rows of one)
- * may share memory.  At most 256 beams and 65535 groups, and 2^32 columns of a row (16 bytes where addresses, strides and run
+ * may share memory (not checked here; beam_reorder does).  At most 256 beams and 65535 groups, and 2^32 columns of a row (16 bytes where addresses, strides and run
  * are multiples of 16; one byte where they are odd). */
 int mpnn_beam_reorder(int n, const mpnn_beam_state* states, const int64_t* parent, int n_groups, int n_beams,
                       int length_all, const int32_t* length, const int32_t* rank, void* stream);

@@ -615,6 +615,8 @@ struct Logits {
   }
 };
 
+// Four waves a SIMD leave 128 registers: with U = 32 and no bias 2 of them are spilled (12 bytes of scratch a lane), 14 (60 bytes)
+// for fp16; the other instances spill none.
 template <typename T, int U, bool BIAS, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, U > 8 ? 4 : 1)
 k_select_slice(SelectArgs a, int splits, int depth, SlicePart* __restrict__ part, long long* __restrict__ pk,
@@ -1085,7 +1087,9 @@ int launch_select(const SelectArgs& a, const SelectPlan& p, void* ws, hipStream_
 // to one lane from first read to last write, so the update is in place without a barrier.  Bound by the bytes of the rows
 // that move: a row that stays is not written, one that nobody else becomes is not read.  Up to 64 beams the rows wait in
 // registers (all reads in flight at once, and more waves a CU than when they wait in LDS: 36 us against 56 for 16 structures
-// x 16 beams x 512 residues, half of them decided), beyond that in LDS.  234 us for 1.05 GB of caches of four beams.
+// x 16 beams x 512 residues, half of them decided), beyond that in LDS.  234 us for 1.05 GB of caches of four beams; of 1.6 GB of
+// rows that move 309-350 us with 16 to 64 beams (5.3 to 4.9 TB/s), but 868, 1440 and 2566 us with 65, 128 and 256: 33 to 64 KB
+// of LDS a wave leave two to four waves a CU, with eight rows of 4 or 8 bytes a lane in flight each.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int RO_MAX = 32;
 struct ReorderTable {

@@ -95,7 +95,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_
     fp32 moments; the others hold float8_e4m3fn codes and fp32 scales (see the module's docstring; zeros and ones to begin
     with).  step: 1 for the first.  seed, step, the place in the list and the element decide the rounding of 8-bit moments.
     max_grad_norm > 0 clips by the norm over all gradients.  Returns the squared norm (a device scalar) then, else None.
-    No two tensors may share memory, but for gradients among themselves.  A replayed HIP graph of this call repeats its step and its hyper-parameters."""
+    No two tensors may share memory, but for gradients among themselves.  A replayed HIP graph of this call repeats its step and
+    its hyper-parameters."""
     return host_call("mpnn_adamw_mixed", "adamw", params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step,
                      lr, betas[0], betas[1], eps, weight_decay, int(seed) & 0xFFFFFFFF, 0, max_grad_norm, None)
 
